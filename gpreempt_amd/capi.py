@@ -11,11 +11,12 @@ import numpy as np
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgpreempt_hip.so")
 
-F32, F16, BF16, I32, I64 = 0, 1, 2, 3, 4
+F32, F16, BF16, I32, I64, E4M3 = 0, 1, 2, 3, 4, 5
 ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
 MAT_AUTO, MAT_STAGED, MAT_PIPE, MAT_PIPE_SPLITK, MAT_WIDE, MAT_WIDE8 = 0, 1, 2, 3, 4, 5
 SUCC, FAIL, TIMEOUT, NOTFOUND, OUTOFRANGE, FULL = range(6)
-DTYPE_SIZE = {F32: 4, F16: 2, BF16: 2, I32: 4, I64: 8}
+ROT_HALVES, ROT_NEIGHBOURS = 0, 1
+DTYPE_SIZE = {F32: 4, F16: 2, BF16: 2, I32: 4, I64: 8, E4M3: 1}
 DTYPE_BY_NAME = {"f32": F32, "f16": F16, "bf16": BF16}
 
 vp = C.c_void_p
@@ -97,13 +98,38 @@ class EmbedParams(C.Structure):
                 ("ids", vp), ("tok", vp), ("pos", vp), ("seg", vp), ("out", vp)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int), ("pages", C.c_int),
+                ("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp)]
+
+
+_SEQUENCES = [("start", vp), ("kv_len", vp), ("page_table", vp), ("table_width", C.c_int), ("heads", C.c_int)]
+
+
+class KvAppendParams(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("cache", KvCache), ("batch", C.c_int), ("tokens", C.c_long), ("max_new", C.c_int)] + _SEQUENCES + [
+                ("q", vp), ("k", vp), ("v", vp), ("ld_qkv", C.c_long), ("q_out", vp), ("ld_q_out", C.c_long),
+                ("inv_freq", vp), ("rot_dim", C.c_int), ("rot_pairs", C.c_int)]
+
+
+class PagedAttentionParams(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("cache", KvCache), ("batch", C.c_int), ("tokens", C.c_long), ("max_new", C.c_int), ("max_len", C.c_int)] + _SEQUENCES + [
+                ("q", vp), ("ld_q", C.c_long), ("out", vp), ("ld_out", C.c_long), ("scale", C.c_float), ("causal", C.c_int),
+                ("work", vp), ("work_bytes", C.c_size_t)]
+
+
+class TokenLogprobsParams(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("rows", C.c_long), ("vocab", C.c_int), ("logits", vp), ("ld", C.c_long), ("tokens", vp), ("scale", C.c_float),
+                ("logprob", vp), ("entropy", vp), ("top", C.c_int), ("top_ids", vp), ("top_logprobs", vp), ("work", vp), ("work_bytes", C.c_size_t)]
+
+
 # every symbol include/gpreempt_hip.h declares
 SYMBOLS = """gp_init gp_last_error gp_device_info gp_device_clock gp_stream_create gp_stream_destroy gp_stream_sync
 gp_stream_exists gp_stream_capturing gp_stream_query gp_stream_priority gp_stream_set_priority gp_stream_native gp_event_create gp_event_destroy gp_event_record
 gp_event_sync gp_event_query gp_event_elapsed_ms gp_malloc gp_malloc_capturing gp_free gp_host_alloc gp_host_alloc_coherent gp_host_free gp_memcpy_h2d gp_memcpy_d2h
 gp_memcpy_h2d_async gp_memcpy_d2h_async gp_memcpy_d2d_async gp_fill32_async gp_fetch gp_stage_create gp_stage_destroy gp_stage_upload_async gp_flag_create gp_flag_destroy gp_store_word_async gp_report_stop_async gp_flag_relay_start
 gp_launch_gemm gp_gemm_ln_supported gp_launch_gemm_noalloc gp_gemm_ckpt_bytes gp_conv_ckpt_bytes gp_ckpt_reset_async gp_launch_conv2d gp_conv2d_body gp_conv2d_group_supported gp_launch_conv2d_group gp_launch_nchw_to_nhwc gp_launch_pool2d gp_launch_eltwise gp_eltwise_conv2d_supported gp_launch_eltwise_conv2d gp_launch_softmax
-gp_launch_layernorm gp_launch_attention gp_launch_miniweather gp_launch_miniweather_sweep gp_launch_graph gp_launch_graph_iter gp_graph_pack_async gp_launch_embed gp_launch_gate gp_launch_noop gp_graph_begin gp_graph_end gp_graph_launch
+gp_launch_layernorm gp_launch_attention gp_launch_miniweather gp_launch_miniweather_sweep gp_launch_graph gp_launch_graph_iter gp_graph_pack_async gp_launch_embed gp_launch_kv_append gp_paged_attention_work_bytes gp_launch_paged_attention gp_token_logprobs_work_bytes gp_launch_token_logprobs gp_launch_gate gp_launch_noop gp_graph_begin gp_graph_end gp_graph_launch
 gp_graph_destroy gp_program_create gp_program_destroy gp_program_add_gemm gp_program_add_conv2d
 gp_program_add_nchw_to_nhwc gp_program_add_pool2d gp_program_add_eltwise gp_program_add_softmax gp_program_add_layernorm
 gp_program_add_attention gp_program_add_embed gp_program_add_copy gp_program_finalize gp_program_launch gp_program_layers gp_program_read_state""".split()

@@ -45,7 +45,7 @@ inline hipStream_t native(gp_stream s) { return s ? s->s : nullptr; }
 inline size_t dtype_size(int dt) {
     switch (dt) {
         case GP_F32: return 4; case GP_F16: return 2; case GP_BF16: return 2;
-        case GP_I32: return 4; case GP_I64: return 8; default: return 0;
+        case GP_I32: return 4; case GP_I64: return 8; case GP_E4M3: return 1; default: return 0;
     }
 }
 

@@ -24,7 +24,8 @@ extern "C" {
 /* Mirrors `enum Status` of the reference (include/util/common.h:16-23). */
 enum gp_status { GP_SUCC = 0, GP_FAIL = 1, GP_TIMEOUT = 2, GP_NOTFOUND = 3, GP_OUTOFRANGE = 4, GP_FULL = 5 };
 
-enum gp_dtype { GP_F32 = 0, GP_F16 = 1, GP_BF16 = 2, GP_I32 = 3, GP_I64 = 4 };
+/* GP_E4M3 (8-bit floating point with 4 exponent and 3 mantissa bits, no infinities, largest value 448) is a type of caches only. */
+enum gp_dtype { GP_F32 = 0, GP_F16 = 1, GP_BF16 = 2, GP_I32 = 3, GP_I64 = 4, GP_E4M3 = 5 };
 enum gp_act { GP_ACT_NONE = 0, GP_ACT_RELU = 1, GP_ACT_GELU = 2 };
 /* Matrix-kernel variants: register-staged (handles B stored K x N), pipelined direct-to-LDS,
  * pipelined with K split across the four waves of a workgroup, and "wide": 16 (GP_MAT_WIDE) or 8
@@ -543,6 +544,105 @@ typedef struct gp_embed_params {
     void *out;
 } gp_embed_params;
 int gp_launch_embed(const gp_embed_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
+
+/* ---- a decoder's serving step ----------------------------------------------------------------
+ * No counterparts in the reference, whose models have no cache.  New keys and values go into a cache of pages, queries attend to
+ * what it holds, logits become log probabilities; the products in between are gp_launch_gemm.
+ *
+ * The cache: a pool of `pages` pages, each with room for page_size tokens of every head of the cache,
+ *   k, v[page][kv head][slot][head_dim]
+ * in the activations' type or, with k_scale and v_scale[page][kv head], in GP_E4M3: a value is its 8 bits times the scale of
+ * its page and head.  Scales are positive; attention takes one outside 2^-60 .. 2^60 as the nearer border.
+ * page_size 16, 32, 64 or 128; head_dim 64 or 128; k and v 16-byte aligned. */
+typedef struct gp_kv_cache {
+    int dtype;                /* GP_F16, GP_BF16 or GP_E4M3 */
+    int kv_heads, head_dim, page_size;
+    int pages;
+    void *k; void *v;
+    float *k_scale; float *v_scale; /* GP_E4M3 only */
+} gp_kv_cache;
+
+/* The sequences of a call, for both entry points that follow (device memory, read by the kernels):
+ *   start       batch + 1 row numbers: sequence b's new tokens are the rows start[b] .. start[b + 1] - 1 of q, k, v and the
+ *               outputs.  NULL: one new token per sequence, row b
+ *   kv_len      batch: tokens of each sequence in the cache, the new ones included: row start[b] + i has position
+ *               kv_len[b] - (start[b + 1] - start[b]) + i
+ *   page_table  batch x table_width page numbers: position p lies in page page_table[b][p / page_size], slot p % page_size
+ *   tokens      rows that q, k, v and the outputs have.  Rows of no sequence are neither read nor written
+ *   max_new     no sequence has more new tokens (the rows past that many of a sequence are left as they are)
+ * Whatever the arrays hold, nothing outside these bounds is touched: a token at a negative position, past the table or in a page
+ * that is not in the pool (a negative number marks one that is not there) is not stored, and is not among the keys. */
+
+/* Appends the new tokens' keys and values to the cache, the keys rotated by the angle of their position, and writes the rotated
+ * queries to q_out.  Element j of the rot_dim / 2 pairs of a head's first rot_dim values (a, b) becomes (a cos - b sin,
+ * b cos + a sin), the angle being position * inv_freq[j], multiplied in 64 bits.  rot_dim 0: no rotation; a multiple of 16 otherwise.
+ * Row t of k (v, q) for head h is k + t * ld_qkv + h * head_dim (16-byte aligned rows).  Values are rounded once, to the cache's type.
+ * GP_E4M3: a page's scale is set by the call that writes its slot 0, to the smallest power of two (2^-40 at least) that brings the
+ * largest finite magnitude of its tokens to 448 or less; a later call raises it when larger values come.  Where that changes the scale of
+ * the first page that a sequence's new tokens touch, what its other slots hold is rounded anew (nothing counts in a page whose
+ * slot 0 is written: zeros); the other slots of further pages are left as they were.  Values beyond 448 scales (infinities)
+ * become the largest, NaN stays NaN.
+ * No two positions of a call may share a page and a slot, nor, in GP_E4M3, two sequences a page that both write to.
+ * q may be NULL (no queries); q_out may be q. */
+enum gp_rot_pairs { GP_ROT_HALVES = 0 /* (j, j + rot_dim / 2) */, GP_ROT_NEIGHBOURS = 1 /* (2 j, 2 j + 1) */ };
+typedef struct gp_kv_append_params {
+    int dtype;                /* of q, k, v: GP_F16 or GP_BF16 */
+    gp_kv_cache cache;
+    int batch; long tokens; int max_new;
+    const int *start; const int *kv_len;
+    const int *page_table; int table_width;
+    int heads;                /* of q */
+    const void *q; const void *k; const void *v; long ld_qkv;
+    void *q_out; long ld_q_out;
+    const float *inv_freq; int rot_dim; int rot_pairs;
+} gp_kv_append_params;
+int gp_launch_kv_append(const gp_kv_append_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
+
+/* Attention over the cache: for every new token's row and head h
+ *   out[row, h] = sum_j softmax_j(scale * <q[row, h], k_j>) v_j
+ * over the keys and values of head h / (heads / kv_heads) of its sequence's first kv_len tokens, with `causal` those up to
+ * its own position.  A row that sees no key becomes zeros.  Not causal it is the attention of a decoder's tokens to an encoder's
+ * states in the cache.  Beyond gp_launch_attention: a cache, several query heads to one of its heads, any length, sequences of
+ * their own lengths.  max_len: no sequence is longer (what lies beyond is not among the keys); sizes the launch.
+ * Scores, softmax and sums in fp32; the probabilities are rounded to the type of q for the second product.  scale 0 counts as 1.
+ * work: gp_paged_attention_work_bytes() of device memory (0: none), zeroed before its first use (gp_fill32_async), and before the
+ * next one when a stopped launch is not resumed; a launch that has run to its end leaves it ready for the next.  Launches that may
+ * overlap need workspaces of their own. */
+typedef struct gp_paged_attention_params {
+    int dtype;                /* of q and out: GP_F16 or GP_BF16 */
+    gp_kv_cache cache;
+    int batch; long tokens; int max_new; int max_len;
+    const int *start; const int *kv_len;
+    const int *page_table; int table_width;
+    int heads;
+    const void *q; long ld_q;
+    void *out; long ld_out;
+    float scale; int causal;
+    void *work; size_t work_bytes;
+} gp_paged_attention_params;
+int gp_paged_attention_work_bytes(const gp_paged_attention_params *p, size_t *bytes);
+int gp_launch_paged_attention(const gp_paged_attention_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
+
+/* Log probabilities under p = softmax(scale * logits[row]): for every row that of a given token, the entropy
+ * (in nats), and the `top` (0 .. 32) largest with their token numbers, the lower number first among equals.
+ * logprob, entropy, top_ids + top_logprobs may be NULL (not all).  A token number outside 0 .. vocab - 1 (padding) gets 0.
+ * Logits of -infinity have probability 0 and are no alternatives: where fewer than `top` are left, and for a row that has nothing else, the number is
+ * -1 and the log probability -infinity; such an empty row has logprob -infinity and entropy 0.  A NaN or +infinity makes its row's log
+ * probabilities and entropy NaN (NaN is no alternative either).  scale (one over the temperature): finite, positive; 0 counts as 1.
+ * ld: elements from one row to the next.  work: as gp_paged_attention_params::work, of gp_token_logprobs_work_bytes(). */
+typedef struct gp_token_logprobs_params {
+    int dtype;                /* of the logits: GP_F32, GP_F16 or GP_BF16 */
+    long rows; int vocab;
+    const void *logits; long ld;
+    const int64_t *tokens;    /* rows; needed by logprob */
+    float scale;
+    float *logprob; float *entropy;  /* rows */
+    int top;
+    int *top_ids; float *top_logprobs; /* rows x top */
+    void *work; size_t work_bytes;
+} gp_token_logprobs_params;
+int gp_token_logprobs_work_bytes(const gp_token_logprobs_params *p, size_t *bytes);
+int gp_launch_token_logprobs(const gp_token_logprobs_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
 
 /* ---- whole-model program -------------------------------------------------------------------
  * The launch-bound inner loop of the reference (one GPULaunchKernel or graph node per kernel,
