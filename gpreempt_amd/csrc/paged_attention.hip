@@ -1,97 +1,51 @@
 // Attention of a batch of sequences' new tokens over the pages of a cache.
 #include <algorithm>
-#include "kv_cache.hpp"
+#include "paged_few.hpp"
 #include "launch_tiles.hpp"
 
 namespace gp {
 
-constexpr int PA_NT = 256;
-
-struct PagedArgs {
-    gp_paged_attention_params p;
-    int group;  // query heads to a head of the cache
+struct PagedPlan {
+    FewArgs few;
+    int nt;             // query rows of a tile, in sixteens
+    long tiles_y;
+    size_t work_bytes;
 };
 
-// the scale of a page's head, within the bounds that the header names
-__device__ __forceinline__ float page_scale(const float *scales, long at) { return fminf(fmaxf(scales[at], 0x1p-60f), 0x1p60f); }
-
-// One query of one head per tile: 256 keys at a time, one to a thread; then a thread to every value of the head.
-template <typename T, int D, bool E8>
-__device__ __forceinline__ void attend_tile(const PagedArgs &a, TileIdx t, float *lds) {
-    const gp_paged_attention_params &p = a.p;
-    float *q = lds, *w = q + D, *red = w + PA_NT;
-    const int head = t.x, i = t.y % p.max_new, b = t.y / p.max_new, tid = threadIdx.x, P = p.cache.page_size, kvh = head / a.group;
-    const SeqTokens s = seq_tokens(p.start, p.kv_len, b, p.tokens, p.max_new);
-    if (i >= s.rows) return;
-    const long bound = seq_bound(s, p.max_len, p.table_width, P), seen = keys_seen(bound, s.first + i, p.causal);
-    const T *qrow = (const T *)p.q + (s.row0 + i) * p.ld_q + (long)head * D;
-    __syncthreads();
-    if (tid < D) q[tid] = Elem<T>::to_f(qrow[tid]);
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (long k0 = 0; k0 < seen; k0 += PA_NT) {
-        const long key = k0 + tid;
-        const int page = key < seen ? page_of(p.page_table, p.table_width, b, key / P, p.cache.pages) : -1;
-        float x = -INFINITY;
-        if (page >= 0) {
-            const long at = (((long)page * p.cache.kv_heads + kvh) * P + key % P) * D;
-            float dot = 0.f;
-            for (int d = 0; d < D; d += 8) {
-                float y[8];
-                if constexpr (E8) unpack_e4m3(*(const u32x2 *)((const unsigned char *)p.cache.k + at + d), y);
-                else for (int e = 0; e < 8; ++e) y[e] = Elem<T>::to_f(((const T *)p.cache.k)[at + d + e]);
-                for (int e = 0; e < 8; ++e) dot = fmaf(q[d + e], y[e], dot);
-            }
-            if constexpr (E8) dot *= page_scale(p.cache.k_scale, (long)page * p.cache.kv_heads + kvh);
-            x = dot * p.scale;
-        }
-        red[tid] = x;
-        __syncthreads();
-        float mm = m;
-        for (int e = 0; e < PA_NT; ++e) mm = fmaxf(mm, red[e]);
-        const float base = mm == -INFINITY ? 0.f : mm, f = expf(m - base);
-        w[tid] = page < 0 ? 0.f : expf(x - base);
-        __syncthreads();
-        float sum = 0.f;
-        for (int e = 0; e < PA_NT; ++e) sum += w[e];
-        l = l * f + sum;
-        if (tid < D) {
-            o *= f;
-            for (int e = 0; e < PA_NT && k0 + e < seen; ++e) {
-                const int pg = page_of(p.page_table, p.table_width, b, (k0 + e) / P, p.cache.pages);
-                if (pg < 0) continue;
-                const long hd = (long)pg * p.cache.kv_heads + kvh, at = (hd * P + (k0 + e) % P) * D + tid;
-                float v;
-                if constexpr (E8) v = __builtin_amdgcn_cvt_pk_f32_fp8(((const unsigned char *)p.cache.v)[at], false)[0] * page_scale(p.cache.v_scale, hd);
-                else v = Elem<T>::to_f(((const T *)p.cache.v)[at]);
-                o = fmaf(w[e], v, o);
-            }
-        }
-        m = mm;
-        __syncthreads();
-    }
-    if (tid < D) ((T *)p.out)[(s.row0 + i) * p.ld_out + (long)head * D + tid] = Elem<T>::from_f(l == 0.f ? 0.f : o / l);
-}
-
-template <typename T, int D, bool E8, int LOOP = LOOP_ANY>
-__global__ __launch_bounds__(PA_NT) void paged_attention_kernel(PagedArgs a, BlpArgs blp) {
-    __shared__ float lds[D + 2 * PA_NT];
-    tiles<LOOP>(blp, [&](TileIdx t) { attend_tile<T, D, E8>(a, t, lds); });
-}
-
-static int check_paged_attention(const gp_paged_attention_params *p, PagedArgs *a) {
+static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *pl) {
     GP_REQUIRE(p && p->kv_len && p->page_table && p->q && p->out, "null paged_attention params");
     if (int rc = check_kv_cache(p->cache, p->dtype, "paged_attention")) return rc;
     GP_REQUIRE(p->batch > 0 && p->tokens > 0 && p->max_new > 0 && p->max_len > 0 && p->table_width > 0, "paged_attention: batch, tokens, max_new, max_len and table_width must be positive");
+    GP_REQUIRE(p->max_len <= (1 << 30), "paged_attention: max_len must be at most 2^30");
     GP_REQUIRE(p->start || p->tokens >= p->batch, "paged_attention: one new token per sequence needs a row for each");
     GP_REQUIRE(p->heads > 0 && p->heads % p->cache.kv_heads == 0, "paged_attention: heads must be a multiple of the cache's");
     const long cols = (long)p->heads * p->cache.head_dim;
     GP_REQUIRE(p->ld_q % 8 == 0 && p->ld_out % 8 == 0 && p->ld_q >= cols && p->ld_out >= cols, "paged_attention: row strides must be multiples of 8 elements that hold the heads");
     GP_REQUIRE(aligned16(p->q) && aligned16(p->out), "paged_attention: 16-byte alignment");
-    *a = PagedArgs{*p, p->heads / p->cache.kv_heads};
-    if (!p->start) a->p.max_new = 1;
-    if (a->p.scale == 0.f) a->p.scale = 1.f;
-    GP_REQUIRE((long)p->batch * a->p.max_new < (1L << 31) && (long)p->batch * a->p.max_new * p->heads < (1L << 31), "paged_attention: too large");
+    *pl = PagedPlan{};
+    FewArgs &a = pl->few;
+    a.p = *p;
+    a.group = p->heads / p->cache.kv_heads;
+    if (!p->start) a.p.max_new = 1;
+    if (a.p.scale == 0.f) a.p.scale = 1.f;
+    const long rows = (long)a.p.max_new * a.group;
+    GP_REQUIRE(rows < (1L << 30), "paged_attention: too large");
+    pl->nt = rows <= 16 ? 1 : 2;
+    const long blocks = (rows + 16 * pl->nt - 1) / (16 * pl->nt), heads = blocks * p->cache.kv_heads, units = heads * p->batch;
+    GP_REQUIRE(units < (1L << 30), "paged_attention: too large");
+    a.row_blocks = (int)blocks;
+    // a sequence's keys are cut into stretches until there are four tiles per compute unit, of 256 keys at least
+    const long want = std::max(1l, std::min(4l * device_cus() / units, (p->max_len + 255l) / 256));
+    a.chunk = (int)(((p->max_len + want - 1) / want + 255) / 256 * 256);
+    a.splits = (p->max_len + a.chunk - 1) / a.chunk;
+    pl->tiles_y = heads * a.splits;
+    GP_REQUIRE(pl->tiles_y * p->batch < (1L << 31), "paged_attention: too large");
+    if (a.splits > 1) {
+        const size_t counters = ((size_t)units * sizeof(int) + 255) / 256 * 256;
+        pl->work_bytes = counters + (size_t)units * a.splits * 16 * pl->nt * (p->cache.head_dim + 2) * sizeof(float);
+        a.arrived = (int *)p->work;
+        a.partial = (float *)((char *)p->work + counters);
+    }
     return GP_SUCC;
 }
 
@@ -100,25 +54,26 @@ static int check_paged_attention(const gp_paged_attention_params *p, PagedArgs *
 using namespace gp;
 
 extern "C" int gp_paged_attention_work_bytes(const gp_paged_attention_params *p, size_t *bytes) {
-    PagedArgs a;
-    if (int rc = check_paged_attention(p, &a)) return rc;
+    PagedPlan pl;
+    if (int rc = plan_paged_attention(p, &pl)) return rc;
     GP_REQUIRE(bytes, "paged_attention: no place for the size");
-    *bytes = 0;
+    *bytes = pl.work_bytes;
     return GP_SUCC;
 }
 
 extern "C" int gp_launch_paged_attention(const gp_paged_attention_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
-    PagedArgs a;
-    if (int rc = check_paged_attention(p, &a)) return rc;
+    PagedPlan pl;
+    if (int rc = plan_paged_attention(p, &pl)) return rc;
+    GP_REQUIRE(pl.work_bytes == 0 || (p->work && aligned16(p->work) && p->work_bytes >= pl.work_bytes), "paged_attention: needs a workspace of %zu bytes, 16-byte aligned", pl.work_bytes);
     const bool e8 = p->cache.dtype == GP_E4M3, f16 = p->dtype == GP_F16;
-#define GP_PAGED(T, D, E8) return launch_tiles(GP_KSET(paged_attention_kernel<T, D, E8), p->heads, p->batch * a.p.max_new, ctx, s, info, a, 0, 1, PA_NT)
-    if (p->cache.head_dim == 128) {
-        if (f16) { if (e8) GP_PAGED(_Float16, 128, true); GP_PAGED(_Float16, 128, false); }
-        if (e8) GP_PAGED(__bf16, 128, true);
-        GP_PAGED(__bf16, 128, false);
+    const int key = p->cache.head_dim * 8 + e8 * 4 + f16 * 2 + (pl.nt == 2);
+    switch (key) {
+#define GP_FEW(T, F16, D, E8, NT) case D * 8 + E8 * 4 + F16 * 2 + (NT == 2): return launch_tiles(GP_KSET(paged_few_kernel<T, D, E8, NT), p->batch, (int)pl.tiles_y, ctx, s, info, pl.few, few_lds_bytes<NT, D>(), 1, FEW_NT);
+#define GP_FEW_BOTH(D, E8, NT) GP_FEW(_Float16, 1, D, E8, NT) GP_FEW(__bf16, 0, D, E8, NT)
+        GP_FEW_BOTH(64, 0, 1) GP_FEW_BOTH(64, 0, 2) GP_FEW_BOTH(64, 1, 1) GP_FEW_BOTH(64, 1, 2)
+        GP_FEW_BOTH(128, 0, 1) GP_FEW_BOTH(128, 0, 2) GP_FEW_BOTH(128, 1, 1) GP_FEW_BOTH(128, 1, 2)
+#undef GP_FEW_BOTH
+#undef GP_FEW
     }
-    if (f16) { if (e8) GP_PAGED(_Float16, 64, true); GP_PAGED(_Float16, 64, false); }
-    if (e8) GP_PAGED(__bf16, 64, true);
-    GP_PAGED(__bf16, 64, false);
-#undef GP_PAGED
+    return GP_OUTOFRANGE;
 }

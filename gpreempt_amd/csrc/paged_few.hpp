@@ -1,0 +1,363 @@
+// Attention over a paged cache for few query rows: a step of a decoder, where the cache is read once and its arithmetic is little.
+//
+// A tile is one head of the cache, up to 16 * NT query rows that share it (a sequence's new tokens times the query heads of the head),
+// and a stretch of the sequence's keys.  Bound by memory: 2 * D values of the cache per key.  So keys and values go from memory to the registers that
+// the matrix instructions read, without LDS and without a barrier; the four wavefronts of a workgroup take turns over the stretch, each with a running
+// maximum and sum of its own, and meet at its end.
+//
+//   S^T = K Q^T    v_mfma_f32_16x16x32, K as A: lane l holds 8 values of key l % 16.  Which of the head's values a lane holds is free as long as the
+//                  queries are laid out alike: 16 consecutive bytes of a key per lane and load.
+//   O^T = V^T P^T  V^T as A, and P as B in the layout that S^T came out in: lane l has keys 4 * (l / 16) + 0..3 of two neighbouring tiles of
+//                  16.  So lane l loads these eight rows of V, D / 16 consecutive values from (D / 16) * (l % 16) on, and a few byte permutations turn
+//                  them into eight (four) A operands whose row l % 16 is the head's value (D / 16) * (l % 16) + j.
+#pragma once
+#include "kv_cache.hpp"
+#include "tile_loop.hpp"
+
+namespace gp {
+
+constexpr int FEW_NT = 256, FEW_WAVES = 4;
+constexpr int FEW_SPAN = 4096;  // keys for which a wavefront's lanes hold the pages and scales: 64 tiles of 16 for each of four
+
+struct FewArgs {
+    gp_paged_attention_params p;
+    int group;        // query heads to a head of the cache
+    int row_blocks;   // of 16 * NT rows
+    int splits;       // stretches of `chunk` keys per sequence, at most
+    int chunk;
+    int *arrived;     // workspace: a counter for every (sequence, head, row block), 0 between launches
+    float *partial;   // ... and for every tile 16 * NT rows of D values, then their maxima and sums
+};
+
+template <int NT, int D> constexpr int few_partial_floats() { return 16 * NT * (D + 2); }
+template <int NT, int D> constexpr size_t few_lds_bytes() { return (size_t)FEW_WAVES * 16 * NT * (D + 4 + 2) * sizeof(float); }
+
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c, _Float16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c, __bf16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+// two e4m3 values (bytes 0 and 1, or 2 and 3) in 16 bits: exact in either type
+template <bool HI> __device__ __forceinline__ unsigned widen(unsigned raw, _Float16) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw, 1.f, HI)); }
+template <bool HI> __device__ __forceinline__ unsigned widen(unsigned raw, __bf16) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw, 1.f, HI)); }
+
+// the scale of a page's head, within the bounds that the header names
+__device__ __forceinline__ float page_scale(const float *scales, long at) { return fminf(fmaxf(scales[at], 0x1p-60f), 0x1p60f); }
+
+// stores and loads of what another workgroup reads or has written within the launch
+__device__ __forceinline__ void put_shared(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float get_shared(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+template <typename T, int D, bool E8, int NT>
+__device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *lds) {
+    const gp_paged_attention_params &p = a.p;
+    constexpr int KS = E8 ? 64 : 32, TILES = KS / 16, PAIRS = KS / 32;  // keys of a wavefront's step
+    constexpr int ROWS = 16 * NT, VD = D / 16, KL = E8 ? D / 64 : D / 32;
+    constexpr int ES = E8 ? 1 : 2;  // bytes of a value
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
+    const int b = t.x, split = t.y % a.splits, hr = t.y / a.splits, rb = hr % a.row_blocks, kvh = hr / a.row_blocks, P = p.cache.page_size;
+    const SeqTokens s = seq_tokens(p.start, p.kv_len, b, p.tokens, p.max_new);
+    const int nrows = s.rows * a.group - rb * ROWS;  // of this block
+    if (nrows <= 0) return;
+    const int bound = (int)seq_bound(s, p.max_len, p.table_width, P);
+    const int last_token = (rb * ROWS + (nrows < ROWS ? nrows : ROWS) - 1) / a.group, first_token = rb * ROWS / a.group;
+    const int kend_all = (int)keys_seen(bound, s.first + last_token, p.causal), kmin = (int)keys_seen(bound, s.first + first_token, p.causal);
+    const int nsplits = kend_all <= a.chunk ? 1 : (kend_all + a.chunk - 1) / a.chunk;
+    if (split >= nsplits) return;
+    const int c0 = split * a.chunk, kend = c0 + a.chunk < kend_all ? c0 + a.chunk : kend_all;
+
+    // ---- queries: column l % 16 of tile n, in the order of values that the keys are loaded in ----
+    u32x4 q[NT][D / 32];
+    int seen[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = rb * ROWS + n * 16 + col, token = r / a.group, hg = r - token * a.group;
+        const bool there = n * 16 + col < nrows;
+        seen[n] = there ? (int)keys_seen(bound, s.first + token, p.causal) : 0;
+        const T *row = (const T *)p.q + (s.row0 + (there ? token : 0)) * p.ld_q + ((long)kvh * a.group + (there ? hg : 0)) * D;
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+            const int d = E8 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 32 * k + 8 * g;
+            q[n][k] = *(const u32x4 *)(row + d);
+            if (!there) q[n][k] = u32x4{0, 0, 0, 0};
+        }
+    }
+    f32x4 o[NT][VD];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        m[n] = -INFINITY; l[n] = 0.f;
+#pragma unroll
+        for (int j = 0; j < VD; ++j) o[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float scale2 = p.scale * 1.44269504088896340736f;  // log2(e): exponentials are powers of two
+    const char *K = (const char *)p.cache.k, *V = (const char *)p.cache.v;
+    const unsigned koff = (unsigned)(col * D + (E8 ? 16 : 8) * g) * ES, voff = (unsigned)(4 * g * D + VD * col) * ES;
+
+    for (int base = c0; base < kend; base += FEW_SPAN) {
+        // lane i: the page and the scales of the i-th tile of 16 keys that this wavefront takes
+        const int key_of_lane = base + ((lane / TILES) * FEW_WAVES + wave) * KS + lane % TILES * 16;
+        const int page_l = key_of_lane < kend ? page_of(p.page_table, p.table_width, b, key_of_lane / P, p.cache.pages) : -1;
+        float ks_l = scale2, vs_l = 1.f, lv_l = 0.f;
+        if constexpr (E8) {
+            if (page_l >= 0) {
+                const long at = (long)page_l * p.cache.kv_heads + kvh;
+                ks_l = scale2 * page_scale(p.cache.k_scale, at);
+                vs_l = page_scale(p.cache.v_scale, at);
+            }
+            lv_l = __builtin_amdgcn_logf(vs_l);
+            vs_l = 1.f / vs_l;
+        }
+        const int left = (kend - base < FEW_SPAN ? kend - base : FEW_SPAN) - wave * KS;
+        const int steps = left <= 0 ? 0 : (left + FEW_WAVES * KS - 1) / (FEW_WAVES * KS);
+        u32x4 kr[TILES][KL];
+        u32x4 vr[PAIRS][8];
+        auto tile_at = [&](int step, int i) -> long {  // byte offset of the i-th tile of a step in the pool (one that is not there: page 0)
+            const int at = step * TILES + i, page = __builtin_amdgcn_readlane(page_l, at);
+            const int key = base + (step * FEW_WAVES + wave) * KS + i * 16;
+            return (((long)(page < 0 ? 0 : page) * p.cache.kv_heads + kvh) * P + (key & (P - 1))) * D * ES;
+        };
+        auto load_k = [&](int step) {
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) {
+                const char *at = K + tile_at(step, i);
+#pragma unroll
+                for (int k = 0; k < KL; ++k) kr[i][k] = *(const u32x4 *)(at + koff + k * 64);
+            }
+        };
+        auto load_v = [&](int step) {
+#pragma unroll
+            for (int pr = 0; pr < PAIRS; ++pr)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const char *at = V + tile_at(step, 2 * pr + h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const char *from = at + voff + e * D * ES;
+                        u32x4 x = {0, 0, 0, 0};
+                        if constexpr (VD * ES == 16) x = *(const u32x4 *)from;
+                        else if constexpr (VD * ES == 8) { const u32x2 y = *(const u32x2 *)from; x[0] = y[0]; x[1] = y[1]; }
+                        else x[0] = *(const unsigned *)from;
+                        vr[pr][4 * h + e] = x;
+                    }
+                }
+        };
+        if (steps > 0) { load_k(0); load_v(0); }
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+            // ---- scores of 16 keys at a time: x[n][i][e] belongs to key 4 g + e of tile i and query l % 16 ----
+            f32x4 x[NT][TILES];
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) x[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KL; ++k) {
+                    if constexpr (E8) {
+                        const u32x4 r = kr[i][k];
+                        const u32x4 k0 = {widen<false>(r[0], T()), widen<true>(r[0], T()), widen<false>(r[1], T()), widen<true>(r[1], T())};
+                        const u32x4 k1 = {widen<false>(r[2], T()), widen<true>(r[2], T()), widen<false>(r[3], T()), widen<true>(r[3], T())};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            x[n][i] = mma16(k0, q[n][2 * k], x[n][i], T());
+                            x[n][i] = mma16(k1, q[n][2 * k + 1], x[n][i], T());
+                        }
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) x[n][i] = mma16(kr[i][k], q[n][k], x[n][i], T());
+                    }
+                }
+            }
+            if (step + 1 < steps) load_k(step + 1);
+            // ---- masks: the keys behind a row's last, tiles that are not there, and (once for all rows) what is behind the sequence's end ----
+            const int key0 = base + (step * FEW_WAVES + wave) * KS;
+            float ks[TILES], lv[TILES], iv[TILES];
+            bool whole = key0 + KS <= kmin && key0 + KS <= kend;
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) {
+                const int at = step * TILES + i;
+                whole = whole && __builtin_amdgcn_readlane(page_l, at) >= 0;
+                ks[i] = E8 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks_l), at)) : scale2;
+                lv[i] = E8 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lv_l), at)) : 0.f;
+                iv[i] = E8 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs_l), at)) : 1.f;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][i][e] = E8 ? fmaf(x[n][i][e], ks[i], lv[i]) : x[n][i][e] * ks[i];
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {
+                    const int first = key0 + i * 16;
+                    int lim = __builtin_amdgcn_readlane(page_l, step * TILES + i) < 0 ? 0 : kend;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = first + 4 * g + e;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            if (key >= lim || key >= seen[n]) x[n][i][e] = -INFINITY;
+                        if (key >= lim) vr[i / 2][4 * (i % 2) + e] = u32x4{0, 0, 0, 0};
+                    }
+                }
+            }
+            // ---- running maximum and sum.  8 bits: x has the logarithm of the values' scale added, so that what is rounded to 16
+            // bits is the probability times that scale, at most 1; the sum takes the scale back out ----
+            u32x4 pb[NT][PAIRS];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float top = x[n][0][0];
+#pragma unroll
+                for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, x[n][i][e]);
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                if (__any(top > m[n])) {
+                    const float now = fmaxf(m[n], top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[n] - now);
+                    m[n] = now;
+                    l[n] *= f;
+#pragma unroll
+                    for (int j = 0; j < VD; ++j) o[n][j] *= f;
+                }
+                const float mm = m[n] == -INFINITY ? 0.f : m[n];
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {
+                    float part = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[n][i][e] = __builtin_amdgcn_exp2f(x[n][i][e] - mm);
+                        part += x[n][i][e];
+                    }
+                    l[n] = E8 ? fmaf(part, iv[i], l[n]) : l[n] + part;
+                }
+#pragma unroll
+                for (int pr = 0; pr < PAIRS; ++pr) {
+                    typedef T tx8 __attribute__((ext_vector_type(8)));
+                    tx8 y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { y[e] = Elem<T>::from_f(x[n][2 * pr][e]); y[4 + e] = Elem<T>::from_f(x[n][2 * pr + 1][e]); }
+                    pb[n][pr] = __builtin_bit_cast(u32x4, y);
+                }
+            }
+            // ---- O^T += V^T P^T ----
+#pragma unroll
+            for (int pr = 0; pr < PAIRS; ++pr)
+#pragma unroll
+                for (int j = 0; j < VD; j += 2) {
+                    u32x4 v0, v1;  // of the lane's values j and j + 1, eight keys each
+#pragma unroll
+                    for (int kp = 0; kp < 4; ++kp) {
+                        if constexpr (E8) {
+                            // bytes j of two keys, then bytes j + 1
+                            const unsigned two = __builtin_amdgcn_perm(vr[pr][2 * kp + 1][j / 4], vr[pr][2 * kp][j / 4], j % 4 == 0 ? 0x05010400u : 0x07030602u);
+                            v0[kp] = widen<false>(two, T());
+                            v1[kp] = widen<true>(two, T());
+                        } else {
+                            v0[kp] = __builtin_amdgcn_perm(vr[pr][2 * kp + 1][j / 2], vr[pr][2 * kp][j / 2], 0x05040100u);
+                            v1[kp] = __builtin_amdgcn_perm(vr[pr][2 * kp + 1][j / 2], vr[pr][2 * kp][j / 2], 0x07060302u);
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        o[n][j] = mma16(v0, pb[n][pr], o[n][j], T());
+                        o[n][j + 1] = mma16(v1, pb[n][pr], o[n][j + 1], T());
+                    }
+                }
+            if (step + 1 < steps) load_v(step + 1);
+        }
+    }
+
+    // ---- the four wavefronts' results meet: O = sum_w a_w O_w, a_w = 2^(m_w - max m) ----
+    constexpr int LD = D + 4;
+    float *ml = lds + FEW_WAVES * ROWS * LD;
+    __syncthreads();  // (the previous tile's are still being read)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        l[n] += __shfl_xor(l[n], 16, 64);
+        l[n] += __shfl_xor(l[n], 32, 64);
+        const int r = n * 16 + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < VD; j += 4)
+                *(f32x4 *)(lds + (wave * ROWS + r) * LD + (4 * g + e) * VD + j) = f32x4{o[n][j][e], o[n][j + 1][e], o[n][j + 2][e], o[n][j + 3][e]};
+        if (g == 0) *(f32x2 *)(ml + 2 * (wave * ROWS + r)) = f32x2{m[n], l[n]};
+    }
+    __syncthreads();
+    const int rows = nrows < ROWS ? nrows : ROWS;
+    auto finish = [&](int r, int d, f32x4 v, float sum) {
+        const int rr = rb * ROWS + r, token = rr / a.group, hg = rr - token * a.group;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        typedef T tx4 __attribute__((ext_vector_type(4)));
+        tx4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f(v[e] * inv);
+        *(tx4 *)((T *)p.out + (s.row0 + token) * p.ld_out + ((long)kvh * a.group + hg) * D + d) = y;
+    };
+    float *mine = a.partial + (((long)hr * p.batch + b) * a.splits + split) * few_partial_floats<NT, D>();
+    for (int u = tid; u < rows * (D / 4); u += FEW_NT) {
+        const int r = u / (D / 4), d = u % (D / 4) * 4;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; ++w) top = fmaxf(top, ml[2 * (w * ROWS + r)]);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; ++w) {
+            const f32x2 x = *(const f32x2 *)(ml + 2 * (w * ROWS + r));
+            const float f = x[0] == -INFINITY ? (x[1] == 0.f ? 0.f : x[1]) : __builtin_amdgcn_exp2f(x[0] - top);
+            sum += f * x[1];
+            const f32x4 y = *(const f32x4 *)(lds + (w * ROWS + r) * LD + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = x[1] == 0.f ? v[e] : fmaf(f, y[e], v[e]);
+        }
+        if (nsplits == 1) finish(r, d, v, sum);
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) put_shared(mine + r * D + d + e, v[e]);
+            if (d == 0) { put_shared(mine + ROWS * D + 2 * r, top); put_shared(mine + ROWS * D + 2 * r + 1, sum); }
+        }
+    }
+    if (nsplits == 1) return;
+    // ---- whoever comes last joins the stretches, in their order ----
+    __shared__ int came;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above have reached the memory that all XCDs see
+    __syncthreads();
+    int *arrived = a.arrived + (long)hr * p.batch + b;
+    if (tid == 0) came = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (came != nsplits - 1) return;
+    if (tid == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const float *all = a.partial + ((long)hr * p.batch + b) * a.splits * few_partial_floats<NT, D>();
+    for (int u = tid; u < rows * (D / 4); u += FEW_NT) {
+        const int r = u / (D / 4), d = u % (D / 4) * 4;
+        float top = -INFINITY, sum = 0.f;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < nsplits; ++i) {
+            const float *x = all + (long)i * few_partial_floats<NT, D>();
+            const float mi = get_shared(x + ROWS * D + 2 * r), si = get_shared(x + ROWS * D + 2 * r + 1);
+            f32x4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = get_shared(x + r * D + d + e);
+            if (si == 0.f) continue;
+            const float now = fmaxf(top, mi), fo = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now), fi = mi == -INFINITY ? si : __builtin_amdgcn_exp2f(mi - now);
+            top = now;
+            sum = sum * fo + si * fi;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = v[e] * fo + y[e] * fi;
+        }
+        finish(r, d, v, sum);
+    }
+}
+
+template <typename T, int D, bool E8, int NT, int LOOP = LOOP_ANY>
+__global__ __launch_bounds__(FEW_NT, 2) void paged_few_kernel(FewArgs a, BlpArgs blp) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char few_lds[];
+    tiles<LOOP>(blp, [&](TileIdx t) { attend_few<T, D, E8, NT>(a, t, (float *)few_lds); });
+}
+
+}  // namespace gp
