@@ -8,7 +8,7 @@ namespace gp {
 struct PagedPlan {
     FewArgs few;
     int nt;             // query rows of a tile, in sixteens
-    long tiles_y;
+    int tiles_x; long tiles_y;
     size_t work_bytes;
 };
 
@@ -34,18 +34,22 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
     const long blocks = (rows + 16 * pl->nt - 1) / (16 * pl->nt), heads = blocks * p->cache.kv_heads, units = heads * p->batch;
     GP_REQUIRE(units < (1L << 30), "paged_attention: too large");
     a.row_blocks = (int)blocks;
-    // a sequence's keys are cut into stretches until there are four tiles per compute unit, of 256 keys at least
-    const long want = std::max(1l, std::min(4l * device_cus() / units, (p->max_len + 255l) / 256));
-    a.chunk = (int)(((p->max_len + want - 1) / want + 255) / 256 * 256);
-    a.splits = (p->max_len + a.chunk - 1) / a.chunk;
-    pl->tiles_y = heads * a.splits;
-    GP_REQUIRE(pl->tiles_y * p->batch < (1L << 31), "paged_attention: too large");
-    if (a.splits > 1) {
+    // Short sequences get a tile each.  The keys of longer ones are dealt out in equal parts, one per compute unit: 64 sequences of 2048 to 8192 keys (8 heads
+    // of 128, e4m3) 108 us, with tiles of 2816 keys of one sequence 119; one sequence of 131072 keys 50 us, with two or four parts per compute unit 56 and
+    // 68 (whoever comes last has more to join).
+    const int unit = p->cache.dtype == GP_E4M3 ? few_unit<true>() : few_unit<false>();
+    const long most = (p->max_len + unit - 1l) / unit;
+    GP_REQUIRE(most * p->batch < (1L << 31), "paged_attention: too large");
+    pl->tiles_x = p->batch;
+    pl->tiles_y = heads;
+    if (most > 4) {
+        pl->tiles_x = a.shares = (int)std::min((device_cus() + heads - 1) / heads, most * p->batch);
         const size_t counters = ((size_t)units * sizeof(int) + 255) / 256 * 256;
-        pl->work_bytes = counters + (size_t)units * a.splits * 16 * pl->nt * (p->cache.head_dim + 2) * sizeof(float);
+        pl->work_bytes = counters + (size_t)heads * a.shares * 2 * 16 * pl->nt * (p->cache.head_dim + 2) * sizeof(float);
         a.arrived = (int *)p->work;
         a.partial = (float *)((char *)p->work + counters);
     }
+    GP_REQUIRE(heads * pl->tiles_x < (1L << 31), "paged_attention: too large");
     return GP_SUCC;
 }
 
@@ -68,7 +72,7 @@ extern "C" int gp_launch_paged_attention(const gp_paged_attention_params *p, con
     const bool e8 = p->cache.dtype == GP_E4M3, f16 = p->dtype == GP_F16;
     const int key = p->cache.head_dim * 8 + e8 * 4 + f16 * 2 + (pl.nt == 2);
     switch (key) {
-#define GP_FEW(T, F16, D, E8, NT) case D * 8 + E8 * 4 + F16 * 2 + (NT == 2): return launch_tiles(GP_KSET(paged_few_kernel<T, D, E8, NT), p->batch, (int)pl.tiles_y, ctx, s, info, pl.few, few_lds_bytes<NT, D>(), 1, FEW_NT);
+#define GP_FEW(T, F16, D, E8, NT) case D * 8 + E8 * 4 + F16 * 2 + (NT == 2): return launch_tiles(GP_KSET(paged_few_kernel<T, D, E8, NT), pl.tiles_x, (int)pl.tiles_y, ctx, s, info, pl.few, few_lds_floats<NT, D>() * sizeof(float), 1, FEW_NT);
 #define GP_FEW_BOTH(D, E8, NT) GP_FEW(_Float16, 1, D, E8, NT) GP_FEW(__bf16, 0, D, E8, NT)
         GP_FEW_BOTH(64, 0, 1) GP_FEW_BOTH(64, 0, 2) GP_FEW_BOTH(64, 1, 1) GP_FEW_BOTH(64, 1, 2)
         GP_FEW_BOTH(128, 0, 1) GP_FEW_BOTH(128, 0, 2) GP_FEW_BOTH(128, 1, 1) GP_FEW_BOTH(128, 1, 2)

@@ -1,9 +1,12 @@
 // Attention over a paged cache for few query rows: a step of a decoder, where the cache is read once and its arithmetic is little.
 //
-// A tile is one head of the cache, up to 16 * NT query rows that share it (a sequence's new tokens times the query heads of the head),
-// and a stretch of the sequence's keys.  Bound by memory: 2 * D values of the cache per key.  So keys and values go from memory to the registers that
-// the matrix instructions read, without LDS and without a barrier; the four wavefronts of a workgroup take turns over the stretch, each with a running
+// Bound by memory: 2 * D values of the cache per key.  So keys and values go from memory to the registers that the matrix instructions
+// read, without LDS and without a barrier; the four wavefronts of a workgroup take turns over a stretch of keys, each with a running
 // maximum and sum of its own, and meet at its end.
+//
+// A tile is one head of the cache, up to 16 * NT query rows of a sequence that share it (its new tokens times the query heads of the
+// head), and one of `shares` equal parts of the keys of all sequences, one sequence behind the other: how long they are only the device knows,
+// and a part that ends inside a sequence leaves a result to be joined with its neighbours', by whoever of them comes last.
 //
 //   S^T = K Q^T    v_mfma_f32_16x16x32, K as A: lane l holds 8 values of key l % 16.  Which of the head's values a lane holds is free as long as the
 //                  queries are laid out alike: 16 consecutive bytes of a key per lane and load.
@@ -16,21 +19,22 @@
 
 namespace gp {
 
-constexpr int FEW_NT = 256, FEW_WAVES = 4;
-constexpr int FEW_SPAN = 4096;  // keys for which a wavefront's lanes hold the pages and scales: 64 tiles of 16 for each of four
+constexpr int FEW_WAVES = 4, FEW_NT = 64 * FEW_WAVES;
+template <bool E8> constexpr int few_step_keys() { return E8 ? 64 : 32; }  // of a wavefront: 16 KB of keys and values of 128
+template <bool E8> constexpr int few_unit() { return FEW_WAVES * few_step_keys<E8>(); }
+constexpr int FEW_SPAN = 64 * 16 * FEW_WAVES;  // keys for which the lanes hold the pages and scales: 64 tiles of 16 for each wavefront
 
 struct FewArgs {
     gp_paged_attention_params p;
     int group;        // query heads to a head of the cache
     int row_blocks;   // of 16 * NT rows
-    int splits;       // stretches of `chunk` keys per sequence, at most
-    int chunk;
-    int *arrived;     // workspace: a counter for every (sequence, head, row block), 0 between launches
-    float *partial;   // ... and for every tile 16 * NT rows of D values, then their maxima and sums
+    int shares;       // parts of the keys, per head and row block, at most; 0: every sequence is a part
+    int *arrived;     // workspace: a counter for every (head, row block, sequence), 0 between launches
+    float *partial;   // ... and for every tile two results: 16 * NT rows of D values, then their maxima and sums
 };
 
 template <int NT, int D> constexpr int few_partial_floats() { return 16 * NT * (D + 2); }
-template <int NT, int D> constexpr size_t few_lds_bytes() { return (size_t)FEW_WAVES * 16 * NT * (D + 4 + 2) * sizeof(float); }
+template <int NT, int D> constexpr int few_lds_floats() { return FEW_WAVES * 16 * NT * (D + 4 + 2); }
 
 __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c, _Float16) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -48,26 +52,48 @@ template <bool HI> __device__ __forceinline__ unsigned widen(unsigned raw, __bf1
 __device__ __forceinline__ float page_scale(const float *scales, long at) { return fminf(fmaxf(scales[at], 0x1p-60f), 0x1p60f); }
 
 // stores and loads of what another workgroup reads or has written within the launch
-__device__ __forceinline__ void put_shared(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float get_shared(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void put_shared(float *p, f32x2 v) { __hip_atomic_store((unsigned long long *)p, __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ f32x2 get_shared(const float *p) { return __builtin_bit_cast(f32x2, __hip_atomic_load((const unsigned long long *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)); }
 
-template <typename T, int D, bool E8, int NT>
-__device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *lds) {
+template <typename V> __device__ __forceinline__ V load_cache(const char *p) { return __builtin_nontemporal_load((const V *)p); }
+
+// One sequence as a block of rows sees it
+struct FewSequence {
+    SeqTokens s;
+    int nrows;       // of the block and those behind it
+    int bound, kmin, kend;  // keys; those that every row of the block sees, and that some row does
+    int units;       // of few_unit keys: what the parts are made of (a sequence that sees nothing counts as one: it gets its zeros)
+};
+template <int ROWS, int UNIT>
+__device__ __forceinline__ FewSequence few_sequence(const FewArgs &a, const SeqTokens &s, int rb) {
     const gp_paged_attention_params &p = a.p;
-    constexpr int KS = E8 ? 64 : 32, TILES = KS / 16, PAIRS = KS / 32;  // keys of a wavefront's step
+    FewSequence f;
+    f.s = s;
+    f.nrows = f.s.rows * a.group - rb * ROWS;
+    f.bound = (int)seq_bound(f.s, p.max_len, p.table_width, p.cache.page_size);
+    const int last = (rb * ROWS + (f.nrows < ROWS ? f.nrows : ROWS) - 1) / a.group, first = rb * ROWS / a.group;
+    f.kend = (int)keys_seen(f.bound, f.s.first + last, p.causal);
+    f.kmin = (int)keys_seen(f.bound, f.s.first + first, p.causal);
+    f.units = f.nrows <= 0 ? 0 : f.kend <= UNIT ? 1 : (f.kend + UNIT - 1) / UNIT;
+    return f;
+}
+
+// the part of `units` units, in `shares` parts, that unit x is in
+__device__ __forceinline__ int share_of(long x, long units, long shares) { return (int)(((x + 1) * shares - 1) / units); }
+
+// Keys [c0, kend) of one sequence; then its rows are finished, or its part of them waits in slot `slot` for the others.
+// first_share, last_share: the parts that the sequence's keys are spread over.
+template <typename T, int D, bool E8, int NT>
+__device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequence &f, int b, int hr, int c0, int c1, float *slot, int first_share, int last_share, float *lds) {
+    const gp_paged_attention_params &p = a.p;
+    constexpr int KS = few_step_keys<E8>(), TILES = KS / 16, PAIRS = KS / 32;  // keys of a wavefront's step
     constexpr int ROWS = 16 * NT, VD = D / 16, KL = E8 ? D / 64 : D / 32;
     constexpr int ES = E8 ? 1 : 2;  // bytes of a value
+    typedef unsigned int VRow __attribute__((ext_vector_type(VD * ES / 4)));  // a lane's values of one key
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
-    const int b = t.x, split = t.y % a.splits, hr = t.y / a.splits, rb = hr % a.row_blocks, kvh = hr / a.row_blocks, P = p.cache.page_size;
-    const SeqTokens s = seq_tokens(p.start, p.kv_len, b, p.tokens, p.max_new);
-    const int nrows = s.rows * a.group - rb * ROWS;  // of this block
-    if (nrows <= 0) return;
-    const int bound = (int)seq_bound(s, p.max_len, p.table_width, P);
-    const int last_token = (rb * ROWS + (nrows < ROWS ? nrows : ROWS) - 1) / a.group, first_token = rb * ROWS / a.group;
-    const int kend_all = (int)keys_seen(bound, s.first + last_token, p.causal), kmin = (int)keys_seen(bound, s.first + first_token, p.causal);
-    const int nsplits = kend_all <= a.chunk ? 1 : (kend_all + a.chunk - 1) / a.chunk;
-    if (split >= nsplits) return;
-    const int c0 = split * a.chunk, kend = c0 + a.chunk < kend_all ? c0 + a.chunk : kend_all;
+    const int rb = hr % a.row_blocks, kvh = hr / a.row_blocks, P = p.cache.page_size;
+    const SeqTokens &s = f.s;
+    const int nrows = f.nrows, bound = f.bound, kmin = f.kmin, kend = c1 < f.kend ? c1 : f.kend;
 
     // ---- queries: column l % 16 of tile n, in the order of values that the keys are loaded in ----
     u32x4 q[NT][D / 32];
@@ -114,7 +140,7 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
         const int left = (kend - base < FEW_SPAN ? kend - base : FEW_SPAN) - wave * KS;
         const int steps = left <= 0 ? 0 : (left + FEW_WAVES * KS - 1) / (FEW_WAVES * KS);
         u32x4 kr[TILES][KL];
-        u32x4 vr[PAIRS][8];
+        VRow vr[PAIRS][8];
         auto tile_at = [&](int step, int i) -> long {  // byte offset of the i-th tile of a step in the pool (one that is not there: page 0)
             const int at = step * TILES + i, page = __builtin_amdgcn_readlane(page_l, at);
             const int key = base + (step * FEW_WAVES + wave) * KS + i * 16;
@@ -125,7 +151,7 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
             for (int i = 0; i < TILES; ++i) {
                 const char *at = K + tile_at(step, i);
 #pragma unroll
-                for (int k = 0; k < KL; ++k) kr[i][k] = *(const u32x4 *)(at + koff + k * 64);
+                for (int k = 0; k < KL; ++k) kr[i][k] = load_cache<u32x4>(at + koff + k * 64);
             }
         };
         auto load_v = [&](int step) {
@@ -135,14 +161,7 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
                 for (int h = 0; h < 2; ++h) {
                     const char *at = V + tile_at(step, 2 * pr + h);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const char *from = at + voff + e * D * ES;
-                        u32x4 x = {0, 0, 0, 0};
-                        if constexpr (VD * ES == 16) x = *(const u32x4 *)from;
-                        else if constexpr (VD * ES == 8) { const u32x2 y = *(const u32x2 *)from; x[0] = y[0]; x[1] = y[1]; }
-                        else x[0] = *(const unsigned *)from;
-                        vr[pr][4 * h + e] = x;
-                    }
+                    for (int e = 0; e < 4; ++e) vr[pr][4 * h + e] = load_cache<VRow>(at + voff + e * D * ES);
                 }
         };
         if (steps > 0) { load_k(0); load_v(0); }
@@ -201,7 +220,7 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
                             if (key >= lim || key >= seen[n]) x[n][i][e] = -INFINITY;
-                        if (key >= lim) vr[i / 2][4 * (i % 2) + e] = u32x4{0, 0, 0, 0};
+                        if (key >= lim) vr[i / 2][4 * (i % 2) + e] = VRow(0);
                     }
                 }
             }
@@ -299,58 +318,150 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
         for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f(v[e] * inv);
         *(tx4 *)((T *)p.out + (s.row0 + token) * p.ld_out + ((long)kvh * a.group + hg) * D + d) = y;
     };
-    float *mine = a.partial + (((long)hr * p.batch + b) * a.splits + split) * few_partial_floats<NT, D>();
+    const int parts = last_share - first_share + 1;
     for (int u = tid; u < rows * (D / 4); u += FEW_NT) {
         const int r = u / (D / 4), d = u % (D / 4) * 4;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < FEW_WAVES; ++w) top = fmaxf(top, ml[2 * (w * ROWS + r)]);
+        const float base = top == -INFINITY ? 0.f : top;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < FEW_WAVES; ++w) {
             const f32x2 x = *(const f32x2 *)(ml + 2 * (w * ROWS + r));
-            const float f = x[0] == -INFINITY ? (x[1] == 0.f ? 0.f : x[1]) : __builtin_amdgcn_exp2f(x[0] - top);
+            const float f = __builtin_amdgcn_exp2f(x[0] - base);
             sum += f * x[1];
             const f32x4 y = *(const f32x4 *)(lds + (w * ROWS + r) * LD + d);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = x[1] == 0.f ? v[e] : fmaf(f, y[e], v[e]);
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(f, y[e], v[e]);
         }
-        if (nsplits == 1) finish(r, d, v, sum);
+        if (parts == 1) finish(r, d, v, sum);
         else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) put_shared(mine + r * D + d + e, v[e]);
-            if (d == 0) { put_shared(mine + ROWS * D + 2 * r, top); put_shared(mine + ROWS * D + 2 * r + 1, sum); }
+            put_shared(slot + r * D + d, f32x2{v[0], v[1]});
+            put_shared(slot + r * D + d + 2, f32x2{v[2], v[3]});
+            if (d == 0) put_shared(slot + ROWS * D + 2 * r, f32x2{top, sum});
         }
     }
-    if (nsplits == 1) return;
-    // ---- whoever comes last joins the stretches, in their order ----
+    if (parts == 1) return;
+    // ---- whoever comes last joins the parts, in their order ----
     __shared__ int came;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above have reached the memory that all XCDs see
     __syncthreads();
     int *arrived = a.arrived + (long)hr * p.batch + b;
     if (tid == 0) came = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (came != nsplits - 1) return;
+    if (came != parts - 1) return;
     if (tid == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const float *all = a.partial + ((long)hr * p.batch + b) * a.splits * few_partial_floats<NT, D>();
-    for (int u = tid; u < rows * (D / 4); u += FEW_NT) {
-        const int r = u / (D / 4), d = u % (D / 4) * 4;
-        float top = -INFINITY, sum = 0.f;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < nsplits; ++i) {
-            const float *x = all + (long)i * few_partial_floats<NT, D>();
-            const float mi = get_shared(x + ROWS * D + 2 * r), si = get_shared(x + ROWS * D + 2 * r + 1);
-            f32x4 y;
+    // (up to FEW_JOIN of them at a time: first their factors, which every thread needs, then their values, eight loads of a thread in flight.
+    // A part that no row saw anything of has factor 0, and its values are zeros.)
+    const float *all = a.partial + ((long)hr * a.shares + first_share) * 2 * few_partial_floats<NT, D>();
+    auto part_at = [&](int i) { return all + (2l * i + (i == 0)) * few_partial_floats<NT, D>(); };  // the first part is what its tile did last
+    constexpr int FEW_JOIN = few_lds_floats<NT, D>() / (2 * ROWS) < 256 ? few_lds_floats<NT, D>() / (2 * ROWS) : 256;
+    constexpr int ITEMS = (ROWS * D / 4 + FEW_NT - 1) / FEW_NT;  // of a thread: four values of one row
+    f32x4 v[ITEMS];
+    float top[ITEMS], sum[ITEMS];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = get_shared(x + r * D + d + e);
-            if (si == 0.f) continue;
-            const float now = fmaxf(top, mi), fo = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now), fi = mi == -INFINITY ? si : __builtin_amdgcn_exp2f(mi - now);
-            top = now;
-            sum = sum * fo + si * fi;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = v[e] * fo + y[e] * fi;
+    for (int k = 0; k < ITEMS; ++k) { v[k] = f32x4{0.f, 0.f, 0.f, 0.f}; top[k] = -INFINITY; sum[k] = 0.f; }
+    for (int i0 = 0; i0 < parts; i0 += FEW_JOIN) {
+        const int n = parts - i0 < FEW_JOIN ? parts - i0 : FEW_JOIN;
+        __syncthreads();
+        for (int u = tid; u < n * rows; u += FEW_NT) {
+            const int i = u / rows, r = u - i * rows;
+            *(f32x2 *)(lds + 2 * (i * ROWS + r)) = get_shared(part_at(i0 + i) + ROWS * D + 2 * r);
         }
-        finish(r, d, v, sum);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
+            if (r >= rows) continue;
+            float now = top[k];
+            for (int i = 0; i < n; ++i) now = fmaxf(now, lds[2 * (i * ROWS + r)]);
+            const float base = now == -INFINITY ? 0.f : now, f0 = __builtin_amdgcn_exp2f(top[k] - base);
+            top[k] = now;
+            sum[k] *= f0;
+            v[k] *= f0;
+            for (int i = 0; i < n; i += 8) {
+                f32x2 y[8][2];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float *from = part_at(i0 + (i + e < n ? i + e : i)) + r * D + d;
+                    y[e][0] = get_shared(from);
+                    y[e][1] = get_shared(from + 2);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (i + e >= n) break;
+                    const f32x2 ms = *(const f32x2 *)(lds + 2 * ((i + e) * ROWS + r));
+                    const float f = __builtin_amdgcn_exp2f(ms[0] - base);
+                    sum[k] += f * ms[1];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[k][c] = fmaf(f, y[e][c / 2][c % 2], v[k][c]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
+        if (r < rows) finish(r, d, v[k], sum[k]);
+    }
+}
+
+template <typename T, int D, bool E8, int NT>
+__device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *lds) {
+    const gp_paged_attention_params &p = a.p;
+    constexpr int ROWS = 16 * NT, UNIT = few_unit<E8>();
+    const int lane = threadIdx.x & 63, hr = t.y, rb = hr % a.row_blocks, batch = p.batch;
+    if (a.shares == 0) {  // a tile per sequence
+        const FewSequence f = few_sequence<ROWS, UNIT>(a, seq_tokens(p.start, p.kv_len, t.x, p.tokens, p.max_new), rb);
+        if (f.nrows > 0) attend_stretch<T, D, E8, NT>(a, f, t.x, hr, 0, f.kend, nullptr, 0, 0, lds);
+        return;
+    }
+    // ---- all units; then the sequence in which this part begins.  Every wavefront for itself, 64 sequences at a time, one to a lane ----
+    int r0, r1, len;  // of the lane's sequence
+    auto look = [&](int b0) {
+        const int b = b0 + lane < batch ? b0 + lane : batch - 1;
+        r0 = p.start ? p.start[b] : b;
+        r1 = p.start ? p.start[b + 1] : b + 1;
+        len = p.kv_len[b];
+        return b0 + lane < batch ? few_sequence<ROWS, UNIT>(a, seq_tokens_of(r0, r1, len, p.tokens, p.max_new), rb).units : 0;
+    };
+    int total = 0, n = 0;
+    for (int b0 = batch <= 64 ? 0 : (batch - 1) / 64 * 64; b0 >= 0; b0 -= 64) total += n = look(b0);  // (the first 64 last: they are looked at next)
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d, 64);
+    total = __builtin_amdgcn_readfirstlane(total);
+    // (a part has four units or more: joining costs as much as a few units)
+    const int shares = total / 4 < 1 ? 1 : total / 4 < a.shares ? total / 4 : a.shares;
+    if (t.x >= shares) return;
+    const int lo = (int)((long)t.x * total / shares), hi = (int)((t.x + 1l) * total / shares);
+    int at = 0, b0 = 0, b = 0;  // units in front of sequence b, which is one of the 64 from b0 on
+    for (;; b0 += 64) {
+        if (b0) n = look(b0);
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int x = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += x;
+        }
+        const unsigned long long behind = __ballot(at + upto > lo);
+        if (behind) {
+            b = b0 + __builtin_ctzll(behind);
+            at += __builtin_amdgcn_readlane(upto - n, b - b0);
+            break;
+        }
+        at += __builtin_amdgcn_readlane(upto, 63);
+    }
+    float *slots = a.partial + ((long)hr * a.shares + t.x) * 2 * few_partial_floats<NT, D>();
+    for (; at < hi; ++b) {
+        if (b - b0 == 64) look(b0 += 64);
+        const int i = b - b0;
+        const FewSequence f = few_sequence<ROWS, UNIT>(a, seq_tokens_of(__builtin_amdgcn_readlane(r0, i), __builtin_amdgcn_readlane(r1, i), __builtin_amdgcn_readlane(len, i), p.tokens, p.max_new), rb);
+        if (f.units == 0) continue;
+        const int u0 = lo > at ? lo - at : 0, u1 = hi - at < f.units ? hi - at : f.units;
+        attend_stretch<T, D, E8, NT>(a, f, b, hr, u0 * UNIT, u1 == f.units ? f.kend : u1 * UNIT, slots + (u0 == 0) * few_partial_floats<NT, D>(),
+                                     share_of(at, total, shares), share_of(at + f.units - 1l, total, shares), lds);
+        at += f.units;
     }
 }
 

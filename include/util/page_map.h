@@ -15,17 +15,21 @@ struct SeqTokens {
     long len;    // tokens in the cache, the new ones included
 };
 
-// start: batch + 1 row numbers, or nullptr: one new token per sequence
-GP_HD SeqTokens seq_tokens(const int *start, const int *kv_len, int b, long tokens, int max_new) {
+// r0, r1: its first row and the one behind its last; len: tokens in the cache
+GP_HD SeqTokens seq_tokens_of(long r0, long r1, int len, long tokens, int max_new) {
     SeqTokens s;
-    const long r0 = start ? start[b] : b, r1 = start ? start[b + 1] : (long)b + 1;
     s.row0 = r0;
-    s.len = kv_len[b];
+    s.len = len;
     s.first = s.len - (r1 - r0);
     long n = (r1 < tokens ? r1 : tokens) - r0;
     if (n > max_new) n = max_new;
     s.rows = r0 < 0 || n < 0 ? 0 : (int)n;
     return s;
+}
+
+// start: batch + 1 row numbers, or nullptr: one new token per sequence
+GP_HD SeqTokens seq_tokens(const int *start, const int *kv_len, int b, long tokens, int max_new) {
+    return seq_tokens_of(start ? start[b] : b, start ? start[b + 1] : (long)b + 1, kv_len[b], tokens, max_new);
 }
 
 // the first `bound` of a sequence's tokens lie in its table and in front of max_len
