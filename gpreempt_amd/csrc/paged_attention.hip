@@ -29,7 +29,7 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
     if (!p->start) a.p.max_new = 1;
     if (a.p.scale == 0.f) a.p.scale = 1.f;
     const long rows = (long)a.p.max_new * a.group;
-    GP_REQUIRE(rows < (1L << 30), "paged_attention: too large");
+    GP_REQUIRE(rows < (1L << 30) && (long)p->batch * a.p.max_new < (1L << 31), "paged_attention: too large");
     pl->nt = rows <= 16 ? 1 : 2;
     const long blocks = (rows + 16 * pl->nt - 1) / (16 * pl->nt), heads = blocks * p->cache.kv_heads, units = heads * p->batch;
     GP_REQUIRE(units < (1L << 30), "paged_attention: too large");
