@@ -1,4 +1,12 @@
-// Log probabilities of given tokens, entropy and largest alternatives of rows of logits.
+// Log probabilities of given tokens, entropy and largest alternatives of rows of logits, in one pass over the row.
+//
+// With m the largest logit so far, y = scale * (x - m), S = sum 2^(y log2 e) and W = sum y 2^(..): log p = y - log S, entropy = log S - W / S, and a
+// larger m' turns them into f S and f (W + d S), f = 2^(d log2 e), d = scale * (m - m').  Every thread keeps m, S and W of what it has seen.
+// Bound by memory for many rows: a workgroup takes a row, 16384 logits at a time, 32 to a thread, the next ones on their way while these are worked on.
+// A few long rows are cut into parts, joined by whoever comes last.
+//
+// The alternatives: of 64 groups of threads the top-th largest maximum is a bound that at least `top` logits reach; the few that reach it go to a list
+// in LDS, from which the largest are picked by their rank.  The bound is raised only when many threads have something above it.
 #include <algorithm>
 #include <cmath>
 #include "mma.hpp"
@@ -6,7 +14,28 @@
 
 namespace gp {
 
-constexpr int LP_NT = 256, LP_TOP = 32;
+constexpr int LP_NT = 512, LP_WAVES = LP_NT / 64, LP_TOP = 32;
+constexpr int LP_EACH = 32;                 // logits of a thread at a time
+constexpr int LP_TILE = LP_NT * LP_EACH;
+constexpr int LP_LIST = 2048;               // places for candidates
+constexpr int LP_MANY = 128;                // threads above the bound from which it is raised
+constexpr int LP_PARTS = 16;                // of a row, at most
+constexpr int LP_PART_WORDS = 2 + LP_TOP;   // 64-bit words of a part's result
+
+struct LogprobsArgs {
+    gp_token_logprobs_params p;
+    int parts, tiles_per_part;
+    int *arrived;                 // workspace: a counter per row, 0 between launches
+    unsigned long long *partial;  // ... and LP_PART_WORDS for every part
+};
+
+struct LogprobsLds {
+    float groups[2][64];
+    int hits[2];
+    int count, came;
+    float red[3][LP_WAVES];
+    unsigned long long list[2][LP_LIST];
+};
 
 // Order of the alternatives in one number: the larger logit first, then the lower token.  0: no alternative (NaN, -infinity).
 __device__ __forceinline__ unsigned long long rank_key(float x, int id) {
@@ -16,80 +45,259 @@ __device__ __forceinline__ unsigned long long rank_key(float x, int id) {
 }
 __device__ __forceinline__ float key_value(unsigned long long key) {
     const unsigned u = (unsigned)(key >> 32);
-    return __builtin_bit_cast(float, u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+    return key ? __builtin_bit_cast(float, u & 0x80000000u ? u & 0x7FFFFFFFu : ~u) : -INFINITY;
 }
-__device__ __forceinline__ int key_id(unsigned long long key) { return (int)(0xFFFFFFFFu - (unsigned)key); }
+__device__ __forceinline__ int key_id(unsigned long long key) { return key ? (int)(0xFFFFFFFFu - (unsigned)key) : -1; }
 
-__device__ __forceinline__ float block_sum(float x, float *lds) {
-    __syncthreads();
-    lds[threadIdx.x] = x;
-    __syncthreads();
-    float s = 0.f;
-    for (int i = 0; i < LP_NT; ++i) s += lds[i];
-    return s;
-}
-
-// One row per tile, read once for the largest value, once for the sums, once more for every alternative.
-template <typename T>
-__device__ __forceinline__ void logprobs_tile(const gp_token_logprobs_params &p, TileIdx t, float *lds, unsigned long long *keys) {
-    const int tid = threadIdx.x;
-    const T *x = (const T *)p.logits + (long)t.x * p.ld;
-    float m = -INFINITY;
-    for (int i = tid; i < p.vocab; i += LP_NT) m = fmaxf(m, Elem<T>::to_f(x[i]));
-    __syncthreads();
-    lds[tid] = m;
-    __syncthreads();
-    for (int i = 0; i < LP_NT; ++i) m = fmaxf(m, lds[i]);
-    float sum = 0.f, weighted = 0.f;
-    for (int i = tid; i < p.vocab; i += LP_NT) {
-        const float v = Elem<T>::to_f(x[i]);
-        const float y = v == -INFINITY ? -INFINITY : (v - m) * p.scale, e = expf(y);
-        sum += e;
-        if (e > 0.f) weighted = fmaf(e, y, weighted);
+// the top-th largest of the 64 lanes' values
+__device__ __forceinline__ float kth_of_64(float v, int top) {
+    int rank = 0;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) {
+        const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), j));
+        rank += o > v || (o == v && j < lane);
     }
-    sum = block_sum(sum, lds);
-    weighted = block_sum(weighted, lds);
-    const float log_sum = logf(sum);
-    const bool empty = sum == 0.f;
-    if (tid == 0) {
-        if (p.logprob) {
-            const long id = p.tokens[t.x];
-            float r = 0.f;
-            if (id >= 0 && id < p.vocab) {
-                const float v = Elem<T>::to_f(x[id]);
-                r = empty ? -INFINITY : (v == -INFINITY && sum == sum ? -INFINITY : (v - m) * p.scale - log_sum);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), __builtin_ctzll(__ballot(rank == top - 1))));
+}
+__device__ __forceinline__ float max_of_8_lanes(float v) {
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) v = fmaxf(v, __shfl_xor(v, d, 64));
+    return v;
+}
+
+// a thread's logits of one tile: LOADS times VEC neighbours, those behind the row's end -infinity
+template <typename T> struct Logits {
+    static constexpr int VEC = 16 / sizeof(T), LOADS = LP_EACH / VEC;
+    typedef T Raw __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));  // (rows start anywhere)
+    typedef T Chunk __attribute__((ext_vector_type(VEC)));
+    static __device__ __forceinline__ int at(int tile, int load) { return tile * LP_TILE + load * (LP_NT * VEC) + (int)threadIdx.x * VEC; }
+    Chunk raw[LOADS];
+    __device__ __forceinline__ void load(const T *row, int vocab, int tile) {
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) {
+            const int i = at(tile, k);
+            if (i + VEC <= vocab) raw[k] = *(const Raw *)(row + i);
+            else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) raw[k][e] = i + e < vocab ? row[i + e] : Elem<T>::from_f(-INFINITY);
             }
-            p.logprob[t.x] = r;
         }
-        if (p.entropy) p.entropy[t.x] = empty ? 0.f : log_sum - weighted / sum;
     }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < p.top; ++k) {
-        unsigned long long best = 0;
-        for (int i = tid; i < p.vocab; i += LP_NT) {
-            const unsigned long long key = rank_key(Elem<T>::to_f(x[i]), i);
-            if (key < last && key > best) best = key;
+    __device__ __forceinline__ float operator()(int k, int e) const { return Elem<T>::to_f(raw[k][e]); }
+};
+
+// the largest `top` of a list of keys (no 0 among them), of which there may be fewer: put(rank, key)
+template <class Put>
+__device__ __forceinline__ void pick(LogprobsLds &l, int which, int count, int top, Put &&put) {
+    const int tid = threadIdx.x;
+    float bound = -INFINITY;
+    while (count > 256) {  // (of a long list, those that reach a bound: as for the logits)
+        float most = -INFINITY;
+        for (int i = tid; i < count; i += LP_NT) most = fmaxf(most, key_value(l.list[which][i]));
+        most = max_of_8_lanes(most);
+        __syncthreads();
+        if ((tid & 7) == 0) l.groups[0][tid >> 3] = most;
+        if (tid == 0) l.count = 0;
+        __syncthreads();
+        const float next = kth_of_64(l.groups[0][tid & 63], top);
+        if (!(next > bound)) break;
+        bound = next;
+        for (int i = tid; i < count; i += LP_NT) {
+            const unsigned long long key = l.list[which][i];
+            if (key_value(key) >= bound) l.list[!which][atomicAdd(&l.count, 1)] = key;
         }
         __syncthreads();
-        keys[tid] = best;
-        __syncthreads();
-        for (int i = 0; i < LP_NT; ++i) best = best < keys[i] ? keys[i] : best;
+        count = l.count;
+        which = !which;
+    }
+    for (int i = tid; i < count; i += LP_NT) {
+        const unsigned long long key = l.list[which][i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += l.list[which][j] > key;
+        if (rank < top) put(rank, key);
+    }
+    for (int i = count + tid; i < top; i += LP_NT) put(i, 0ull);
+}
+
+template <typename T>
+__device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, LogprobsLds &l) {
+    const gp_token_logprobs_params &p = a.p;
+    const int tid = threadIdx.x, wave = tid >> 6, top = p.top, vocab = p.vocab;
+    const long r = t.y;
+    const T *row = (const T *)p.logits + r * p.ld;
+    const float c = p.scale * 1.44269504088896340736f;
+    const int tiles = (vocab + LP_TILE - 1) / LP_TILE, first = t.x * a.tiles_per_part, last = first + a.tiles_per_part < tiles ? first + a.tiles_per_part : tiles;
+    // the given token's logit (asked for first, needed last)
+    const long token = p.logprob ? p.tokens[r] : -1;
+    const float said = token >= 0 && token < vocab ? Elem<T>::to_f(row[token]) : 0.f;
+    __syncthreads();  // (the previous row's lists are still being read)
+    if (tid == 0) { l.count = 0; l.hits[0] = l.hits[1] = 0; }
+    __syncthreads();
+
+    float m = -INFINITY, s = 0.f, w = 0.f, bound = -INFINITY;
+    Logits<T> x, next;
+    x.load(row, vocab, first);
+    for (int tile = first; tile < last; ++tile) {
+        if (tile + 1 < last) next.load(row, vocab, tile + 1);
+        float most = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < Logits<T>::LOADS; ++k)
+#pragma unroll
+            for (int e = 0; e < Logits<T>::VEC; ++e) most = fmaxf(most, x(k, e));
+        if (most > m) {
+            if (m > -INFINITY) {
+                const float d = (m - most) * c, f = __builtin_amdgcn_exp2f(d);
+                w = f == 0.f ? 0.f : f * fmaf(d, s, w);
+                s *= f;
+            }
+            m = most;
+        }
+        const float base = m > -INFINITY ? m : 0.f;  // (nothing but -infinity so far; or NaN, whose sum is NaN all the same)
+#pragma unroll
+        for (int k = 0; k < Logits<T>::LOADS; ++k)
+#pragma unroll
+            for (int e = 0; e < Logits<T>::VEC; ++e) {
+                const float y = (x(k, e) - base) * c, z = __builtin_amdgcn_exp2f(y);
+                s += z;
+                w = fmaf(z, fmaxf(y, -150.f), w);  // (where 2^y is 0, y may be -infinity)
+            }
+        if (top) {
+            const int par = (tile - first) & 1;
+            const float group = max_of_8_lanes(most);
+            if ((tid & 7) == 0) l.groups[par][tid >> 3] = group;
+            const unsigned long long above = __ballot(most >= bound && most > -INFINITY);
+            if ((tid & 63) == 0 && above) atomicAdd(&l.hits[par], __popcll(above));
+            __syncthreads();
+            const int hits = l.hits[par];
+            if (tid == 0) l.hits[!par] = 0;  // (read in front of the last barrier, added to behind the next)
+            if (hits > LP_MANY) bound = fmaxf(bound, kth_of_64(l.groups[par][tid & 63], top));
+            if (__any(most >= bound && most > -INFINITY)) {
+#pragma unroll
+                for (int k = 0; k < Logits<T>::LOADS; ++k)
+#pragma unroll
+                    for (int e = 0; e < Logits<T>::VEC; ++e) {
+                        const float v = x(k, e);
+                        if (v >= bound && v > -INFINITY) {
+                            const int at = atomicAdd(&l.count, 1);
+                            if (at < LP_LIST) l.list[0][at] = rank_key(v, Logits<T>::at(tile, k) + e);
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        x = next;
+    }
+
+    // ---- the threads' sums ----
+    float M = m;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d, 64));
+    if ((tid & 63) == 0) l.red[0][wave] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < LP_WAVES; ++i) M = fmaxf(M, l.red[0][i]);
+    if (m > -INFINITY) {
+        const float d = (m - M) * c, f = __builtin_amdgcn_exp2f(d);
+        w = f == 0.f ? 0.f : f * fmaf(d, s, w);
+        s *= f;
+    } else w = 0.f;  // (s is 0, or NaN)
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) { s += __shfl_xor(s, d, 64); w += __shfl_xor(w, d, 64); }
+    if ((tid & 63) == 0) { l.red[1][wave] = s; l.red[2][wave] = w; }
+    __syncthreads();
+    s = w = 0.f;
+#pragma unroll
+    for (int i = 0; i < LP_WAVES; ++i) { s += l.red[1][i]; w += l.red[2][i]; }
+    int count = l.count;
+
+    auto finish = [&](float M, float s, float w, int which, int count) {
+        const float log_sum = __builtin_amdgcn_logf(s) * 0.69314718055994530942f;
         if (tid == 0) {
-            p.top_ids[(long)t.x * p.top + k] = best ? key_id(best) : -1;
-            p.top_logprobs[(long)t.x * p.top + k] = best ? (key_value(best) - m) * p.scale - log_sum : -INFINITY;
+            if (p.logprob) p.logprob[r] = token < 0 || token >= vocab ? 0.f : s == 0.f || (said == -INFINITY && s == s) ? -INFINITY : (said - M) * p.scale - log_sum;
+            if (p.entropy) p.entropy[r] = s == 0.f ? 0.f : log_sum - w * 0.69314718055994530942f / s;
         }
-        last = best;
+        if (top) pick(l, which, count, top, [&](int rank, unsigned long long key) {
+            p.top_ids[r * top + rank] = key_id(key);
+            p.top_logprobs[r * top + rank] = key ? (key_value(key) - M) * p.scale - log_sum : -INFINITY;
+        });
+    };
+    // more candidates than the list holds (equal logits, say): one after the other, each the largest behind the last one
+    if (top && count > LP_LIST) {
+        const int from = first * LP_TILE, to = last * LP_TILE < vocab ? last * LP_TILE : vocab;
+        unsigned long long before = ~0ull;
+        for (int k = 0; k < top; ++k) {
+            unsigned long long best = 0;
+            for (int i = from + tid; i < to; i += LP_NT) {
+                const unsigned long long key = rank_key(Elem<T>::to_f(row[i]), i);
+                if (key < before && key > best) best = key;
+            }
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const unsigned long long o = __shfl_xor(best, d, 64);
+                best = o > best ? o : best;
+            }
+            __syncthreads();
+            if ((tid & 63) == 0) l.list[1][wave] = best;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < LP_WAVES; ++i) best = l.list[1][i] > best ? l.list[1][i] : best;
+            if (tid == 0) l.list[0][k] = best;
+            before = best;
+        }
+        __syncthreads();
+        count = top;
     }
+    if (a.parts == 1) { finish(M, s, w, 0, count); return; }
+
+    // ---- a part of a row: its result, and whoever comes last joins them ----
+    auto put = [&](unsigned long long *q, unsigned long long v) { __hip_atomic_store(q, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    auto get = [&](const unsigned long long *q) { return __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    unsigned long long *mine = a.partial + (r * a.parts + t.x) * LP_PART_WORDS;
+    if (tid == 0) { put(mine, __builtin_bit_cast(unsigned long long, f32x2{M, s})); put(mine + 1, __builtin_bit_cast(unsigned long long, f32x2{w, 0.f})); }
+    if (top) pick(l, 0, count, top, [&](int rank, unsigned long long key) { put(mine + 2 + rank, key); });
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above have reached the memory that all XCDs see
+    __syncthreads();
+    if (tid == 0) l.came = __hip_atomic_fetch_add(a.arrived + r, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (l.came != a.parts - 1) return;
+    if (tid == 0) __hip_atomic_store(a.arrived + r, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned long long *all = a.partial + r * a.parts * LP_PART_WORDS;
+    M = -INFINITY;
+    f32x2 ms[LP_PARTS], wz[LP_PARTS];
+#pragma unroll
+    for (int i = 0; i < LP_PARTS; ++i) {
+        ms[i] = __builtin_bit_cast(f32x2, get(all + (i < a.parts ? i : 0) * LP_PART_WORDS));
+        wz[i] = __builtin_bit_cast(f32x2, get(all + (i < a.parts ? i : 0) * LP_PART_WORDS + 1));
+        M = fmaxf(M, ms[i][0]);
+    }
+    if (tid == 0) l.count = 0;
+    __syncthreads();
+    for (int i = tid; i < a.parts * top; i += LP_NT) {
+        const unsigned long long key = get(all + i / top * LP_PART_WORDS + 2 + i % top);
+        if (key) l.list[0][atomicAdd(&l.count, 1)] = key;
+    }
+    s = w = 0.f;
+#pragma unroll
+    for (int i = 0; i < LP_PARTS; ++i)
+        if (i < a.parts) {
+            if (ms[i][0] > -INFINITY) {
+                const float d = (ms[i][0] - M) * c, f = __builtin_amdgcn_exp2f(d);
+                w += f == 0.f ? 0.f : f * fmaf(d, ms[i][1], wz[i][0]);
+                s = fmaf(f, ms[i][1], s);
+            } else s += ms[i][1];
+        }
+    __syncthreads();
+    finish(M, s, w, 0, l.count);
 }
 
 template <typename T, int LOOP = LOOP_ANY>
-__global__ __launch_bounds__(LP_NT) void token_logprobs_kernel(gp_token_logprobs_params p, BlpArgs blp) {
-    __shared__ float lds[LP_NT];
-    __shared__ unsigned long long keys[LP_NT];
-    tiles<LOOP>(blp, [&](TileIdx t) { logprobs_tile<T>(p, t, lds, keys); });
+__global__ __launch_bounds__(LP_NT) void token_logprobs_kernel(LogprobsArgs a, BlpArgs blp) {
+    __shared__ LogprobsLds l;
+    tiles<LOOP>(blp, [&](TileIdx t) { logprobs_tile<T>(a, t, l); });
 }
 
-static int check_token_logprobs(const gp_token_logprobs_params *p) {
+static int plan_token_logprobs(const gp_token_logprobs_params *p, LogprobsArgs *a, size_t *work_bytes) {
     GP_REQUIRE(p && p->logits, "null token_logprobs params");
     GP_REQUIRE(p->dtype == GP_F32 || p->dtype == GP_F16 || p->dtype == GP_BF16, "token_logprobs dtype %d", p->dtype);
     GP_REQUIRE(p->rows > 0 && p->rows < (1L << 31) && p->vocab > 0 && p->vocab < (1 << 30) && p->ld >= p->vocab, "token_logprobs: rows, vocab (below 2^30) and a row stride that holds it");
@@ -99,6 +307,21 @@ static int check_token_logprobs(const gp_token_logprobs_params *p) {
     GP_REQUIRE(p->logprob || p->entropy || p->top, "token_logprobs: nothing is asked for");
     GP_REQUIRE(!p->logprob || p->tokens, "token_logprobs: log probabilities of which tokens?");
     GP_REQUIRE(p->scale >= 0.f && std::isfinite(p->scale), "token_logprobs: the scale must be finite and not negative");
+    *a = LogprobsArgs{};
+    a->p = *p;
+    if (p->scale == 0.f) a->p.scale = 1.f;
+    // rows of at least four tiles are cut while there are compute units without one, into parts of two tiles or more
+    const long tiles = ((long)p->vocab + LP_TILE - 1) / LP_TILE;
+    const long want = std::max(1l, std::min({(long)LP_PARTS, device_cus() / p->rows, tiles / 2}));
+    a->tiles_per_part = (int)((tiles + want - 1) / want);
+    a->parts = (int)((tiles + a->tiles_per_part - 1) / a->tiles_per_part);
+    *work_bytes = 0;
+    if (a->parts > 1) {
+        const size_t counters = ((size_t)p->rows * sizeof(int) + 255) / 256 * 256;
+        *work_bytes = counters + (size_t)p->rows * a->parts * LP_PART_WORDS * sizeof(unsigned long long);
+        a->arrived = (int *)p->work;
+        a->partial = (unsigned long long *)((char *)p->work + counters);
+    }
     return GP_SUCC;
 }
 
@@ -107,19 +330,23 @@ static int check_token_logprobs(const gp_token_logprobs_params *p) {
 using namespace gp;
 
 extern "C" int gp_token_logprobs_work_bytes(const gp_token_logprobs_params *p, size_t *bytes) {
-    if (int rc = check_token_logprobs(p)) return rc;
+    LogprobsArgs a;
+    size_t n;
+    if (int rc = plan_token_logprobs(p, &a, &n)) return rc;
     GP_REQUIRE(bytes, "token_logprobs: no place for the size");
-    *bytes = 0;
+    *bytes = n;
     return GP_SUCC;
 }
 
 extern "C" int gp_launch_token_logprobs(const gp_token_logprobs_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
-    if (int rc = check_token_logprobs(p)) return rc;
-    gp_token_logprobs_params a = *p;
-    if (a.scale == 0.f) a.scale = 1.f;
+    LogprobsArgs a;
+    size_t n;
+    if (int rc = plan_token_logprobs(p, &a, &n)) return rc;
+    GP_REQUIRE(n == 0 || (p->work && ((uintptr_t)p->work & 15) == 0 && p->work_bytes >= n), "token_logprobs: needs a workspace of %zu bytes, 16-byte aligned", n);
+    const int rows = (int)p->rows;
     switch (p->dtype) {
-        case GP_F32: return launch_tiles(GP_KSET(token_logprobs_kernel<float), (int)p->rows, 1, ctx, s, info, a, 0, 1, LP_NT);
-        case GP_F16: return launch_tiles(GP_KSET(token_logprobs_kernel<_Float16), (int)p->rows, 1, ctx, s, info, a, 0, 1, LP_NT);
-        default: return launch_tiles(GP_KSET(token_logprobs_kernel<__bf16), (int)p->rows, 1, ctx, s, info, a, 0, 1, LP_NT);
+        case GP_F32: return launch_tiles(GP_KSET(token_logprobs_kernel<float), a.parts, rows, ctx, s, info, a, 0, 1, LP_NT);
+        case GP_F16: return launch_tiles(GP_KSET(token_logprobs_kernel<_Float16), a.parts, rows, ctx, s, info, a, 0, 1, LP_NT);
+        default: return launch_tiles(GP_KSET(token_logprobs_kernel<__bf16), a.parts, rows, ctx, s, info, a, 0, 1, LP_NT);
     }
 }
