@@ -5,8 +5,9 @@
 // Bound by memory for many rows: a workgroup takes a row, 16384 logits at a time, 32 to a thread, the next ones on their way while these are worked on.
 // A few long rows are cut into parts, joined by whoever comes last.
 //
-// The alternatives: of 64 groups of threads the top-th largest maximum is a bound that at least `top` logits reach; the few that reach it go to a list
-// in LDS, from which the largest are picked by their rank.  The bound is raised only when many threads have something above it.
+// The alternatives: every group of eight threads leaves the largest logit of each tile in LDS.  Of the 64 lanes' largest logits, all wavefronts together, the
+// top-th largest is a bound that at least `top` logits reach; the few groups and tiles that reach it are looked at again, what reaches it goes to a list
+// in LDS, and the largest are picked from there by their rank.
 #include <algorithm>
 #include <cmath>
 #include "mma.hpp"
@@ -17,8 +18,10 @@ namespace gp {
 constexpr int LP_NT = 512, LP_WAVES = LP_NT / 64, LP_TOP = 32;
 constexpr int LP_EACH = 32;                 // logits of a thread at a time
 constexpr int LP_TILE = LP_NT * LP_EACH;
-constexpr int LP_LIST = 2048;               // places for candidates
-constexpr int LP_MANY = 128;                // threads above the bound from which it is raised
+constexpr int LP_LIST = 1024;               // places for candidates
+constexpr int LP_GROUPS = LP_NT / 8;          // of eight threads
+constexpr int LP_KEPT = 32;                 // tiles whose groups' largest logits are kept apart (tile t and t + 32 together)
+static_assert(LP_GROUPS == 64, "a lane for each group");
 constexpr int LP_PARTS = 16;                // of a row, at most
 constexpr int LP_PART_WORDS = 2 + LP_TOP;   // 64-bit words of a part's result
 
@@ -30,11 +33,11 @@ struct LogprobsArgs {
 };
 
 struct LogprobsLds {
-    float groups[2][64];
-    int hits[2];
-    int count, came;
+    float groups[LP_KEPT][LP_GROUPS], lanes[LP_WAVES][64];
+    int count, hits, came;
     float red[3][LP_WAVES];
     unsigned long long list[2][LP_LIST];
+    unsigned short hit[LP_KEPT * LP_GROUPS];
 };
 
 // Order of the alternatives in one number: the larger logit first, then the lower token.  0: no alternative (NaN, -infinity).
@@ -49,40 +52,70 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
 }
 __device__ __forceinline__ int key_id(unsigned long long key) { return key ? (int)(0xFFFFFFFFu - (unsigned)key) : -1; }
 
-// the top-th largest of the 64 lanes' values
-__device__ __forceinline__ float kth_of_64(float v, int top) {
-    int rank = 0;
-    const int lane = threadIdx.x & 63;
+// A value that at least `top` of the 64 lanes' values reach, the largest with its 16 leading bits (-infinity: fewer than that are above it).  Bit by bit, in
+// scalar registers: a rank by 64 comparisons takes a wavefront ten times as many vector instructions.
+__device__ __forceinline__ float reached_by(float v, int top) {
+    const unsigned bits = __builtin_bit_cast(unsigned, v), order = v > -INFINITY ? (bits & 0x80000000u ? ~bits : bits | 0x80000000u) : 0u;
+    unsigned t = 0;
 #pragma unroll
-    for (int j = 0; j < 64; ++j) {
-        const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), j));
-        rank += o > v || (o == v && j < lane);
-    }
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), __builtin_ctzll(__ballot(rank == top - 1))));
+    for (int bit = 31; bit >= 16; --bit)
+        if (__popcll(__ballot(order >= (t | 1u << bit))) >= top) t |= 1u << bit;
+    return t == 0 ? -INFINITY : __builtin_bit_cast(float, t & 0x80000000u ? t & 0x7FFFFFFFu : ~t);
 }
+// the largest of three; NaN loses.  (fmaxf makes a signalling NaN a quiet one first, an instruction more for each operand)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+// a value from the lane that a DPP control names
+template <int CTRL> __device__ __forceinline__ float from_lane(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true)); }
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_MIRROR8 = 0x141, DPP_MIRROR16 = 0x140;
 __device__ __forceinline__ float max_of_8_lanes(float v) {
-#pragma unroll
-    for (int d = 1; d < 8; d *= 2) v = fmaxf(v, __shfl_xor(v, d, 64));
-    return v;
+    v = fmaxf(v, from_lane<DPP_XOR1>(v));
+    v = fmaxf(v, from_lane<DPP_XOR2>(v));
+    return fmaxf(v, from_lane<DPP_MIRROR8>(v));
+}
+__device__ __forceinline__ float max_of_wave(float v) {
+    v = max_of_8_lanes(v);
+    v = fmaxf(v, from_lane<DPP_MIRROR16>(v));
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float sum_of_wave(float v) {
+    v += from_lane<DPP_XOR1>(v);
+    v += from_lane<DPP_XOR2>(v);
+    v += from_lane<DPP_MIRROR8>(v);
+    v += from_lane<DPP_MIRROR16>(v);
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
 }
 
-// a thread's logits of one tile: LOADS times VEC neighbours, those behind the row's end -infinity
+// A thread's logits of one tile: LOADS times VEC neighbours.  The chunk in which the row ends is fetched so that it ends there, whoever comes behind it fetches
+// the same; what is in front of a thread's own place counts as -infinity.
 template <typename T> struct Logits {
     static constexpr int VEC = 16 / sizeof(T), LOADS = LP_EACH / VEC;
     typedef T Raw __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));  // (rows start anywhere)
     typedef T Chunk __attribute__((ext_vector_type(VEC)));
-    static __device__ __forceinline__ int at(int tile, int load) { return tile * LP_TILE + load * (LP_NT * VEC) + (int)threadIdx.x * VEC; }
+    static __device__ __forceinline__ int own(int thread, int tile, int load) { return tile * LP_TILE + load * (LP_NT * VEC) + thread * VEC; }
+    static __device__ __forceinline__ int at(int own, int vocab) { return own + VEC <= vocab || vocab < VEC ? own : vocab - VEC; }  // where it is fetched from
     Chunk raw[LOADS];
-    __device__ __forceinline__ void load(const T *row, int vocab, int tile) {
+    static __device__ __forceinline__ void mask(Chunk &c, int vocab, int own) {
 #pragma unroll
-        for (int k = 0; k < LOADS; ++k) {
-            const int i = at(tile, k);
-            if (i + VEC <= vocab) raw[k] = *(const Raw *)(row + i);
-            else {
+        for (int e = 0; e < VEC; ++e)
+            if (e < own - at(own, vocab)) c[e] = Elem<T>::from_f(-INFINITY);
+    }
+    // a row shorter than a chunk
+    static __device__ __forceinline__ Chunk tiny(const T *row, int vocab, int own) {
+        Chunk c;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) raw[k][e] = i + e < vocab ? row[i + e] : Elem<T>::from_f(-INFINITY);
-            }
-        }
+        for (int e = 0; e < VEC; ++e) c[e] = own == 0 && e < vocab ? row[e < vocab ? e : 0] : Elem<T>::from_f(-INFINITY);
+        return c;
+    }
+    // (the same loads whatever the tile, so that the compiler knows at every wait how many are younger; the row's last tile is masked when it is there)
+    __device__ __forceinline__ void fetch(const T *row, int vocab, int tile) {
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) raw[k] = *(const Raw *)(row + at(own((int)threadIdx.x, tile, k), vocab));
     }
     __device__ __forceinline__ float operator()(int k, int e) const { return Elem<T>::to_f(raw[k][e]); }
 };
@@ -100,7 +133,7 @@ __device__ __forceinline__ void pick(LogprobsLds &l, int which, int count, int t
         if ((tid & 7) == 0) l.groups[0][tid >> 3] = most;
         if (tid == 0) l.count = 0;
         __syncthreads();
-        const float next = kth_of_64(l.groups[0][tid & 63], top);
+        const float next = reached_by(l.groups[0][tid & 63], top);
         if (!(next > bound)) break;
         bound = next;
         for (int i = tid; i < count; i += LP_NT) {
@@ -114,6 +147,7 @@ __device__ __forceinline__ void pick(LogprobsLds &l, int which, int count, int t
     for (int i = tid; i < count; i += LP_NT) {
         const unsigned long long key = l.list[which][i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < count; ++j) rank += l.list[which][j] > key;
         if (rank < top) put(rank, key);
     }
@@ -128,23 +162,22 @@ __device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, 
     const T *row = (const T *)p.logits + r * p.ld;
     const float c = p.scale * 1.44269504088896340736f;
     const int tiles = (vocab + LP_TILE - 1) / LP_TILE, first = t.x * a.tiles_per_part, last = first + a.tiles_per_part < tiles ? first + a.tiles_per_part : tiles;
-    // the given token's logit (asked for first, needed last)
+    Logits<T> x;
+    const bool tiny = vocab < Logits<T>::VEC;
+    if (!tiny) x.fetch(row, vocab, first);
+    // the given token's logit (needed last)
     const long token = p.logprob ? p.tokens[r] : -1;
-    const float said = token >= 0 && token < vocab ? Elem<T>::to_f(row[token]) : 0.f;
+    const T said_raw = token >= 0 && token < vocab ? row[token] : Elem<T>::from_f(0.f);
     __syncthreads();  // (the previous row's lists are still being read)
-    if (tid == 0) { l.count = 0; l.hits[0] = l.hits[1] = 0; }
-    __syncthreads();
+    if (tid == 0) l.count = l.hits = 0;
 
-    float m = -INFINITY, s = 0.f, w = 0.f, bound = -INFINITY;
-    Logits<T> x, next;
-    x.load(row, vocab, first);
-    for (int tile = first; tile < last; ++tile) {
-        if (tile + 1 < last) next.load(row, vocab, tile + 1);
+    float m = -INFINITY, s = 0.f, w = 0.f;
+    auto add = [&](const Logits<T> &x, int tile) {
         float most = -INFINITY;
 #pragma unroll
         for (int k = 0; k < Logits<T>::LOADS; ++k)
 #pragma unroll
-            for (int e = 0; e < Logits<T>::VEC; ++e) most = fmaxf(most, x(k, e));
+            for (int e = 0; e < Logits<T>::VEC; e += 2) most = max3(most, x(k, e), x(k, e + 1));
         if (most > m) {
             if (m > -INFINITY) {
                 const float d = (m - most) * c, f = __builtin_amdgcn_exp2f(d);
@@ -160,39 +193,36 @@ __device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, 
             for (int e = 0; e < Logits<T>::VEC; ++e) {
                 const float y = (x(k, e) - base) * c, z = __builtin_amdgcn_exp2f(y);
                 s += z;
-                w = fmaf(z, fmaxf(y, -150.f), w);  // (where 2^y is 0, y may be -infinity)
+                w = fmaf(z, max3(y, -150.f, -150.f), w);  // (where 2^y is 0, y may be -infinity)
             }
         if (top) {
-            const int par = (tile - first) & 1;
             const float group = max_of_8_lanes(most);
-            if ((tid & 7) == 0) l.groups[par][tid >> 3] = group;
-            const unsigned long long above = __ballot(most >= bound && most > -INFINITY);
-            if ((tid & 63) == 0 && above) atomicAdd(&l.hits[par], __popcll(above));
-            __syncthreads();
-            const int hits = l.hits[par];
-            if (tid == 0) l.hits[!par] = 0;  // (read in front of the last barrier, added to behind the next)
-            if (hits > LP_MANY) bound = fmaxf(bound, kth_of_64(l.groups[par][tid & 63], top));
-            if (__any(most >= bound && most > -INFINITY)) {
-#pragma unroll
-                for (int k = 0; k < Logits<T>::LOADS; ++k)
-#pragma unroll
-                    for (int e = 0; e < Logits<T>::VEC; ++e) {
-                        const float v = x(k, e);
-                        if (v >= bound && v > -INFINITY) {
-                            const int at = atomicAdd(&l.count, 1);
-                            if (at < LP_LIST) l.list[0][at] = rank_key(v, Logits<T>::at(tile, k) + e);
-                        }
-                    }
+            if ((tid & 7) == 0) {
+                float *at = &l.groups[(tile - first) % LP_KEPT][tid >> 3];
+                *at = tile - first < LP_KEPT ? group : max3(*at, group, group);
             }
-            __syncthreads();
         }
+    };
+    for (int tile = first; tile + 1 < last; ++tile) {
+        Logits<T> next;
+        next.fetch(row, vocab, tile + 1);
+        add(x, tile);
         x = next;
     }
+    if (last * LP_TILE > vocab) {
+#pragma unroll
+        for (int k = 0; k < Logits<T>::LOADS; ++k) {
+            const int own = Logits<T>::own(tid, last - 1, k);
+            if (tiny) x.raw[k] = Logits<T>::tiny(row, vocab, own);
+            else Logits<T>::mask(x.raw[k], vocab, own);
+        }
+    }
+    add(x, last - 1);
 
     // ---- the threads' sums ----
-    float M = m;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d, 64));
+    const int kept = last - first < LP_KEPT ? last - first : LP_KEPT;
+    float M = max_of_wave(m);
+    l.lanes[wave][tid & 63] = m;
     if ((tid & 63) == 0) l.red[0][wave] = M;
     __syncthreads();
 #pragma unroll
@@ -202,17 +232,52 @@ __device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, 
         w = f == 0.f ? 0.f : f * fmaf(d, s, w);
         s *= f;
     } else w = 0.f;  // (s is 0, or NaN)
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) { s += __shfl_xor(s, d, 64); w += __shfl_xor(w, d, 64); }
+    s = sum_of_wave(s);
+    w = sum_of_wave(w);
     if ((tid & 63) == 0) { l.red[1][wave] = s; l.red[2][wave] = w; }
+    // ---- candidates ----
+    float bound = -INFINITY;
+    if (top) {
+        float lane = l.lanes[0][tid & 63];
+#pragma unroll
+        for (int i = 1; i < LP_WAVES; ++i) lane = fmaxf(lane, l.lanes[i][tid & 63]);
+        bound = reached_by(lane, top);
+        for (int i = tid; i < kept * LP_GROUPS; i += LP_NT) {
+            const float g = l.groups[i / LP_GROUPS][i % LP_GROUPS];
+            if (g >= bound && g > -INFINITY) l.hit[atomicAdd(&l.hits, 1)] = (unsigned short)i;
+        }
+    }
     __syncthreads();
     s = w = 0.f;
 #pragma unroll
     for (int i = 0; i < LP_WAVES; ++i) { s += l.red[1][i]; w += l.red[2][i]; }
+    constexpr int LOOKS = 8 * Logits<T>::LOADS;  // chunks of a group and tile
+    const int looks = l.hits * LOOKS;
+    for (int i = tid; i < looks; i += LP_NT) {
+        const int hit = l.hit[i / LOOKS], thread = hit % LP_GROUPS * 8 + i % 8, load = i / 8 % Logits<T>::LOADS;
+        for (int tile = first + hit / LP_GROUPS; tile < last; tile += LP_KEPT) {
+            const int own = Logits<T>::own(thread, tile, load);
+            typename Logits<T>::Chunk chunk;
+            if (tiny) chunk = Logits<T>::tiny(row, vocab, own);
+            else {
+                chunk = *(const typename Logits<T>::Raw *)(row + Logits<T>::at(own, vocab));
+                Logits<T>::mask(chunk, vocab, own);
+            }
+#pragma unroll
+            for (int e = 0; e < Logits<T>::VEC; ++e) {
+                const float v = Elem<T>::to_f(chunk[e]);
+                if (v >= bound && v > -INFINITY) {
+                    const int at = atomicAdd(&l.count, 1);
+                    if (at < LP_LIST) l.list[0][at] = rank_key(v, Logits<T>::at(own, vocab) + e);
+                }
+            }
+        }
+    }
+    __syncthreads();
     int count = l.count;
 
     auto finish = [&](float M, float s, float w, int which, int count) {
-        const float log_sum = __builtin_amdgcn_logf(s) * 0.69314718055994530942f;
+        const float log_sum = __builtin_amdgcn_logf(s) * 0.69314718055994530942f, said = Elem<T>::to_f(said_raw);
         if (tid == 0) {
             if (p.logprob) p.logprob[r] = token < 0 || token >= vocab ? 0.f : s == 0.f || (said == -INFINITY && s == s) ? -INFINITY : (said - M) * p.scale - log_sum;
             if (p.entropy) p.entropy[r] = s == 0.f ? 0.f : log_sum - w * 0.69314718055994530942f / s;
