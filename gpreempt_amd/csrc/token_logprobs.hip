@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <cmath>
 #include "mma.hpp"
+#include "lanes.hpp"
 #include "launch_tiles.hpp"
 
 namespace gp {
@@ -62,35 +63,6 @@ __device__ __forceinline__ float reached_by(float v, int top) {
         if (__popcll(__ballot(order >= (t | 1u << bit))) >= top) t |= 1u << bit;
     return t == 0 ? -INFINITY : __builtin_bit_cast(float, t & 0x80000000u ? t & 0x7FFFFFFFu : ~t);
 }
-// the largest of three; NaN loses.  (fmaxf makes a signalling NaN a quiet one first, an instruction more for each operand)
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-// a value from the lane that a DPP control names
-template <int CTRL> __device__ __forceinline__ float from_lane(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true)); }
-constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_MIRROR8 = 0x141, DPP_MIRROR16 = 0x140;
-__device__ __forceinline__ float max_of_8_lanes(float v) {
-    v = fmaxf(v, from_lane<DPP_XOR1>(v));
-    v = fmaxf(v, from_lane<DPP_XOR2>(v));
-    return fmaxf(v, from_lane<DPP_MIRROR8>(v));
-}
-__device__ __forceinline__ float max_of_wave(float v) {
-    v = max_of_8_lanes(v);
-    v = fmaxf(v, from_lane<DPP_MIRROR16>(v));
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
-}
-__device__ __forceinline__ float sum_of_wave(float v) {
-    v += from_lane<DPP_XOR1>(v);
-    v += from_lane<DPP_XOR2>(v);
-    v += from_lane<DPP_MIRROR8>(v);
-    v += from_lane<DPP_MIRROR16>(v);
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
-}
-
 // A thread's logits of one tile: LOADS times VEC neighbours.  The chunk in which the row ends is fetched so that it ends there, whoever comes behind it fetches
 // the same; what is in front of a thread's own place counts as -infinity.
 template <typename T> struct Logits {
