@@ -1,13 +1,15 @@
 // Attention of a batch of sequences' new tokens over the pages of a cache.
 #include <algorithm>
 #include "paged_few.hpp"
+#include "paged_many.hpp"
 #include "launch_tiles.hpp"
 
 namespace gp {
 
 struct PagedPlan {
     FewArgs few;
-    int nt;             // query rows of a tile, in sixteens
+    ManyArgs many;
+    int nt;             // query rows of a tile, in sixteens; 0: many
     int tiles_x; long tiles_y;
     size_t work_bytes;
 };
@@ -30,6 +32,24 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
     if (a.p.scale == 0.f) a.p.scale = 1.f;
     const long rows = (long)a.p.max_new * a.group;
     GP_REQUIRE(rows < (1L << 30) && (long)p->batch * a.p.max_new < (1L << 31), "paged_attention: too large");
+    // Many rows: blocks of 128 of them over keys that come through LDS, if there are such blocks for a quarter of the compute units (128 rows of 8 heads of 128 over 4000 keys,
+    // e4m3: one sequence 34 us, blocks of 32 rows with the keys in parts 28; eight 48 and 44; with 256 rows each 58 and 81; 96 rows of 32 sequences over 2000 keys 63 and 97).
+    const long many_blocks = (rows + MANY_ROWS - 1) / MANY_ROWS, many_units = many_blocks * p->cache.kv_heads * p->batch;
+    if (rows > 64 && 4 * many_units >= device_cus()) {
+        const long blocks = many_blocks, tiles_y = (long)p->cache.kv_heads * p->batch, units = many_units;
+        const long want = many_shares((p->max_len + MANY_KEYS - 1) / MANY_KEYS, std::min(64l, 2l * device_cus() / units));
+        GP_REQUIRE(units * want < (1L << 31), "paged_attention: too large");
+        pl->many = ManyArgs{a.p, a.group, (int)blocks, (int)want, nullptr, nullptr};
+        if (want > 1) {
+            const size_t counters = ((size_t)units * sizeof(int) + 255) / 256 * 256;
+            pl->work_bytes = counters + (size_t)(units * want) * (p->cache.head_dim == 64 ? many_partial_floats<64>() : many_partial_floats<128>()) * sizeof(float);
+            pl->many.arrived = (int *)p->work;
+            pl->many.partial = (float *)((char *)p->work + counters);
+        }
+        pl->tiles_x = (int)(blocks * want);
+        pl->tiles_y = tiles_y;
+        return GP_SUCC;
+    }
     pl->nt = rows <= 16 ? 1 : 2;
     const long blocks = (rows + 16 * pl->nt - 1) / (16 * pl->nt), heads = blocks * p->cache.kv_heads, units = heads * p->batch;
     GP_REQUIRE(units < (1L << 30), "paged_attention: too large");
@@ -43,7 +63,7 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
     pl->tiles_x = p->batch;
     pl->tiles_y = heads;
     if (most > 4) {
-        pl->tiles_x = a.shares = (int)std::min((device_cus() + heads - 1) / heads, most * p->batch);
+        pl->tiles_x = a.shares = (int)std::min(std::max(1l, device_cus() / heads), most * p->batch);
         const size_t counters = ((size_t)units * sizeof(int) + 255) / 256 * 256;
         pl->work_bytes = counters + (size_t)heads * a.shares * 2 * 16 * pl->nt * (p->cache.head_dim + 2) * sizeof(float);
         a.arrived = (int *)p->work;
@@ -70,6 +90,15 @@ extern "C" int gp_launch_paged_attention(const gp_paged_attention_params *p, con
     if (int rc = plan_paged_attention(p, &pl)) return rc;
     GP_REQUIRE(pl.work_bytes == 0 || (p->work && aligned16(p->work) && p->work_bytes >= pl.work_bytes), "paged_attention: needs a workspace of %zu bytes, 16-byte aligned", pl.work_bytes);
     const bool e8 = p->cache.dtype == GP_E4M3, f16 = p->dtype == GP_F16;
+    if (pl.nt == 0) {
+        switch (p->cache.head_dim * 4 + e8 * 2 + f16) {
+#define GP_MANY(T, F16, D, E8) case D * 4 + E8 * 2 + F16: return launch_tiles(GP_KSET(paged_many_kernel<T, D, E8), pl.tiles_x, (int)pl.tiles_y, ctx, s, info, pl.many, many_lds_bytes<D>(), 1, MANY_NT);
+            GP_MANY(_Float16, 1, 64, 0) GP_MANY(__bf16, 0, 64, 0) GP_MANY(_Float16, 1, 64, 1) GP_MANY(__bf16, 0, 64, 1)
+            GP_MANY(_Float16, 1, 128, 0) GP_MANY(__bf16, 0, 128, 0) GP_MANY(_Float16, 1, 128, 1) GP_MANY(__bf16, 0, 128, 1)
+#undef GP_MANY
+        }
+        return GP_OUTOFRANGE;
+    }
     const int key = p->cache.head_dim * 8 + e8 * 4 + f16 * 2 + (pl.nt == 2);
     switch (key) {
 #define GP_FEW(T, F16, D, E8, NT) case D * 8 + E8 * 4 + F16 * 2 + (NT == 2): return launch_tiles(GP_KSET(paged_few_kernel<T, D, E8, NT), pl.tiles_x, (int)pl.tiles_y, ctx, s, info, pl.few, few_lds_floats<NT, D>() * sizeof(float), 1, FEW_NT);
