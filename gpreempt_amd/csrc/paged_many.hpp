@@ -25,10 +25,10 @@ struct ManyArgs {
     int *arrived;    // workspace: a counter for every (head, sequence, row block), 0 between launches
     float *partial;  // ... and many_partial_floats for every part
 };
-// Parts of a block's `tiles` tiles of keys, at most: joining a part costs about as much as one and a half tiles, so as many parts as each has of those.
+// Parts of a block's `tiles` tiles of keys, at most: joining a part costs as much as a few tiles.
 __host__ __device__ inline int many_shares(long tiles, long most) {
     int n = 1;
-    while (n < most && 3l * (n + 1) * (n + 1) <= 2 * tiles) ++n;
+    while (n < most && 3l * (n + 1) * (n + 1) <= tiles) ++n;
     return n;
 }
 
@@ -127,6 +127,12 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
     // ---- ... and on to LDS ----
     auto kslot = [&](int row, int chunk) { return row * (D * 2) + (chunk ^ (row & (KCH - 1))) * 16; };
     auto vslot = [&](int d, int chunk) { return TILE_BYTES + d * (MANY_KEYS * 2) + (chunk ^ ((d ^ (d >> 3)) & 7)) * 16; };
+    // (what a lane reads, once for all tiles: 32 keys on, or 64 values on, and in the other buffer are constants away)
+    int kat[KSTEPS], vat[2][4];
+#pragma unroll
+    for (int k = 0; k < KSTEPS; ++k) kat[k] = kslot(l32, 2 * k + half);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { vat[0][u] = vslot(l32, 2 * u + half); vat[1][u] = vslot(32 + l32, 2 * u + half); }
     auto stage = [&](char *buf) {
 #pragma unroll
         for (int i = 0; i < KLOADS; ++i) {
@@ -168,10 +174,12 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         fetch(first_tile);
     }
     __syncthreads();  // (the previous tile's buffers are still being read)
-    if (tiles > first_tile) stage(lds + (first_tile & 1) * 2 * TILE_BYTES);
+    if (tiles > first_tile) stage(lds);
     __syncthreads();
-    for (int tile = first_tile; tile < tiles; ++tile) {
-        const char *buf = lds + (tile & 1) * 2 * TILE_BYTES;
+    // one tile of keys, in buffer BUF; the next one goes to the other
+    auto step = [&](int tile, auto buffer) {
+        constexpr int BUF = decltype(buffer)::value;
+        const char *buf = lds + BUF * 2 * TILE_BYTES;
         const int sub = (tile - first_tile) % 16 * 4, key0 = tile * MANY_KEYS;
         // what of the pages this tile's softmax needs, before they are looked up anew
         float ks[4], lv[4], iv[4];
@@ -196,7 +204,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
 #pragma unroll
             for (int v = 0; v < 16; ++v) x[i][v] = 0.f;
 #pragma unroll
-            for (int k = 0; k < KSTEPS; ++k) Elem<T>::mma(*(const u32x4 *)(buf + kslot(i * 32 + l32, 2 * k + half)), q[k], x[i]);
+            for (int k = 0; k < KSTEPS; ++k) Elem<T>::mma(*(const u32x4 *)(buf + kat[k] + i * 32 * D * 2), q[k], x[i]);
         }
         if (!whole) {
 #pragma unroll
@@ -241,10 +249,14 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             l = E8 ? fmaf(part, iv[u], l) : l + part;
             // ---- O^T += V^T P^T, 16 keys ----
 #pragma unroll
-            for (int i = 0; i < DB; ++i) Elem<T>::mma(*(const u32x4 *)(buf + vslot(i * 32 + l32, 2 * u + half)), __builtin_bit_cast(u32x4, pb), o[i]);
+            for (int i = 0; i < DB; ++i) Elem<T>::mma(*(const u32x4 *)(buf + vat[i % 2][u] + i / 2 * 64 * MANY_KEYS * 2), __builtin_bit_cast(u32x4, pb), o[i]);
         }
-        if (tile + 1 < tiles) stage(lds + ((tile + 1) & 1) * 2 * TILE_BYTES);
+        if (tile + 1 < tiles) stage(lds + (1 - BUF) * 2 * TILE_BYTES);
         __syncthreads();
+    };
+    for (int tile = first_tile; tile < tiles; tile += 2) {
+        step(tile, IntC<0>());
+        if (tile + 1 < tiles) step(tile + 1, IntC<1>());
     }
     // ---- o[i][v] belongs to this lane's query and value 32 i + 8 (v / 4) + 4 half + v % 4 ----
     l += __shfl_xor(l, 32, 64);
