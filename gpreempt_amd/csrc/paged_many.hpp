@@ -97,6 +97,9 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             iv_l = 1.f / vs;
         }
     };
+    // what of them a tile needs while it is worked on (in scalar registers)
+    struct Info { int pages[4], vbound; float ks[4], lv[4], iv[4]; };
+    auto scalar = [](float v, int at) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), at)); };
     // ---- from the pages to registers: thread (tid % 16, tid / 16).  Keys: 16 keys at a time, a row's 16 (8) chunks side by side.  Values: four keys of the
     // wavefront's 16, eight (four) values ----
     constexpr int KLOADS = E8 ? 2 * D / 128 : 4 * D / 128;  // 16-byte loads of a thread for the keys
@@ -106,10 +109,18 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
     static_assert(KROWS * KLOADS == MANY_KEYS, "the loads of a tile's keys");
     u32x4 kr[KLOADS];
     VRow vr[4];
-    bool vthere[4];
     auto block_at = [&](int page, int key) { return (((long)(page < 0 ? 0 : page) * p.cache.kv_heads + kvh) * P + (key & (P - 1))) * D * ES; };
     auto fetch = [&](int tile) {
         const int sub = (tile - first_tile) % 16 * 4;
+        if (sub == 0) look_up(tile);
+        Info info;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            info.pages[i] = __builtin_amdgcn_readlane(page_l, sub + i);
+            info.ks[i] = E8 ? scalar(ks_l, sub + i) : scale2;
+            info.lv[i] = E8 ? scalar(lv_l, sub + i) : 0.f;
+            info.iv[i] = E8 ? scalar(iv_l, sub + i) : 1.f;
+        }
 #pragma unroll
         for (int i = 0; i < KLOADS; ++i) {
             const int row = i * KROWS + tid / (D * ES / 16), chunk = tid % (D * ES / 16);
@@ -119,10 +130,9 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         const int page = __builtin_amdgcn_readlane(page_l, sub + wave), key0 = tile * MANY_KEYS + wave * 16 + lane / 16 * 4;
         const char *at = (const char *)p.cache.v + block_at(page, key0) + lane % 16 * (VV * ES);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            vr[e] = *(const VRow *)(at + e * D * ES);
-            vthere[e] = page >= 0 && key0 + e < bound;
-        }
+        for (int e = 0; e < 4; ++e) vr[e] = *(const VRow *)(at + e * D * ES);
+        info.vbound = page >= 0 ? bound : 0;
+        return info;
     };
     // ---- ... and on to LDS ----
     auto kslot = [&](int row, int chunk) { return row * (D * 2) + (chunk ^ (row & (KCH - 1))) * 16; };
@@ -133,7 +143,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
     for (int k = 0; k < KSTEPS; ++k) kat[k] = kslot(l32, 2 * k + half);
 #pragma unroll
     for (int u = 0; u < 4; ++u) { vat[0][u] = vslot(l32, 2 * u + half); vat[1][u] = vslot(32 + l32, 2 * u + half); }
-    auto stage = [&](char *buf) {
+    auto stage = [&](char *buf, int tile, const Info &info) {
 #pragma unroll
         for (int i = 0; i < KLOADS; ++i) {
             const int row = i * KROWS + tid / (D * ES / 16), chunk = tid % (D * ES / 16);
@@ -147,7 +157,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (!vthere[e]) vr[e] = VRow(0);
+            if (tile * MANY_KEYS + wave * 16 + lane / 16 * 4 + e >= info.vbound) vr[e] = VRow(0);
         // keys 4 g .. 4 g + 3 of the wavefront's 16: half g % 2, and there the first four or the second
         const int g = lane / 16, chunk = 2 * wave + g % 2, d0 = lane % 16 * VV;
 #pragma unroll
@@ -169,34 +179,21 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         }
     };
 
-    if (tiles > first_tile) {
-        look_up(first_tile);
-        fetch(first_tile);
-    }
+    // A tile's way: fetched two steps ahead, put into LDS one step ahead, between the matrix instructions of the scores
+    Info now = {}, next = {};
     __syncthreads();  // (the previous tile's buffers are still being read)
-    if (tiles > first_tile) stage(lds);
+    if (tiles > first_tile) {
+        now = fetch(first_tile);
+        stage(lds, first_tile, now);
+        if (first_tile + 1 < tiles) next = fetch(first_tile + 1);
+    }
     __syncthreads();
-    // one tile of keys, in buffer BUF; the next one goes to the other
+    // one tile of keys, in buffer BUF
     auto step = [&](int tile, auto buffer) {
         constexpr int BUF = decltype(buffer)::value;
         const char *buf = lds + BUF * 2 * TILE_BYTES;
-        const int sub = (tile - first_tile) % 16 * 4, key0 = tile * MANY_KEYS;
-        // what of the pages this tile's softmax needs, before they are looked up anew
-        float ks[4], lv[4], iv[4];
-        bool whole = key0 + MANY_KEYS <= kmin;
-        int pages[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            pages[i] = __builtin_amdgcn_readlane(page_l, sub + i);
-            whole = whole && pages[i] >= 0;
-            ks[i] = E8 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks_l), sub + i)) : scale2;
-            lv[i] = E8 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, lv_l), sub + i)) : 0.f;
-            iv[i] = E8 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, iv_l), sub + i)) : 1.f;
-        }
-        if (tile + 1 < tiles) {
-            if ((tile + 1 - first_tile) % 16 == 0) look_up(tile + 1);
-            fetch(tile + 1);
-        }
+        const int key0 = tile * MANY_KEYS;
+        const bool whole = key0 + MANY_KEYS <= kmin && (now.pages[0] | now.pages[1] | now.pages[2] | now.pages[3]) >= 0;
         // ---- scores ----
         f32x16 x[2];
 #pragma unroll
@@ -206,12 +203,24 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
 #pragma unroll
             for (int k = 0; k < KSTEPS; ++k) Elem<T>::mma(*(const u32x4 *)(buf + kat[k] + i * 32 * D * 2), q[k], x[i]);
         }
+        stage(lds + (1 - BUF) * 2 * TILE_BYTES, tile + 1, next);  // (behind the last tile: the last one again, which nobody reads)
+        // (the order that the compiler is asked for: operands four ahead, a few of the other instructions behind every matrix instruction; prompts of 2600 to 4096 tokens, 32
+        // heads of 128, bf16: 708 us without, 681 with)
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // reads of LDS
+#pragma unroll
+        for (int k = 0; k < 2 * KSTEPS; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix instructions
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);  // vector instructions
+        }
+        Info later = {};
+        if (tile + 2 < tiles) later = fetch(tile + 2);
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int v = 0; v < 16; ++v)
-                    if (pages[2 * i + v / 8] < 0 || key0 + i * 32 + 8 * (v / 4) + 4 * half + v % 4 >= seen) x[i][v] = -INFINITY;
+                    if (now.pages[2 * i + v / 8] < 0 || key0 + i * 32 + 8 * (v / 4) + 4 * half + v % 4 >= seen) x[i][v] = -INFINITY;
         }
         // ---- running maximum (raised only when it is exceeded 256-fold, which the types and the sums have room for) and sum.  8 bits: the logarithm of the
         // values' scale is part of the exponent, so that what is rounded to 16 bits is the probability times that scale; the sum takes it back out ----
@@ -221,12 +230,12 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             float most = x[u / 2][8 * (u % 2)];
 #pragma unroll
             for (int v = 1; v < 8; ++v) most = fmaxf(most, x[u / 2][8 * (u % 2) + v]);
-            top = fmaxf(top, fmaf(most, ks[u], lv[u]));
+            top = fmaxf(top, fmaf(most, now.ks[u], now.lv[u]));
         }
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         if (__any(top > m + 8.f)) {
-            const float now = fmaxf(m, top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
-            m = now;
+            const float high = fmaxf(m, top), f = high == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - high);
+            m = high;
             l *= f;
 #pragma unroll
             for (int i = 0; i < DB; ++i)
@@ -236,23 +245,24 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const float off = lv[u] - base;
+            const float off = now.lv[u] - base;
             float part = 0.f;
             typedef T tx8 __attribute__((ext_vector_type(8)));
             tx8 pb;
 #pragma unroll
             for (int v = 0; v < 8; ++v) {
-                const float y = __builtin_amdgcn_exp2f(fmaf(x[u / 2][8 * (u % 2) + v], ks[u], off));
+                const float y = __builtin_amdgcn_exp2f(fmaf(x[u / 2][8 * (u % 2) + v], now.ks[u], off));
                 part += y;
                 pb[v] = Elem<T>::from_f(y);
             }
-            l = E8 ? fmaf(part, iv[u], l) : l + part;
+            l = E8 ? fmaf(part, now.iv[u], l) : l + part;
             // ---- O^T += V^T P^T, 16 keys ----
 #pragma unroll
             for (int i = 0; i < DB; ++i) Elem<T>::mma(*(const u32x4 *)(buf + vat[i % 2][u] + i / 2 * 64 * MANY_KEYS * 2), __builtin_bit_cast(u32x4, pb), o[i]);
         }
-        if (tile + 1 < tiles) stage(lds + (1 - BUF) * 2 * TILE_BYTES);
         __syncthreads();
+        now = next;
+        next = later;
     };
     for (int tile = first_tile; tile < tiles; tile += 2) {
         step(tile, IntC<0>());
