@@ -440,3 +440,252 @@ def test_logprobs_of_rows_of_a_kind(gp, dt, vocab):
         # the largest value next to the lowest: one takes everything; the lowest everywhere: all are alike
         assert got["logprob"][10] == 0 and got["entropy"][10] == 0 and got["ids"][10, :2].tolist() == [5, 0] and got["logprob"][3] == 0
         assert abs(float(got["logprob"][2]) + math.log(vocab)) < 1e-5 * math.log(vocab) and got["ids"][2].tolist() == list(range(20))
+
+
+# ---- the forms that a call's size chooses -----------------------------------------------------------------------------------
+
+MANY = [
+    # lens, news, page, heads, kv_heads, dim, causal: blocks of 128 rows, which take 64 of them or more (heads x sequences x blocks)
+    ([1300, 1100, 900, 70], [70, 66, 80, 70], 16, 16, 16, 64, True),       # keys in two parts; a sequence of nothing but its new tokens
+    ([1300, 0, 64, 650], [70, 3, 0, 129], 64, 16, 16, 64, False),          # no keys, no rows, two blocks of rows
+    ([700, 130, 65, 1], [50, 130, 2, 1], 128, 48, 16, 128, True),          # three query heads to a head: tokens that straddle blocks
+    ([40, 300], [67, 65], 32, 32, 32, 128, True),                          # the first has tokens in front of position 0
+]
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_attention_of_many_rows(gp, dt, cache, case):
+    lens, news, page, heads, kv_heads, dim, causal = MANY[case]
+    seqs = S.Sequences(lens, news, page, gen(40 + case), tail=1)
+    a = Attend(gp, dt, dt if cache == "same" else cache, seqs, heads, kv_heads, dim, causal, 300 + case, scale=-0.3 if case == 2 else None, pad=8 * (case % 2))
+    info = a.launch()
+    assert info.block == 256 and info.total_tiles % (kv_heads * len(lens) * -(-seqs.max_new * heads // kv_heads // 128)) == 0
+    a.check()
+    first = a.left()
+    a.launch()
+    assert torch.equal(a.left(), first)
+
+
+def test_attention_of_many_rows_and_keys(gp):
+    """more heads than parts would help: every block walks over all keys, more than sixteen tiles of them; pages that are not there among them"""
+    holes = {(0, 5): -1, (0, 16): 10 ** 6, (2, 0): -1}
+    seqs = S.Sequences([1200, 3, 70, 0, 1, 2, 30, 9], [67, 1, 3, 0, 1, 2, 0, 1], 64, gen(50), holes=holes)
+    a = Attend(gp, "bf16", "e4m3", seqs, 64, 64, 64, True, 51)
+    a.launch()
+    a.check()
+
+
+def test_attention_of_more_sequences_than_a_wavefront_has_lanes(gp):
+    """keys in equal parts over 70 sequences, one long and the others short, some of them empty"""
+    lens = [1300] + [i * 37 % 41 for i in range(69)]
+    for news in (None, [2] + [i % 3 for i in range(69)]):
+        seqs = S.Sequences(lens, news, 16, gen(52))
+        a = Attend(gp, "f16", "e4m3", seqs, 2, 1, 64, True, 53)
+        a.launch()
+        a.check()
+        first = a.left()
+        a.launch()
+        assert torch.equal(a.left(), first)
+
+
+def test_attention_of_a_part_longer_than_a_wavefronts_pages(gp):
+    """256 heads: one part each, of more keys than 64 tiles for each wavefront"""
+    seqs = S.Sequences([4400], None, 128, gen(54))
+    a = Attend(gp, "f16", "e4m3", seqs, 256, 256, 64, True, 55)
+    info = a.launch()
+    assert info.total_tiles == 256
+    a.check()
+
+
+# ---- stopped and resumed, other streams, graphs -------------------------------------------------------------------------------
+
+
+def calls(gp):
+    """(a call, its outputs as bytes) of every kernel, with several tiles each"""
+    out = []
+    for cache, news in (("f16", None), ("e4m3", [100, 60, 33])):
+        seqs = S.Sequences([200, 160, 133], news, 16, gen(60))
+        out.append(Append(gp, "f16", cache, seqs, 4, 4, 64, 64, "halves", 61))
+    out.append(Attend(gp, "f16", "f16", S.Sequences([2000, 700, 1], None, 64, gen(62)), 8, 4, 64, True, 63))
+    out.append(Attend(gp, "bf16", "e4m3", S.Sequences([900, 300, 1500], [3, 1, 4], 32, gen(64)), 8, 4, 128, True, 65))
+    out.append(Attend(gp, "bf16", "e4m3", S.Sequences([1300, 1100, 900, 70], [70, 66, 80, 70], 64, gen(66)), 16, 16, 64, True, 67))
+    x = torch.randn((3, 70000), generator=gen(68)).half()
+    out.append(Logprobs(gp, "f16", x, torch.tensor([1, 2, 3]), 20))
+    out.append(Logprobs(gp, "f16", torch.randn((40, 900), generator=gen(69)).half(), torch.arange(40), 5))
+    return out
+
+
+def bits(left):
+    return [x.contiguous().view(torch.uint8) for x in (left.values() if isinstance(left, dict) else [left])]
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(bits(a), bits(b)))
+
+
+def clean(call):
+    """What the call writes, as before its first launch"""
+    if isinstance(call, Append):
+        for n, x in call.cache.items():
+            call.dev[n].copy_(x)
+        call.q_out.fill_(7.0)
+    elif isinstance(call, Attend):
+        call.out.fill_(7.0)
+    else:
+        for x in call.out.values():
+            x.fill_(7)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("which", range(7))
+def test_stopped_and_resumed_has_the_bits_of_an_uninterrupted_launch(gp, which):
+    call = calls(gp)[which]
+    call.launch()
+    want = call.left()
+    for groups in (1, 32):
+        flag = gp.Flag()
+        st = gp.BlpState(1, flag, groups)
+        clean(call)
+        # (one counter: two workgroups, the second claim raises the flag; many: a bit or a count per workgroup)
+        limit = 2 if groups == 1 else 0
+        call.launch(st.ctx(inject_at=1, max_workgroups=limit, poll_every=1))
+        call.left()
+        assert flag.get() == 1
+        if groups == 1:
+            assert st.stop_index() == 0 and not same(call.left(), want)
+        flag.set(0)
+        st.clear_stop()
+        call.launch(st.ctx(max_workgroups=limit, poll_every=1))
+        assert same(call.left(), want), groups
+    # ... and the next launch finds its workspace as it needs it
+    clean(call)
+    call.launch()
+    assert same(call.left(), want)
+
+
+def test_two_streams_at_once(gp):
+    """each call with another of its kind on another stream, each with its own workspace and outputs"""
+    first, second = calls(gp), calls(gp)
+    want = []
+    for c in first:
+        c.launch()
+        want.append(c.left())
+        clean(c)
+    streams = [gp.Stream(0), gp.Stream(1)]
+    for _ in range(3):
+        for a, b in zip(first, second):
+            a.launch(stream=streams[0])
+            b.launch(stream=streams[1])
+        for s in streams:
+            s.sync()
+        for a, b, w in zip(first, second, want):
+            assert same(a.left(), w) and same(b.left(), w)
+            clean(a)
+            clean(b)
+    for s in streams:
+        s.destroy()
+
+
+def test_captured_and_replayed(gp):
+    """a step in a graph: replays with the program's own work in between, with other contents of the same buffers (lengths among them) every time"""
+    stream = gp.Stream(0)
+    news = None
+    seqs = S.Sequences([1800, 900, 300], news, 32, gen(70))
+    app, att = Append(gp, "bf16", "e4m3", seqs, 8, 4, 64, 64, "halves", 71), Attend(gp, "bf16", "e4m3", seqs, 8, 4, 64, True, 72)
+    lp = Logprobs(gp, "f32", torch.randn((2, 70000), generator=gen(73)), torch.tensor([5, 6]), 7)
+    for c in (app, att, lp):  # (what a first launch sets up is not part of the graph)
+        c.launch(stream=stream)
+    stream.sync()
+    graph = gp.vp()
+    gp.check(gp.lib().gp_graph_begin(stream.h))
+    for c in (app, att, lp):
+        c.launch(stream=stream)
+    gp.check(gp.lib().gp_graph_end(stream.h, gp.C.byref(graph)))
+    for i in range(4):
+        lens = [1800 - 311 * i, 900 - i, 300 + 200 * i]
+        for c in (app, att):
+            c.dev["kv_len"].copy_(torch.tensor(lens, dtype=torch.int32))
+        att.dev["q"].copy_(torch.randn(att.q.shape, generator=gen(80 + i)).bfloat16())
+        lp.room.copy_(torch.randn(lp.room.shape, generator=gen(90 + i)))
+        for name in ("k", "v", "k_scale", "v_scale"):  # (the second length is past what was filled: plain values)
+            app.dev[name].copy_(app.cache[name].nan_to_num(0.5) if name in ("k_scale", "v_scale") else app.cache[name])
+            att.dev[name].copy_(att.cache[name])
+        for c in (app, att, lp):
+            clean(c) if c is not app else app.q_out.fill_(7.0)
+        torch.cuda.synchronize()
+        before = {n: app.dev[n].clone() for n in app.cache}
+        gp.check(gp.lib().gp_graph_launch(graph, stream.h))
+        stream.sync()
+        got = [app.left(), att.left(), lp.left()]
+        for n, x in before.items():
+            app.dev[n].copy_(x)
+        for c in (app, att, lp):
+            c.launch()
+        for g, c in zip(got, (app, att, lp)):
+            assert same(g, c.left()), (i, type(c))
+    gp.check(gp.lib().gp_graph_destroy(graph))
+    stream.destroy()
+
+
+# ---- together -------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+def test_a_decoder_steps(gp, cache):
+    """Two prompts, then eight steps of one token: every step appends, attends to what the cache then holds, projects (gp_launch_gemm) and scores, on
+    one stream without a wait in between; each step's attention and scores against 64 bits, from the cache as it is."""
+    heads, kv_heads, dim, page, vocab = 4, 2, 64, 16, 1000
+    rng = gen(100)
+    stream = gp.Stream(0)
+    lens, news, steps = [37, 5], [37, 5], 8
+    W = (0.05 * torch.randn((vocab, heads * dim), generator=rng)).half().cuda()
+    seqs = S.Sequences([n + steps for n in lens], None, page, gen(101))
+    pool = S.cache_of(seqs, kv_heads, dim, cache, rng)  # (its values are old ones: nothing of them may show)
+    dev = {n: x.cuda() for n, x in pool.items()}
+    inv_freq = 10000.0 ** (-torch.arange(0, dim, 2) / dim)
+    freq = inv_freq.float().cuda()
+    keep = []
+    checks = []
+    for step in range(steps + 1):
+        if step:
+            lens, news = [n + 1 for n in lens], [1, 1]
+        s = S.Sequences(lens, None if step else news, page, gen(101), width=seqs.width)
+        s.table, s.pages = seqs.table, seqs.pages
+        d = {**s.device(), **dev}
+        qkv = torch.randn((s.tokens, (heads + 2 * kv_heads) * dim), generator=rng).half().cuda()
+        q, out = (torch.empty((s.tokens, heads * dim), dtype=torch.half, device="cuda") for _ in range(2))
+        logits = torch.empty((s.tokens, vocab), dtype=torch.half, device="cuda")
+        tokens = torch.randint(0, vocab, (s.tokens,), generator=rng).cuda()
+        lp = {n: torch.empty(s.tokens, device="cuda") for n in ("logprob", "entropy")}
+        ids, vals = torch.empty((s.tokens, 4), dtype=torch.int32, device="cuda"), torch.empty((s.tokens, 4), device="cuda")
+        c = S.cache_params(gp, d, cache, kv_heads, dim, s)
+        at, es = qkv.data_ptr(), 2 * dim
+        torch.cuda.synchronize()  # (the inputs were made on torch's stream)
+        gp.launch("gp_launch_kv_append", gp.KvAppendParams(dtype=gp.F16, cache=c, **S.sequence_params(s, d), heads=heads, q=at, k=at + es * heads, v=at + es * (heads + kv_heads),
+                                                           ld_qkv=qkv.shape[1], q_out=q.data_ptr(), ld_q_out=heads * dim, inv_freq=freq.data_ptr(), rot_dim=dim, rot_pairs=gp.ROT_HALVES), stream=stream)
+        gp.launch("gp_launch_paged_attention", gp.PagedAttentionParams(dtype=gp.F16, cache=c, **S.sequence_params(s, d), heads=heads, max_len=64, q=q.data_ptr(), ld_q=heads * dim,
+                                                                       out=out.data_ptr(), ld_out=heads * dim, scale=0.125, causal=1), stream=stream)
+        gp.launch("gp_launch_gemm", gp.GemmParams(dtype=gp.F16, M=s.tokens, N=vocab, K=heads * dim, A=out.data_ptr(), lda=heads * dim, B=W.data_ptr(), ldb=heads * dim, b_is_nk=1,
+                                                  C=logits.data_ptr(), ldc=vocab, alpha=1.0, batch=1), stream=stream)
+        gp.launch("gp_launch_token_logprobs", gp.TokenLogprobsParams(dtype=gp.F16, rows=s.tokens, vocab=vocab, logits=logits.data_ptr(), ld=vocab, tokens=tokens.data_ptr(), scale=1.0,
+                                                                     logprob=lp["logprob"].data_ptr(), entropy=lp["entropy"].data_ptr(), top=4, top_ids=ids.data_ptr(), top_logprobs=vals.data_ptr()), stream=stream)
+        keep.append((d, qkv, tokens))
+        stream.sync()
+        now = {n: x.cpu() for n, x in dev.items()}
+        # the keys that this step appended, rotated in 64 bits, are in the cache up to its rounding
+        for b in range(2):
+            for row, pos in s.rows(b):
+                page_, slot = s.place(b, pos)
+                ref = S.turned(qkv[row, heads * dim: (heads + kv_heads) * dim].cpu().double().view(kv_heads, dim), pos, inv_freq.float(), dim, "halves")
+                assert ((S.values(now, "k")[page_, :, slot] - ref).abs() <= (2.0 ** -11 if cache == "f16" else 2.0 ** -4) * ref.abs() + (2e-5 if cache == "f16" else 2.0 ** -6)).all()
+        want, mass, most = S.attend(s, now, q.cpu().view(s.tokens, heads, dim), 0.125, True)
+        for row, ref in want.items():
+            # (as for the attention alone: two roundings to fp16, a score's products and sums in fp32)
+            allowed = 2.0 ** -11 * (mass[row] + ref.abs()) + 4 * (dim + 8) * 2.0 ** -24 * max(most, 1.0) * mass[row] + 2.0 ** -24 * (1 + 64 * mass[row].amax())
+            assert ((out[row].cpu().view(heads, dim).double() - ref).abs() <= allowed).all()
+        said, entropy, wids, wvals = S.logprobs(logits.cpu(), tokens.cpu(), 1.0, 4)
+        assert (lp["logprob"].cpu().double() - said).abs().max() < 4e-6 and (lp["entropy"].cpu().double() - entropy).abs().max() < 2e-5
+        assert torch.equal(ids.cpu(), wids) and (vals.cpu().double() - wvals).abs().max() < 4e-6
+    stream.destroy()
