@@ -69,15 +69,15 @@ __device__ __forceinline__ void rotate(float (&x)[16], const f32x2 (&cs)[8], int
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float a = x[i], b = x[8 + i];
-            x[i] = a * cs[i][0] - b * cs[i][1];
-            x[8 + i] = b * cs[i][0] + a * cs[i][1];
+            x[i] = rounded(fmaf(a, cs[i][0], -(b * cs[i][1])));
+            x[8 + i] = rounded(fmaf(b, cs[i][0], a * cs[i][1]));
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = a * cs[i][0] - b * cs[i][1];
-            x[2 * i + 1] = b * cs[i][0] + a * cs[i][1];
+            x[2 * i] = rounded(fmaf(a, cs[i][0], -(b * cs[i][1])));
+            x[2 * i + 1] = rounded(fmaf(b, cs[i][0], a * cs[i][1]));
         }
     }
 }

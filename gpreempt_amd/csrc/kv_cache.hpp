@@ -18,6 +18,12 @@ inline int check_kv_cache(const gp_kv_cache &c, int dtype, const char *who) {
     return GP_SUCC;
 }
 
+// keeps the compiler from making one operation, with a single rounding, of the arithmetic in front and a conversion behind
+__device__ __forceinline__ float rounded(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 // eight e4m3 values of 8 bytes

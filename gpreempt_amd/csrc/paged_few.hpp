@@ -85,6 +85,9 @@ __device__ __forceinline__ int share_of(long x, long units, long shares) { retur
 // first_share, last_share: the parts that the sequence's keys are spread over.
 template <typename T, int D, bool E8, int NT>
 __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequence &f, int b, int hr, int c0, int c1, float *slot, int first_share, int last_share, float *lds) {
+    // (products and sums are contracted where the code says so and nowhere else, and rounded to fp32 before they are rounded to 16 bits, so that the
+    // plain and the preemptible kernels give the same bits)
+#pragma clang fp contract(off)
     const gp_paged_attention_params &p = a.p;
     constexpr int KS = few_step_keys<E8>(), TILES = KS / 16, PAIRS = KS / 32;  // keys of a wavefront's step
     constexpr int ROWS = 16 * NT, VD = D / 16, KL = E8 ? D / 64 : D / 32;
@@ -315,7 +318,7 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
         typedef T tx4 __attribute__((ext_vector_type(4)));
         tx4 y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f(v[e] * inv);
+        for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f(rounded(v[e] * inv));
         *(tx4 *)((T *)p.out + (s.row0 + token) * p.ld_out + ((long)kvh * a.group + hg) * D + d) = y;
     };
     const int parts = last_share - first_share + 1;
@@ -330,7 +333,7 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
         for (int w = 0; w < FEW_WAVES; ++w) {
             const f32x2 x = *(const f32x2 *)(ml + 2 * (w * ROWS + r));
             const float f = __builtin_amdgcn_exp2f(x[0] - base);
-            sum += f * x[1];
+            sum = fmaf(f, x[1], sum);
             const f32x4 y = *(const f32x4 *)(lds + (w * ROWS + r) * LD + d);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = fmaf(f, y[e], v[e]);
@@ -393,7 +396,7 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
                     if (i + e >= n) break;
                     const f32x2 ms = *(const f32x2 *)(lds + 2 * ((i + e) * ROWS + r));
                     const float f = __builtin_amdgcn_exp2f(ms[0] - base);
-                    sum[k] += f * ms[1];
+                    sum[k] = fmaf(f, ms[1], sum[k]);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) v[k][c] = fmaf(f, y[e][c / 2][c % 2], v[k][c]);
                 }

@@ -37,6 +37,7 @@ template <int D> constexpr size_t many_lds_bytes() { return 2 * 2 * (size_t)MANY
 
 template <typename T, int D, bool E8>
 __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *lds) {
+#pragma clang fp contract(off)  // (as in attend_stretch)
     const gp_paged_attention_params &p = a.p;
     constexpr int ES = E8 ? 1 : 2, DB = D / 32, KSTEPS = D / 16;
     constexpr int KCH = D / 8;                              // 16-byte chunks of a key's row in LDS
@@ -300,7 +301,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             const float mk = y[8 * DB][0], now = fmaxf(m, mk), base = now == -INFINITY ? 0.f : now;
             const float f = __builtin_amdgcn_exp2f(m - base), fk = __builtin_amdgcn_exp2f(mk - base);
             m = now;
-            l = l * f + y[8 * DB][1] * fk;
+            l = fmaf(l, f, y[8 * DB][1] * fk);
 #pragma unroll
             for (int i = 0; i < DB; ++i)
 #pragma unroll
@@ -317,7 +318,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             typedef T tx4 __attribute__((ext_vector_type(4)));
             tx4 y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f(o[i][v + e] * inv);
+            for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f(rounded(o[i][v + e] * inv));
             *(tx4 *)(out + 32 * i + 2 * v) = y;
         }
 }

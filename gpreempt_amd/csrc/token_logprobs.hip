@@ -128,6 +128,7 @@ __device__ __forceinline__ void pick(LogprobsLds &l, int which, int count, int t
 
 template <typename T>
 __device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, LogprobsLds &l) {
+#pragma clang fp contract(off)  // (contracted where the code says so and nowhere else: the plain and the preemptible kernels give the same bits)
     const gp_token_logprobs_params &p = a.p;
     const int tid = threadIdx.x, wave = tid >> 6, top = p.top, vocab = p.vocab;
     const long r = t.y;

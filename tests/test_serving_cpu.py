@@ -111,6 +111,22 @@ def test_log_probabilities_that_are_refused(change, says):
     refused("gp_launch_token_logprobs", logprobs(**change), says)
 
 
+def test_workspaces_that_are_refused():
+    """what is cut into parts needs one; what is not does without"""
+    n = C.c_size_t()
+    for entry, size, p in (("gp_launch_paged_attention", "gp_paged_attention_work_bytes", attend(max_len=5000)),
+                           ("gp_launch_paged_attention", "gp_paged_attention_work_bytes", attend(max_len=5000, heads=128, cache=cache(kv_heads=64), ld_q=8192, ld_out=8192, max_new=70)),
+                           ("gp_launch_token_logprobs", "gp_token_logprobs_work_bytes", logprobs(vocab=200000, ld=200000))):
+        gp.check(getattr(gp.lib(), size)(C.byref(p), C.byref(n)))
+        assert n.value > 0
+        for work, room in ((None, n.value), (AT, n.value - 1), (AT + 8, n.value)):
+            p.work, p.work_bytes = work, room
+            refused(entry, p, "workspace")
+    for size, p in (("gp_paged_attention_work_bytes", attend()), ("gp_token_logprobs_work_bytes", logprobs()), ("gp_token_logprobs_work_bytes", logprobs(rows=1000, vocab=200000, ld=200000))):
+        gp.check(getattr(gp.lib(), size)(C.byref(p), C.byref(n)))
+        assert n.value == 0
+
+
 def test_null_params():
     for entry in ("gp_launch_kv_append", "gp_launch_paged_attention", "gp_launch_token_logprobs"):
         assert getattr(gp.lib(), entry)(None, None, None, None) == gp.OUTOFRANGE

@@ -383,6 +383,8 @@ LOGPROBS = [
     (1, 30522, 5, 1.0, None, 0),
     (3, 65537, 32, 1.0, 65600, 0),
     (600, 300, 3, 1.0, None, 0),
+    (2, 8, 3, 1.0, None, 0), (2, 9, 4, 1.0, 16, 1), (1, 16384, 6, 1.0, None, 0), (2, 16385, 32, 1.0, None, 1),  # around a chunk, and around a tile
+    (2, 131072 + 8, 20, 1.0, None, 0),  # in parts
 ]
 
 
@@ -405,7 +407,7 @@ def test_logprobs_match_their_definition(gp, dt, case):
 
 
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("vocab", [100, 9001, 40000])
+@pytest.mark.parametrize("vocab", [100, 9001, 40000, 70000])
 def test_logprobs_of_rows_of_a_kind(gp, dt, vocab):
     """rows that are masked all over, or but for a few, or with the type's lowest value; equal, rising and falling ones; zeros of both signs; NaN and infinity"""
     low = torch.finfo(S.TORCH[dt]).min
@@ -440,6 +442,29 @@ def test_logprobs_of_rows_of_a_kind(gp, dt, vocab):
         # the largest value next to the lowest: one takes everything; the lowest everywhere: all are alike
         assert got["logprob"][10] == 0 and got["entropy"][10] == 0 and got["ids"][10, :2].tolist() == [5, 0] and got["logprob"][3] == 0
         assert abs(float(got["logprob"][2]) + math.log(vocab)) < 1e-5 * math.log(vocab) and got["ids"][2].tolist() == list(range(20))
+
+
+def test_logprobs_of_more_tiles_than_are_kept_apart(gp):
+    """as many rows as there are compute units, 33 tiles each: the first and the last share their groups' largest logits"""
+    vocab = 32 * 16384 + 77
+    x = torch.randn((256, vocab), generator=torch.Generator(device="cuda").manual_seed(5), device="cuda", dtype=torch.half)
+    x[3, 5], x[3, vocab - 3], x[7, 16384 * 32 + 1] = 9.0, 9.0, 8.0
+    tokens = torch.arange(256) * 2000
+    out = {n: torch.empty(256, device="cuda") for n in ("logprob", "entropy")}
+    ids, values = torch.empty((256, 12), dtype=torch.int32, device="cuda"), torch.empty((256, 12), device="cuda")
+    t = tokens.cuda()
+    p = gp.TokenLogprobsParams(dtype=gp.F16, rows=256, vocab=vocab, logits=x.data_ptr(), ld=vocab, tokens=t.data_ptr(), scale=1.0, logprob=out["logprob"].data_ptr(),
+                               entropy=out["entropy"].data_ptr(), top=12, top_ids=ids.data_ptr(), top_logprobs=values.data_ptr())
+    assert gp.launch("gp_launch_token_logprobs", p).total_tiles == 256
+    torch.cuda.synchronize()
+    for r in (0, 3, 7, 255):
+        lp = torch.log_softmax(x[r].double(), 0)
+        order = torch.sort(x[r].double(), descending=True, stable=True).indices[:12]
+        assert torch.equal(ids[r].long(), order)
+        # a thread adds 1056 exponentials in turn, of fp32's half unit each
+        near = 1100 * 2.0 ** -24 + 16 * 2.0 ** -21
+        assert (values[r].double() - lp[order]).abs().max() < near and abs(float(out["logprob"][r]) - float(lp[tokens[r]])) < near
+        assert abs(float(out["entropy"][r]) + float((lp.exp() * lp).sum())) < 2 * near * 14
 
 
 # ---- the forms that a call's size chooses -----------------------------------------------------------------------------------
