@@ -319,6 +319,21 @@ def test_attention_with_scales_far_apart(gp, news):
     a.check()
 
 
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+@pytest.mark.parametrize("news", [[1, 2, 0], [0, 0, 0]])
+@pytest.mark.parametrize("heads, max_new", [(2, 50), (8, 50), (8, 800)])
+def test_max_new_is_only_a_bound(gp, heads, max_new, news, cache):
+    """blocks of rows that no sequence has any rows in, a batch without new tokens among them: nothing is written there, and the launch ends"""
+    seqs = S.Sequences([1500, 2100, 40], news, 64, gen(19), tail=3, max_new=max_new)
+    a = Attend(gp, "f16", cache, seqs, heads, 2, 64, True, 20)
+    a.launch()
+    a.check()
+    for dt in DTS:
+        b = Append(gp, dt, "e4m3" if cache == "e4m3" else dt, seqs, heads, 2, 64, 64, "halves", 21)
+        b.launch()
+        b.check()
+
+
 # ---- log probabilities -----------------------------------------------------------------------------------------------------
 
 
