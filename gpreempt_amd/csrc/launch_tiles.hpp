@@ -6,6 +6,11 @@
 
 namespace gp {
 
+// Where parts of a result are joined by whoever comes last: the workspace begins with the counters, one for every compute unit at most (whatever has more
+// results than that is not cut), and the parts lie behind them.  So where the counters are does not depend on a launch's sizes, and one that has run
+// to its end leaves the workspace ready for any other.
+inline size_t join_counter_bytes() { return ((size_t)device_cus() * sizeof(int) + 255) / 256 * 256; }
+
 // the three instantiations of one kernel: general dispatcher loop, no counters, fixed claims
 template <class Kernel> struct KernelSet { Kernel any, plain, fixed; bool long_tiles = false; };  // (long_tiles: see plan_launch)
 template <class Kernel> static KernelSet<Kernel> kernel_set(Kernel a, Kernel p, Kernel f) { return {a, p, f, false}; }

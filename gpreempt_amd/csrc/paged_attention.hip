@@ -41,7 +41,7 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
         GP_REQUIRE(units * want < (1L << 31), "paged_attention: too large");
         pl->many = ManyArgs{a.p, a.group, (int)blocks, (int)want, nullptr, nullptr};
         if (want > 1) {
-            const size_t counters = ((size_t)units * sizeof(int) + 255) / 256 * 256;
+            const size_t counters = join_counter_bytes();  // (units: at most as many as compute units)
             pl->work_bytes = counters + (size_t)(units * want) * (p->cache.head_dim == 64 ? many_partial_floats<64>() : many_partial_floats<128>()) * sizeof(float);
             pl->many.arrived = (int *)p->work;
             pl->many.partial = (float *)((char *)p->work + counters);
@@ -62,9 +62,9 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
     GP_REQUIRE(most * p->batch < (1L << 31), "paged_attention: too large");
     pl->tiles_x = p->batch;
     pl->tiles_y = heads;
-    if (most > 4) {
-        pl->tiles_x = a.shares = (int)std::min(std::max(1l, device_cus() / heads), most * p->batch);
-        const size_t counters = ((size_t)units * sizeof(int) + 255) / 256 * 256;
+    if (most > 4) pl->tiles_x = a.shares = (int)std::min(std::max(1l, device_cus() / heads), most * p->batch);
+    if (a.shares > 1) {
+        const size_t counters = join_counter_bytes();  // (heads * shares: at most as many as compute units)
         pl->work_bytes = counters + (size_t)heads * a.shares * 2 * 16 * pl->nt * (p->cache.head_dim + 2) * sizeof(float);
         a.arrived = (int *)p->work;
         a.partial = (float *)((char *)p->work + counters);

@@ -29,7 +29,7 @@ struct FewArgs {
     int group;        // query heads to a head of the cache
     int row_blocks;   // of 16 * NT rows
     int shares;       // parts of the keys, per head and row block, at most; 0: every sequence is a part
-    int *arrived;     // workspace: a counter for every (head, row block, sequence), 0 between launches
+    int *arrived;     // workspace: a counter for every (head, row block, part), 0 between launches
     float *partial;   // ... and for every tile two results: 16 * NT rows of D values, then their maxima and sums
 };
 
@@ -350,7 +350,7 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
     __shared__ int came;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above have reached the memory that all XCDs see
     __syncthreads();
-    int *arrived = a.arrived + (long)hr * p.batch + b;
+    int *arrived = a.arrived + (long)hr * a.shares + first_share;  // (of the one sequence that goes on behind that part)
     if (tid == 0) came = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (came != parts - 1) return;

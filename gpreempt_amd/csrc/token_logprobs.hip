@@ -355,7 +355,7 @@ static int plan_token_logprobs(const gp_token_logprobs_params *p, LogprobsArgs *
     a->parts = (int)((tiles + a->tiles_per_part - 1) / a->tiles_per_part);
     *work_bytes = 0;
     if (a->parts > 1) {
-        const size_t counters = ((size_t)p->rows * sizeof(int) + 255) / 256 * 256;
+        const size_t counters = join_counter_bytes();  // (rows: at most half as many as compute units)
         *work_bytes = counters + (size_t)p->rows * a->parts * LP_PART_WORDS * sizeof(unsigned long long);
         a->arrived = (int *)p->work;
         a->partial = (unsigned long long *)((char *)p->work + counters);

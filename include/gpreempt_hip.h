@@ -608,8 +608,8 @@ int gp_launch_kv_append(const gp_kv_append_params *p, const gp_preempt_ctx *ctx,
  * What lies in the cache behind a sequence's length, or in slots that nobody has written, may be anything.  The values of a new token that is not
  * finite reach rows in front of it too (0 times infinity).  out must not overlap q or the cache.
  * work: gp_paged_attention_work_bytes() of device memory (0: none), zeroed before its first use (gp_fill32_async), and before the
- * next one when a stopped launch is not resumed; a launch that has run to its end leaves it ready for the next.  Launches that may
- * overlap need workspaces of their own. */
+ * next one when a stopped launch is not resumed; a launch that has run to its end leaves it ready for the next, of whatever sizes (and
+ * gp_token_logprobs_params::work likewise: one workspace of the largest size serves both).  Launches that may overlap need workspaces of their own. */
 typedef struct gp_paged_attention_params {
     int dtype;                /* of q and out: GP_F16 or GP_BF16 */
     gp_kv_cache cache;

@@ -628,6 +628,29 @@ def test_two_streams_at_once(gp):
         s.destroy()
 
 
+def test_one_workspace_for_launches_of_any_sizes(gp):
+    """as a program keeps it: of the largest size, zeroed once, for steps of few and of many sequences, short prompts and rows of logits, one after the other"""
+    calls = []
+    for lens, news, heads, kv_heads, dim in (([1500], None, 2, 2, 64), ([1500, 1100, 2000] * 20, None, 8, 4, 64), ([1700, 900], [1, 90], 16, 8, 128), ([2600] * 8, [70] * 8, 16, 2, 64),
+                                             ([900, 3500], [9, 8], 8, 4, 64), ([3500] * 5, None, 16, 16, 128)):
+        seqs = S.Sequences(lens, news, 64, gen(30))
+        calls.append(Attend(gp, "bf16", "bf16", seqs, heads, kv_heads, dim, True, 31 + len(calls)))
+    for rows, vocab in ((1, 300000), (100, 70000), (2, 66000)):
+        calls.append(Logprobs(gp, "bf16", torch.randn((rows, vocab), generator=gen(40 + rows)).bfloat16(), torch.arange(rows), 32))
+    assert all(c.p.work_bytes for c in calls)
+    room = max(c.p.work_bytes for c in calls)
+    shared = torch.zeros(room, dtype=torch.uint8, device="cuda")
+    for c in calls:
+        c.p.work, c.p.work_bytes = shared.data_ptr(), room
+    for order in (calls, calls[::-1], calls[::2] + calls[1::2]):
+        for c in order:
+            c.launch()
+        for c in order:
+            c.check()
+            for x in c.out.values() if isinstance(c, Logprobs) else [c.out]:
+                x.fill_(7)
+
+
 def test_captured_and_replayed(gp):
     """a step in a graph: replays with the program's own work in between, with other contents of the same buffers (lengths among them) every time"""
     stream = gp.Stream(0)
