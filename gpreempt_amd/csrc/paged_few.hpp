@@ -13,6 +13,10 @@
 //   O^T = V^T P^T  V^T as A, and P as B in the layout that S^T came out in: lane l has keys 4 * (l / 16) + 0..3 of two neighbouring tiles of
 //                  16.  So lane l loads these eight rows of V, D / 16 consecutive values from (D / 16) * (l % 16) on, and a few byte permutations turn
 //                  them into eight (four) A operands whose row l % 16 is the head's value (D / 16) * (l % 16) + j.
+//
+// Measured (32 heads, 8 cached of 128): 64 sequences of 2048 to 8192 keys, e4m3, 108 us for 625 MB, 5.8 TB/s (a kernel that only reads: 7.1; sequences of one
+// length: 6.2 to 6.7, since where a sequence ends its successor's loads begin anew); one of 131072 keys, 50 us for 268 MB, of which some 10 are the chain
+// length, pages, keys in front and the join of 32 parts behind; 24 sequences with 4 new tokens each, bf16, 57 us for 282 MB.
 #pragma once
 #include "kv_cache.hpp"
 #include "tile_loop.hpp"

@@ -2,8 +2,10 @@
 //
 // With m the largest logit so far, y = scale * (x - m), S = sum 2^(y log2 e) and W = sum y 2^(..): log p = y - log S, entropy = log S - W / S, and a
 // larger m' turns them into f S and f (W + d S), f = 2^(d log2 e), d = scale * (m - m').  Every thread keeps m, S and W of what it has seen.
-// Bound by memory for many rows: a workgroup takes a row, 16384 logits at a time, 32 to a thread, the next ones on their way while these are worked on.
+// Many rows: a workgroup takes a row, 16384 logits at a time, 32 to a thread, the next ones on their way while these are worked on.
 // A few long rows are cut into parts, joined by whoever comes last.
+// Measured: 500 rows of 131001 bf16 logits, 20 alternatives: 35 us, 3.8 TB/s (a kernel that only reads: 7.1), bound by vector instructions:
+// a wavefront takes some 62 cycles of them per 64 logits (16 of these the exponential) for the maximum, the two sums and their exponents.  One row of 30522: 7.5 us, of which a launch is 4.5.
 //
 // The alternatives: every group of eight threads leaves the largest logit of each tile in LDS.  Of the 64 lanes' largest logits, all wavefronts together, the
 // top-th largest is a bound that at least `top` logits reach; the few groups and tiles that reach it are looked at again, what reaches it goes to a list
