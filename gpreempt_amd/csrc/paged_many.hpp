@@ -11,7 +11,7 @@
 // Bound by the vector instructions of the softmax and the matrix instructions alike (32 of each lane's values cost about 900 cycles, the
 // products of 64 keys 1024), so two workgroups share a compute unit and fill each other's gaps.
 //
-// Measured: four sequences of 2900 to 5000 keys, 1358 to 4096 of them new, 32 heads, 8 cached of 128, e4m3: 605 to 615 us, 890 TFLOP/s (a large matrix product: 1200).  The matrix
+// Measured: four sequences of 2900 to 5000 keys, 1358 to 4096 of them new, 32 heads, 8 cached of 128, e4m3: 593 us, 915 TFLOP/s (a large matrix product: 1200).  The matrix
 // instructions are busy 36 % of the cycles and vector instructions 52 %, and they seldom overlap; LDS is in conflict for a quarter of the cycles it is active.
 #pragma once
 #include "paged_few.hpp"
@@ -87,11 +87,12 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         for (int v = 0; v < 16; ++v) o[i][v] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    // ---- pages: lane i has that of the i-th 16 keys of sixteen tiles ----
-    int page_l = -1;
+    // ---- pages: lane i has that of the i-th 16 keys of the sixteen tiles from `window` on; what a tile needs is read from there when it is needed (kept in
+    // scalar registers over three steps there were too many of them: 608 us for the sequences named above, 593 so) ----
+    int page_l = -1, window = first_tile;
     float ks_l = scale2, lv_l = 0.f, iv_l = 1.f;
-    auto look_up = [&](int tile) {
-        const int key = tile * MANY_KEYS + lane * 16;
+    auto look_up = [&]() {
+        const int key = window * MANY_KEYS + lane * 16;
         page_l = key < kend ? page_of(p.page_table, p.table_width, b, key / P, p.cache.pages) : -1;
         if constexpr (E8) {
             const long at = (long)(page_l < 0 ? 0 : page_l) * p.cache.kv_heads + kvh;
@@ -101,8 +102,6 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             iv_l = 1.f / vs;
         }
     };
-    // what of them a tile needs while it is worked on (in scalar registers)
-    struct Info { int pages[4], vbound; float ks[4], lv[4], iv[4]; };
     auto scalar = [](float v, int at) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), at)); };
     // ---- from the pages to registers: thread (tid % 16, tid / 16).  Keys: 16 keys at a time, a row's 16 (8) chunks side by side.  Values: four keys of the
     // wavefront's 16, eight (four) values ----
@@ -115,16 +114,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
     VRow vr[4];
     auto block_at = [&](int page, int key) { return (((long)(page < 0 ? 0 : page) * p.cache.kv_heads + kvh) * P + (key & (P - 1))) * D * ES; };
     auto fetch = [&](int tile) {
-        const int sub = (tile - first_tile) % 16 * 4;
-        if (sub == 0) look_up(tile);
-        Info info;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            info.pages[i] = __builtin_amdgcn_readlane(page_l, sub + i);
-            info.ks[i] = E8 ? scalar(ks_l, sub + i) : scale2;
-            info.lv[i] = E8 ? scalar(lv_l, sub + i) : 0.f;
-            info.iv[i] = E8 ? scalar(iv_l, sub + i) : 1.f;
-        }
+        const int sub = (tile - window) * 4;
 #pragma unroll
         for (int i = 0; i < KLOADS; ++i) {
             const int row = i * KROWS + tid / (D * ES / 16), chunk = tid % (D * ES / 16);
@@ -135,8 +125,6 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         const char *at = (const char *)p.cache.v + block_at(page, key0) + lane % 16 * (VV * ES);
 #pragma unroll
         for (int e = 0; e < 4; ++e) vr[e] = *(const VRow *)(at + e * D * ES);
-        info.vbound = page >= 0 ? bound : 0;
-        return info;
     };
     // ---- ... and on to LDS ----
     auto kslot = [&](int row, int chunk) { return row * (D * 2) + (chunk ^ (row & (KCH - 1))) * 16; };
@@ -147,7 +135,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
     for (int k = 0; k < KSTEPS; ++k) kat[k] = kslot(l32, 2 * k + half);
 #pragma unroll
     for (int u = 0; u < 4; ++u) { vat[0][u] = vslot(l32, 2 * u + half); vat[1][u] = vslot(32 + l32, 2 * u + half); }
-    auto stage = [&](char *buf, int tile, const Info &info) {
+    auto stage = [&](char *buf, int tile) {
 #pragma unroll
         for (int i = 0; i < KLOADS; ++i) {
             const int row = i * KROWS + tid / (D * ES / 16), chunk = tid % (D * ES / 16);
@@ -159,9 +147,10 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
                 *(u32x4 *)(buf + kslot(row, chunk)) = kr[i];
             }
         }
+        const int vbound = __builtin_amdgcn_readlane(page_l, (tile - window) * 4 + wave) >= 0 ? bound : 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (tile * MANY_KEYS + wave * 16 + lane / 16 * 4 + e >= info.vbound) vr[e] = VRow(0);
+            if (tile * MANY_KEYS + wave * 16 + lane / 16 * 4 + e >= vbound) vr[e] = VRow(0);
         // keys 4 g .. 4 g + 3 of the wavefront's 16: half g % 2, and there the first four or the second
         const int g = lane / 16, chunk = 2 * wave + g % 2, d0 = lane % 16 * VV;
 #pragma unroll
@@ -184,12 +173,12 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
     };
 
     // A tile's way: fetched two steps ahead, put into LDS one step ahead, between the matrix instructions of the scores
-    Info now = {}, next = {};
     __syncthreads();  // (the previous tile's buffers are still being read)
     if (tiles > first_tile) {
-        now = fetch(first_tile);
-        stage(lds, first_tile, now);
-        if (first_tile + 1 < tiles) next = fetch(first_tile + 1);
+        look_up();
+        fetch(first_tile);
+        stage(lds, first_tile);
+        if (first_tile + 1 < tiles) fetch(first_tile + 1);
     }
     __syncthreads();
     // one tile of keys, in buffer BUF
@@ -197,7 +186,17 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         constexpr int BUF = decltype(buffer)::value;
         const char *buf = lds + BUF * 2 * TILE_BYTES;
         const int key0 = tile * MANY_KEYS;
-        const bool whole = key0 + MANY_KEYS <= kmin && (now.pages[0] | now.pages[1] | now.pages[2] | now.pages[3]) >= 0;
+        if (tile + 2 - window >= 16) { window = tile; look_up(); }  // (this tile, the one that is staged and the one that is fetched)
+        const int sub = (tile - window) * 4;
+        int pages[4];
+        float ks[4], lv[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            pages[u] = __builtin_amdgcn_readlane(page_l, sub + u);
+            ks[u] = E8 ? scalar(ks_l, sub + u) : scale2;
+            lv[u] = E8 ? scalar(lv_l, sub + u) : 0.f;
+        }
+        const bool whole = key0 + MANY_KEYS <= kmin && (pages[0] | pages[1] | pages[2] | pages[3]) >= 0;
         // ---- scores ----
         f32x16 x[2];
 #pragma unroll
@@ -207,7 +206,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
 #pragma unroll
             for (int k = 0; k < KSTEPS; ++k) Elem<T>::mma(*(const u32x4 *)(buf + kat[k] + i * 32 * D * 2), q[k], x[i]);
         }
-        stage(lds + (1 - BUF) * 2 * TILE_BYTES, tile + 1, next);  // (behind the last tile: the last one again, which nobody reads)
+        stage(lds + (1 - BUF) * 2 * TILE_BYTES, tile + 1);  // (behind the last tile: the last one again, which nobody reads)
         // (the order that the compiler is asked for: operands four ahead, a few of the other instructions behind every matrix instruction; four prompts of 2600 to 4096 tokens,
         // 32 heads of 128, bf16: 708 us without, 681 with)
         __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // reads of LDS
@@ -217,14 +216,13 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);  // vector instructions
         }
-        Info later = {};
-        if (tile + 2 < tiles) later = fetch(tile + 2);
+        if (tile + 2 < tiles) fetch(tile + 2);
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int v = 0; v < 16; ++v)
-                    if (now.pages[2 * i + v / 8] < 0 || key0 + i * 32 + 8 * (v / 4) + 4 * half + v % 4 >= seen) x[i][v] = -INFINITY;
+                    if (pages[2 * i + v / 8] < 0 || key0 + i * 32 + 8 * (v / 4) + 4 * half + v % 4 >= seen) x[i][v] = -INFINITY;
         }
         // ---- running maximum (raised only when it is exceeded 256-fold, which the types and the sums have room for) and sum.  8 bits: the logarithm of the
         // values' scale is part of the exponent, so that what is rounded to 16 bits is the probability times that scale; the sum takes it back out ----
@@ -234,7 +232,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             float most = x[u / 2][8 * (u % 2)];
 #pragma unroll
             for (int v = 1; v < 8; ++v) most = fmaxf(most, x[u / 2][8 * (u % 2) + v]);
-            top = fmaxf(top, fmaf(most, now.ks[u], now.lv[u]));
+            top = fmaxf(top, fmaf(most, ks[u], lv[u]));
         }
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         if (__any(top > m + 8.f)) {
@@ -249,24 +247,22 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const float off = now.lv[u] - base;
+            const float off = lv[u] - base;
             float part = 0.f;
             typedef T tx8 __attribute__((ext_vector_type(8)));
             tx8 pb;
 #pragma unroll
             for (int v = 0; v < 8; ++v) {
-                const float y = __builtin_amdgcn_exp2f(fmaf(x[u / 2][8 * (u % 2) + v], now.ks[u], off));
+                const float y = __builtin_amdgcn_exp2f(fmaf(x[u / 2][8 * (u % 2) + v], ks[u], off));
                 part += y;
                 pb[v] = Elem<T>::from_f(y);
             }
-            l = E8 ? fmaf(part, now.iv[u], l) : l + part;
+            l = E8 ? fmaf(part, scalar(iv_l, sub + u), l) : l + part;
             // ---- O^T += V^T P^T, 16 keys ----
 #pragma unroll
             for (int i = 0; i < DB; ++i) Elem<T>::mma(*(const u32x4 *)(buf + vat[i % 2][u] + i / 2 * 64 * MANY_KEYS * 2), __builtin_bit_cast(u32x4, pb), o[i]);
         }
         __syncthreads();
-        now = next;
-        next = later;
     };
     for (int tile = first_tile; tile < tiles; tile += 2) {
         step(tile, IntC<0>());
