@@ -11,8 +11,8 @@
 // Bound by the vector instructions of the softmax and the matrix instructions alike (32 of each lane's values cost about 900 cycles, the
 // products of 64 keys 1024), so two workgroups share a compute unit and fill each other's gaps.
 //
-// Measured: four sequences of 2900 to 5000 keys, 1358 to 4096 of them new, 32 heads, 8 cached of 128, e4m3: 593 us, 915 TFLOP/s (a large matrix product: 1200).  The matrix
-// instructions are busy 36 % of the cycles and vector instructions 52 %, and they seldom overlap; LDS is in conflict for a quarter of the cycles it is active.
+// Measured: four sequences of 2900 to 5000 keys, 1358 to 4096 of them new, 32 heads, 8 cached of 128, e4m3: 587 to 593 us, 920 TFLOP/s (a large matrix product: 1200).  The matrix
+// instructions are busy 41 % of the cycles and vector instructions 58 %, and they seldom overlap; LDS is in conflict for a quarter of the cycles it is active.
 #pragma once
 #include "paged_few.hpp"
 
