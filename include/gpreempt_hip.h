@@ -582,7 +582,7 @@ typedef struct gp_kv_cache {
  * the first page that a sequence's new tokens touch, what its other slots hold is rounded anew (nothing counts in a page whose
  * slot 0 is written: zeros); the other slots of further pages are left as they were.  Values beyond 448 scales (infinities)
  * become the largest, NaN stays NaN.
- * No two positions of a call may share a page and a slot, nor, in GP_E4M3, two sequences a page that both write to.
+ * No two positions of a call may share a page and a slot, nor, in GP_E4M3, may two entries of the table that are written to name one page.
  * q may be NULL (no queries); q_out may be q. */
 enum gp_rot_pairs { GP_ROT_HALVES = 0 /* (j, j + rot_dim / 2) */, GP_ROT_NEIGHBOURS = 1 /* (2 j, 2 j + 1) */ };
 typedef struct gp_kv_append_params {
@@ -609,7 +609,8 @@ int gp_launch_kv_append(const gp_kv_append_params *p, const gp_preempt_ctx *ctx,
  * finite reach rows in front of it too (0 times infinity).  out must not overlap q or the cache.
  * work: gp_paged_attention_work_bytes() of device memory (0: none), zeroed before its first use (gp_fill32_async), and before the
  * next one when a stopped launch is not resumed; a launch that has run to its end leaves it ready for the next, of whatever sizes (and
- * gp_token_logprobs_params::work likewise: one workspace of the largest size serves both).  Launches that may overlap need workspaces of their own. */
+ * gp_token_logprobs_params::work likewise: one workspace of the largest size serves both).  Launches that may overlap need workspaces of their own, a stopped
+ * one and what runs before it is resumed among them. */
 typedef struct gp_paged_attention_params {
     int dtype;                /* of q and out: GP_F16 or GP_BF16 */
     gp_kv_cache cache;

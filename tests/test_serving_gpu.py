@@ -651,6 +651,54 @@ def test_one_workspace_for_launches_of_any_sizes(gp):
                 x.fill_(7)
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("news", [None, [70, 40]])
+def test_pages_and_rows_behind_four_gigabytes(gp, news, cache):
+    """the last pages of a large pool, and rows far apart: the bits of the same call in a small one"""
+    seqs = S.Sequences([700, 1300], news, 64, gen(80))
+    app, att = Append(gp, "bf16", cache, seqs, 8, 4, 128, 128, "halves", 81), Attend(gp, "bf16", cache, seqs, 8, 4, 128, True, 82)
+    att.p.cache = app.p.cache  # (one cache for both)
+    att.p.q, att.p.ld_q = app.q_out.data_ptr(), app.q_out.shape[1]
+    app.launch()
+    att.launch()
+    small = app.left(), att.left()
+    clean(app)
+    clean(att)
+    block = 4 * 64 * 128 * app.dev["k"].element_size()
+    pages = (5 << 30) // block
+    big = {n: torch.empty((pages,) + tuple(app.dev[n].shape[1:]), dtype=app.dev[n].dtype, device="cuda") for n in app.cache}
+    for n, x in app.cache.items():
+        big[n][-seqs.pages:].copy_(x)
+        setattr(app.p.cache, n, big[n].data_ptr())
+    app.p.cache.pages = pages
+    table = app.dev["table"] + (pages - seqs.pages)
+    app.p.page_table = att.p.page_table = table.data_ptr()
+    att.p.cache = app.p.cache
+    ld = (1 << 32) // (seqs.tokens - 1) // 8 * 8 + 8  # the last row begins behind 2^32 values
+    far_q, far_out = (torch.empty(ld * (seqs.tokens - 1) + 8 * 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    app.p.q_out, app.p.ld_q_out, att.p.q, att.p.ld_q, att.p.out, att.p.ld_out = far_q.data_ptr(), ld, far_q.data_ptr(), ld, far_out.data_ptr(), ld
+    app.launch()
+    att.launch()
+    torch.cuda.synchronize()
+    for n in app.cache:
+        assert torch.equal(big[n][-seqs.pages:].cpu().view(torch.uint8), small[0][n].view(torch.uint8)), n
+    for row in range(seqs.tokens):
+        assert torch.equal(far_q[row * ld:row * ld + 1024].cpu(), small[0]["q"][row, :1024])
+        assert torch.equal(far_out[row * ld:row * ld + 1024].cpu(), small[1][row, :1024])
+
+
+def test_logits_behind_four_gigabytes(gp):
+    x = (3 * torch.randn((5, 20000), generator=gen(83))).bfloat16()
+    a = Logprobs(gp, "bf16", x, torch.arange(5), 10)
+    ld = (1 << 30) + 1  # the last row begins behind 2^32 values
+    far = torch.empty(4 * ld + 20000, dtype=torch.bfloat16, device="cuda")
+    for row in range(5):
+        far[row * ld:row * ld + 20000].copy_(x[row])
+    a.p.logits, a.p.ld = far.data_ptr(), ld
+    a.launch()
+    a.check()
+
+
 def test_captured_and_replayed(gp):
     """a step in a graph: replays with the program's own work in between, with other contents of the same buffers (lengths among them) every time"""
     stream = gp.Stream(0)
