@@ -82,9 +82,6 @@ __device__ __forceinline__ FewSequence few_sequence(const FewArgs &a, const SeqT
     return f;
 }
 
-// the part of `units` units, in `shares` parts, that unit x is in
-__device__ __forceinline__ int share_of(long x, long units, long shares) { return (int)(((x + 1) * shares - 1) / units); }
-
 // Keys [c0, kend) of one sequence; then its rows are finished, or its part of them waits in slot `slot` for the others.
 // first_share, last_share: the parts that the sequence's keys are spread over.
 template <typename T, int D, bool E8, int NT>
@@ -443,9 +440,9 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
     constexpr int LEAST = NT == 1 ? 2 : 4;
     const int shares = total / LEAST < 1 ? 1 : total / LEAST < a.shares ? total / LEAST : a.shares;
     if (total == 0 || t.x >= shares) return;  // (no sequence has rows in this block)
-    const int lo = (int)((long)t.x * total / shares), hi = (int)((t.x + 1l) * total / shares);
-    int at = 0, b0 = 0, b = 0;  // units in front of sequence b, which is one of the 64 from b0 on
-    for (;; b0 += 64) {
+    const int lo = part_begin(t.x, total, shares), hi = part_begin(t.x + 1, total, shares);
+    float *slots = a.partial + ((long)hr * a.shares + t.x) * 2 * few_partial_floats<NT, D>();
+    walk_part(batch, 64, lo, hi, [&](int b0, int unit, int &at, int &i) {
         if (b0) n = look(b0);
         int upto = n;
 #pragma unroll
@@ -453,25 +450,18 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
             const int x = __shfl_up(upto, d, 64);
             if (lane >= d) upto += x;
         }
-        const unsigned long long behind = __ballot(at + upto > lo);
-        if (behind) {
-            b = b0 + __builtin_ctzll(behind);
-            at += __builtin_amdgcn_readlane(upto - n, b - b0);
-            break;
-        }
-        at += __builtin_amdgcn_readlane(upto, 63);
-    }
-    float *slots = a.partial + ((long)hr * a.shares + t.x) * 2 * few_partial_floats<NT, D>();
-    for (; at < hi; ++b) {
-        if (b - b0 == 64) look(b0 += 64);
-        const int i = b - b0;
+        const unsigned long long behind = __ballot(at + upto > unit);
+        if (behind) i = __builtin_ctzll(behind);
+        at += behind ? __builtin_amdgcn_readlane(upto - n, i) : __builtin_amdgcn_readlane(upto, 63);
+        return behind != 0;
+    }, look, [&](int b, int i, int at) {
         const FewSequence f = few_sequence<ROWS, UNIT>(a, seq_tokens_of(__builtin_amdgcn_readlane(r0, i), __builtin_amdgcn_readlane(r1, i), __builtin_amdgcn_readlane(len, i), p.tokens, p.max_new), rb);
-        if (f.units == 0) continue;
+        if (f.units == 0) return 0;
         const int u0 = lo > at ? lo - at : 0, u1 = hi - at < f.units ? hi - at : f.units;
         attend_stretch<T, D, E8, NT>(a, f, b, hr, u0 * UNIT, u1 == f.units ? f.kend : u1 * UNIT, slots + (u0 == 0) * few_partial_floats<NT, D>(),
-                                     share_of(at, total, shares), share_of(at + f.units - 1l, total, shares), lds);
-        at += f.units;
-    }
+                                     part_of(at, total, shares), part_of(at + f.units - 1l, total, shares), lds);
+        return f.units;
+    });
 }
 
 template <typename T, int D, bool E8, int NT, int LOOP = LOOP_ANY>

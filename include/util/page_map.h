@@ -69,4 +69,30 @@ GP_HD PageSpan page_span(const SeqTokens &s, int j, int page_size) {
     return p;
 }
 
+// All sequences' keys in equal parts: sequence b has some number of units, one sequence behind the other, `total` of them in all, and part x of `shares` (at most
+// as many as units) has the units [part_begin(x), part_begin(x + 1)).
+GP_HD int part_begin(long x, long total, long shares) { return (int)(x * total / shares); }
+// the part that unit x is in
+GP_HD int part_of(long x, long total, long shares) {
+    const long part = ((x + 1) * shares - 1) / total;
+    return (int)(part < shares ? part : shares - 1);
+}
+
+// The sequences that a part [lo, hi) has units of, in their order.  `lanes` of them are looked at together, and looked at anew whenever they are needed, so the lengths that
+// this walk meets need not be those that `total` was added up from if somebody writes to them meanwhile: it ends with the last sequence, whatever they are.
+//   find(b0, lo, at, i)  looks at the sequences from b0 on, in front of which there are `at` units: whether unit lo is among theirs; then i is which of them has it and `at` the
+//                        units in front of that one, else `at` goes behind them all
+//   look(b0)             looks at the sequences from b0 on
+//   visit(b, i, at)      sequence b, the i-th of those looked at last, in front of which there are `at` units: its units
+template <class Find, class Look, class Visit>
+GP_HD void walk_part(int batch, int lanes, int lo, int hi, Find &&find, Look &&look, Visit &&visit) {
+    int at = 0, i = 0, b0 = 0;
+    while (!find(b0, lo, at, i))
+        if ((b0 += lanes) >= batch) return;
+    for (int b = b0 + i; at < hi && b < batch; ++b) {
+        if (b - b0 == lanes) look(b0 += lanes);
+        at += visit(b, b - b0, at);
+    }
+}
+
 }  // namespace gp
