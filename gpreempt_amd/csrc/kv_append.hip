@@ -98,11 +98,11 @@ __device__ __forceinline__ void store_runs(T *row, const Share &s, const float (
     }
 }
 
-// the smallest power of two that a magnitude is at most 448 = 1.75 * 2^8 times, from its exponent and mantissa
+// the smallest power of two that a magnitude is at most 448 = 1.75 * 2^8 times, from its exponent and mantissa, as far as pages' scales go
 __device__ __forceinline__ float scale_for(float most) {
     const unsigned bits = __builtin_bit_cast(unsigned, most);
     const int k = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u);
-    return k < -40 ? LOWEST_SCALE : __builtin_bit_cast(float, (unsigned)(k + 127) << 23);
+    return k < -40 ? LOWEST_SCALE : fminf(__builtin_bit_cast(float, (unsigned)(k + 127) << 23), MOST_SCALE);
 }
 
 // The new values of one page and head in 8 bits: the scale that they need, what the page holds on a new one, and the values.
@@ -129,14 +129,14 @@ __device__ __forceinline__ void append_e4m3(const AppendArgs &a, const PageSpan 
     __syncthreads();
     most = fmaxf(fmaxf(lds_most[0], lds_most[1]), fmaxf(lds_most[2], lds_most[3]));
     float *scale_at = (values ? p.cache.v_scale : p.cache.k_scale) + (long)page * p.cache.kv_heads + head;
-    float before = span.lo ? *scale_at : 0.f;
-    if (!(before > 0.f && before < INFINITY)) before = 0.f;  // (a scale that nobody has set)
+    const float stored = span.lo ? *scale_at : 0.f;
+    const float before = stored > 0.f && stored < INFINITY ? within_scales(stored) : 0.f;  // (0: a scale that nobody has set)
     const float scale = most > 448.f * before || before == 0.f ? scale_for(most) : before;
     const float inv = 1.f / scale;
     unsigned char *dst = (unsigned char *)(values ? p.cache.v : p.cache.k) + block;
     __syncthreads();  // everybody has read the scale
+    if (threadIdx.x == 0 && scale != stored) *scale_at = scale;
     if (scale != before) {
-        if (threadIdx.x == 0) *scale_at = scale;
         // what else the page holds, on the new scale (in the first page that the sequence writes to: the others begin here)
         if (j == 0) {
             const float ratio = before * inv;

@@ -24,6 +24,11 @@ __device__ __forceinline__ float rounded(float x) {
     return x;
 }
 
+// A page's scale as everybody takes it, between the borders that the header names: their ratio, and its inverse, are in fp32's normal range, so no
+// probability times a scale is lost next to another's.  (NaN becomes the lower one)
+constexpr float LEAST_SCALE = 0x1p-60f, MOST_SCALE = 0x1p60f;
+__device__ __forceinline__ float within_scales(float s) { return fminf(fmaxf(s, LEAST_SCALE), MOST_SCALE); }
+
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 
 // eight e4m3 values of 8 bytes

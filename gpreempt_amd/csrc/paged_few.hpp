@@ -52,8 +52,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 template <bool HI> __device__ __forceinline__ unsigned widen(unsigned raw, _Float16) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw, 1.f, HI)); }
 template <bool HI> __device__ __forceinline__ unsigned widen(unsigned raw, __bf16) { return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw, 1.f, HI)); }
 
-// the scale of a page's head, within the bounds that the header names
-__device__ __forceinline__ float page_scale(const float *scales, long at) { return fminf(fmaxf(scales[at], 0x1p-60f), 0x1p60f); }
+// the scale of a page's head
+__device__ __forceinline__ float page_scale(const float *scales, long at) { return within_scales(scales[at]); }
 
 // stores and loads of what another workgroup reads or has written within the launch
 __device__ __forceinline__ void put_shared(float *p, f32x2 v) { __hip_atomic_store((unsigned long long *)p, __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }

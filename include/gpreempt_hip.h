@@ -552,7 +552,8 @@ int gp_launch_embed(const gp_embed_params *p, const gp_preempt_ctx *ctx, gp_stre
  * The cache: a pool of `pages` pages, each with room for page_size tokens of every head of the cache,
  *   k, v[page][kv head][slot][head_dim]
  * in the activations' type or, with k_scale and v_scale[page][kv head], in GP_E4M3: a value is its 8 bits times the scale of
- * its page and head.  Scales are positive; attention takes one outside 2^-60 .. 2^60 as the nearer border.
+ * its page and head.  Scales are positive; one outside 2^-60 .. 2^60 is taken as the nearer border (an append leaves the border in
+ * its place).
  * page_size 16, 32, 64 or 128; head_dim 64 or 128; k and v 16-byte aligned. */
 typedef struct gp_kv_cache {
     int dtype;                /* GP_F16, GP_BF16 or GP_E4M3 */
@@ -579,7 +580,7 @@ typedef struct gp_kv_cache {
  * queries to q_out.  Element j of the rot_dim / 2 pairs of a head's first rot_dim values (a, b) becomes (a cos - b sin,
  * b cos + a sin), the angle being position * inv_freq[j], multiplied in 64 bits.  rot_dim 0: no rotation; a multiple of 16 otherwise.
  * Row t of k (v, q) for head h is k + t * ld_qkv + h * head_dim (16-byte aligned rows).  Values are rounded once, to the cache's type.
- * GP_E4M3: a page's scale is set by the call that writes its slot 0, to the smallest power of two (2^-40 at least) that brings the
+ * GP_E4M3: a page's scale is set by the call that writes its slot 0, to the smallest power of two (2^-40 at least, 2^60 at most) that brings the
  * largest finite magnitude of its tokens to 448 or less; a later call raises it when larger values come.  Where that changes the scale of
  * the first page that a sequence's new tokens touch, what its other slots hold is rounded anew (nothing counts in a page whose
  * slot 0 is written: zeros); the other slots of further pages are left as they were.  Values beyond 448 scales (infinities)
