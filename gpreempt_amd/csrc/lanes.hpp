@@ -4,7 +4,8 @@
 
 namespace gp {
 
-// the largest of three; NaN loses.  (fmaxf makes a signalling NaN a quiet one first, an instruction more for each operand)
+// The largest of three; a quiet NaN loses, a signalling one becomes a quiet one, in whose place the largest of the others is forgotten.  (fmaxf makes it a quiet one
+// first, an instruction more for each operand)
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));

@@ -262,11 +262,13 @@ __device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, 
             p.top_logprobs[r * top + rank] = key ? (key_value(key) - M) * p.scale - log_sum : -INFINITY;
         });
     };
-    // more candidates than the list holds (equal logits, say): one after the other, each the largest behind the last one
-    if (top && count > LP_LIST) {
+    // more candidates than the list holds (equal logits, say): one after the other, each the largest behind the last one.  And so where there is a NaN (the sum is one then):
+    // a signalling one makes the instruction above forget the largest so far, which the groups' largest then do not name.  (Making it a quiet one first
+    // is an instruction more for every logit of every row)
+    if (top && (count > LP_LIST || s != s)) {
         const int from = first * LP_TILE, to = last * LP_TILE < vocab ? last * LP_TILE : vocab;
         unsigned long long before = ~0ull;
-        for (int k = 0; k < top; ++k) {
+        for (count = 0; count < top; ++count) {
             unsigned long long best = 0;
             for (int i = from + tid; i < to; i += LP_NT) {
                 const unsigned long long key = rank_key(Elem<T>::to_f(row[i]), i);
@@ -282,11 +284,11 @@ __device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, 
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < LP_WAVES; ++i) best = l.list[1][i] > best ? l.list[1][i] : best;
-            if (tid == 0) l.list[0][k] = best;
+            if (best == 0) break;  // (no more alternatives)
+            if (tid == 0) l.list[0][count] = best;
             before = best;
         }
         __syncthreads();
-        count = top;
     }
     if (a.parts == 1) { finish(M, s, w, 0, count); return; }
 

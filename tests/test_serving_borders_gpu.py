@@ -39,3 +39,25 @@ def test_append_to_a_page_whose_scale_attention_takes_as_a_border(gp, dt):
             for slot in range(n - 1):
                 step = torch.maximum(2.0 ** -4 * old[:, slot].abs(), 2.0 ** -10 * scale)
                 assert ((got[:, slot] - old[:, slot]).abs() <= step).all(), (name, b, slot)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [40, 9001, 70000])
+def test_alternatives_next_to_a_nan_of_either_kind(gp, dt, vocab):
+    """a signalling or a quiet NaN right behind the row's largest logit, whose neighbours are all small: the alternatives are the others, in order"""
+    ints, bad = {"f32": (torch.int32, (0x7F800001, 0x7FC00000)), "f16": (torch.int16, (0x7C01, 0x7E00)), "bf16": (torch.int16, (0x7F81, 0x7FC0))}[dt]
+    rng = T.gen(3)
+    x = torch.randn((4, vocab), generator=rng)
+    vec = 4 if dt == "f32" else 8
+    for at in range(0, vocab, 512 * vec):  # what eight threads next to each other read
+        x[:, at: at + 8 * vec] = -50.0 - torch.arange(vocab)[at: at + 8 * vec] / 4096
+    x = x.to(S.TORCH[dt])
+    x[:, 0] = 9.0
+    for r in range(4):
+        x.view(ints)[r, 2 + r // 2] = bad[r % 2]
+    a = T.Logprobs(gp, dt, x, torch.tensor([0, 1, 2, 3]), 20)
+    assert torch.equal(a.room.cpu().view(ints), x.view(ints).flatten())  # (no copy has made them quiet)
+    a.launch()
+    got = a.left()
+    assert torch.equal(got["ids"], S.logprobs(x, torch.zeros(4), 1.0, 20)[2])
+    assert got["logprob"].isnan().all() and got["entropy"].isnan().all() and got["values"].isnan().all()
