@@ -2,7 +2,7 @@
 //
 // Bound by memory: 2 * D values of the cache per key.  So keys and values go from memory to the registers that the matrix instructions
 // read, without LDS and without a barrier; the four wavefronts of a workgroup take turns over a stretch of keys, each with a running
-// maximum and sum of its own, and meet at its end.
+// reference (the largest score, or a little below it) and sum of its own, and meet at its end.
 //
 // A tile is one head of the cache, up to 16 * NT query rows of a sequence that share it (its new tokens times the query heads of the
 // head), and one of `shares` equal parts of the keys of all sequences, one sequence behind the other: how long they are only the device knows,
@@ -18,6 +18,7 @@
 // length: 6.2 to 6.7, since where a sequence ends its successor's loads begin anew); one of 131072 keys, 50 us for 268 MB, of which some 10 are the chain
 // length, pages, keys in front and the join of 32 parts behind; 24 sequences with 4 new tokens each, bf16, 57 us for 282 MB.
 #pragma once
+#include <type_traits>
 #include "kv_cache.hpp"
 #include "tile_loop.hpp"
 
@@ -54,6 +55,18 @@ template <bool HI> __device__ __forceinline__ unsigned widen(unsigned raw, __bf1
 
 // the scale of a page's head
 __device__ __forceinline__ float page_scale(const float *scales, long at) { return within_scales(scales[at]); }
+
+// Exponents are taken against a reference m that a row's largest one, `top`, exceeds by at most `room`.  What is rounded to 16 bits for the second product is 2^(x - m).  fp16's
+// numbers become fixed-point ones below 2^-14, so there m is put below the largest and may be exceeded by what fp16 has room for: beside its half unit, a probability
+// is off by at most 2^-36 of the row's largest (against the largest itself by 2^-25: 131072 keys of half that each were lost, 0.2 % of their row, while the sum in the denominator
+// had them).  bf16 has fp32's range.  Measured over many rows of 128, fp16: level with m at the largest, raised when it is exceeded 2^8-fold; put 14 below it, it is raised
+// oftener: 592 -> 604 us.
+template <typename T> struct Reference {
+    static constexpr bool FP16 = std::is_same<T, _Float16>::value;
+    static constexpr float room(float wanted) { return FP16 ? 15.f : wanted; }
+    // (beyond 2^20, where the difference would be rounded to other steps, the largest itself)
+    static __device__ __forceinline__ float below(float top) { return FP16 && fabsf(top) < 0x1p20f ? top - 11.f : top; }
+};
 
 // stores and loads of what another workgroup reads or has written within the launch
 __device__ __forceinline__ void put_shared(float *p, f32x2 v) { __hip_atomic_store((unsigned long long *)p, __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -93,6 +106,7 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
     constexpr int KS = few_step_keys<E8>(), TILES = KS / 16, PAIRS = KS / 32;  // keys of a wavefront's step
     constexpr int ROWS = 16 * NT, VD = D / 16, KL = E8 ? D / 64 : D / 32;
     constexpr int ES = E8 ? 1 : 2;  // bytes of a value
+    constexpr float ROOM = Reference<T>::room(0.f);
     typedef unsigned int VRow __attribute__((ext_vector_type(VD * ES / 4)));  // a lane's values of one key
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
     const int rb = hr % a.row_blocks, kvh = hr / a.row_blocks, P = p.cache.page_size;
@@ -228,8 +242,8 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
                     }
                 }
             }
-            // ---- running maximum and sum.  8 bits: x has the logarithm of the values' scale added, so that what is rounded to 16
-            // bits is the probability times that scale, at most 1; the sum takes the scale back out ----
+            // ---- running reference and sum.  8 bits: x has the logarithm of the values' scale added, so that what is rounded to 16
+            // bits is the probability times that scale, at most 2^ROOM; the sum takes the scale back out ----
             u32x4 pb[NT][PAIRS];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -240,8 +254,8 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
                     for (int e = 0; e < 4; ++e) top = fmaxf(top, x[n][i][e]);
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
-                if (__any(top > m[n])) {
-                    const float now = fmaxf(m[n], top), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[n] - now);
+                if (__any(top > m[n] + ROOM)) {
+                    const float now = fmaxf(m[n], Reference<T>::below(top)), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[n] - now);
                     m[n] = now;
                     l[n] *= f;
 #pragma unroll
@@ -295,7 +309,7 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
         }
     }
 
-    // ---- the four wavefronts' results meet: O = sum_w a_w O_w, a_w = 2^(m_w - max m) ----
+    // ---- the four wavefronts' results meet: O = sum_w a_w O_w, a_w = 2^(m_w - max m), m_w its reference ----
     constexpr int LD = D + 4;
     float *ml = lds + FEW_WAVES * ROWS * LD;
     __syncthreads();  // (the previous tile's are still being read)

@@ -43,6 +43,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
 #pragma clang fp contract(off)  // (as in attend_stretch)
     const gp_paged_attention_params &p = a.p;
     constexpr int ES = E8 ? 1 : 2, DB = D / 32, KSTEPS = D / 16;
+    constexpr float ROOM = Reference<T>::room(8.f);
     constexpr int KCH = D / 8;                              // 16-byte chunks of a key's row in LDS
     constexpr int TILE_BYTES = MANY_KEYS * D * 2;           // of keys; values behind them
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5, P = p.cache.page_size;
@@ -224,7 +225,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
                 for (int v = 0; v < 16; ++v)
                     if (pages[2 * i + v / 8] < 0 || key0 + i * 32 + 8 * (v / 4) + 4 * half + v % 4 >= seen) x[i][v] = -INFINITY;
         }
-        // ---- running maximum (raised only when it is exceeded 256-fold, which the types and the sums have room for) and sum.  8 bits: the logarithm of the
+        // ---- running reference (raised only when it is exceeded 2^ROOM-fold, which the types and the sums have room for) and sum.  8 bits: the logarithm of the
         // values' scale is part of the exponent, so that what is rounded to 16 bits is the probability times that scale; the sum takes it back out ----
         float top = -INFINITY;
 #pragma unroll
@@ -235,8 +236,8 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             top = fmaxf(top, fmaf(most, ks[u], lv[u]));
         }
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        if (__any(top > m + 8.f)) {
-            const float high = fmaxf(m, top), f = high == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - high);
+        if (__any(top > m + ROOM)) {
+            const float high = fmaxf(m, Reference<T>::below(top)), f = high == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - high);
             m = high;
             l *= f;
 #pragma unroll

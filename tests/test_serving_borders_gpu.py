@@ -61,3 +61,27 @@ def test_alternatives_next_to_a_nan_of_either_kind(gp, dt, vocab):
     got = a.left()
     assert torch.equal(got["ids"], S.logprobs(x, torch.zeros(4), 1.0, 20)[2])
     assert got["logprob"].isnan().all() and got["entropy"].isnan().all() and got["values"].isnan().all()
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dt", T.DTS)
+@pytest.mark.parametrize("lens, news, heads, kv_heads, dim", [([3000, 700], None, 8, 2, 128), ([2000, 1500, 1000, 300], [70, 66, 67, 80], 16, 16, 64)])
+def test_attention_to_many_unlikely_keys(gp, dt, cache, lens, news, heads, kv_heads, dim):
+    """One key takes nearly everything and its values are zero: the result is what the others, each 2^26 times less likely, add up to."""
+    seqs = S.Sequences(lens, news, 64, T.gen(4))
+    a = T.Attend(gp, dt, dt if cache == "same" else cache, seqs, heads, kv_heads, dim, False, 5, scale=1.0)
+    a.q[:] = 0.0
+    a.q[:, ::dim] = 18.0  # e^18 = 2^26
+    if cache == "e4m3":
+        for n in ("k_scale", "v_scale"):
+            a.cache[n][:] = 1.0
+    one, zero = (torch.tensor(x).to(a.cache["k"].dtype) for x in (1.0, 0.0))
+    a.cache["k"][:], a.cache["v"][:] = zero, one
+    for b in range(seqs.batch):
+        page, slot = seqs.place(b, b)
+        a.cache["k"][page, :, slot, 0], a.cache["v"][page, :, slot] = one, zero
+    for n, x in a.cache.items():
+        a.dev[n].copy_(x)
+    a.dev["q"].copy_(a.q)
+    a.launch()
+    a.check()
