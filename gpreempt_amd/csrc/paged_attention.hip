@@ -24,6 +24,7 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
     const long cols = (long)p->heads * p->cache.head_dim;
     GP_REQUIRE(p->ld_q % 8 == 0 && p->ld_out % 8 == 0 && p->ld_q >= cols && p->ld_out >= cols, "paged_attention: row strides must be multiples of 8 elements that hold the heads");
     GP_REQUIRE(aligned16(p->q) && aligned16(p->out), "paged_attention: 16-byte alignment");
+    GP_REQUIRE(usable_scale(p->scale), "paged_attention: the scale must be 0 (for 1) or of a magnitude from 2^-100 to 2^100");
     *pl = PagedPlan{};
     FewArgs &a = pl->few;
     a.p = *p;

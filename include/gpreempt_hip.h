@@ -608,7 +608,8 @@ int gp_launch_kv_append(const gp_kv_append_params *p, const gp_preempt_ctx *ctx,
  * states in the cache.  Beyond gp_launch_attention: a cache, several query heads to one of its heads, any length, sequences of
  * their own lengths.  max_len: no sequence is longer (what lies beyond is not among the keys); sizes the launch.
  * Scores, softmax and sums in fp32; the probabilities are rounded to the type of q for the second product (fp16: times a power of two,
- * so that beside half a unit it is off by 2^-36 of the row's largest at most).  scale 0 counts as 1.
+ * so that beside half a unit it is off by 2^-36 of the row's largest at most).  scale: of a
+ * magnitude from 2^-100 to 2^100, or 0, which counts as 1.
  * What lies in the cache behind a sequence's length, or in slots that nobody has written, may be anything.  The values of a new token that is not
  * finite reach rows in front of it too (0 times infinity).  out must not overlap q or the cache.
  * work: gp_paged_attention_work_bytes() of device memory (0: none), zeroed before its first use (gp_fill32_async), and before the
