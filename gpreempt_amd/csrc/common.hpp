@@ -1,6 +1,7 @@
 // Shared host-side helpers of the device layer: error capture, handle types, dtype helpers.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -15,6 +16,9 @@ namespace gp {
 
 void set_error(const char *fmt, ...);
 int device_cus();
+
+// A factor of scores or logits that leaves fp32 room for it times log2(e), and for what it makes of differences: 0 stands for 1.
+inline bool usable_scale(float s) { return s == 0.f || (std::fabs(s) >= 0x1p-100f && std::fabs(s) <= 0x1p100f); }
 
 // For a question whose answer may be no (gp_*_supported): the text of the last error stays what it was.
 struct KeepLastError {

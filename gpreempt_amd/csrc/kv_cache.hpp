@@ -1,6 +1,5 @@
 // What the operators on a paged cache share: the check of the cache's description, and conversions of 8-bit values.
 #pragma once
-#include <cmath>
 #include "mma.hpp"
 #include "../../include/util/page_map.h"
 
@@ -18,10 +17,6 @@ inline int check_kv_cache(const gp_kv_cache &c, int dtype, const char *who) {
     GP_REQUIRE(c.dtype != GP_E4M3 || (c.k_scale && c.v_scale), "%s: an 8-bit cache needs its scales", who);
     return GP_SUCC;
 }
-
-// A factor of scores or logits that leaves fp32 room for it times log2(e), and for what it makes of differences: 0 stands for 1.  (Many query rows, say, took NaN as the
-// smallest factor)
-inline bool usable_scale(float s) { return s == 0.f || (std::fabs(s) >= 0x1p-100f && std::fabs(s) <= 0x1p100f); }
 
 // keeps the compiler from making one operation, with a single rounding, of the arithmetic in front and a conversion behind
 __device__ __forceinline__ float rounded(float x) {

@@ -11,7 +11,6 @@
 // top-th largest is a bound that at least `top` logits reach; the few groups and tiles that reach it are looked at again, what reaches it goes to a list
 // in LDS, and the largest are picked from there by their rank.
 #include <algorithm>
-#include <cmath>
 #include "mma.hpp"
 #include "lanes.hpp"
 #include "launch_tiles.hpp"
@@ -348,7 +347,7 @@ static int plan_token_logprobs(const gp_token_logprobs_params *p, LogprobsArgs *
     GP_REQUIRE(!p->top || (p->top_ids && p->top_logprobs), "token_logprobs: alternatives need a place to go to");
     GP_REQUIRE(p->logprob || p->entropy || p->top, "token_logprobs: nothing is asked for");
     GP_REQUIRE(!p->logprob || p->tokens, "token_logprobs: log probabilities of which tokens?");
-    GP_REQUIRE(p->scale >= 0.f && std::isfinite(p->scale), "token_logprobs: the scale must be finite and not negative");
+    GP_REQUIRE(p->scale >= 0.f && usable_scale(p->scale), "token_logprobs: the scale must be 0 (for 1) or from 2^-100 to 2^100");
     *a = LogprobsArgs{};
     a->p = *p;
     if (p->scale == 0.f) a->p.scale = 1.f;

@@ -20,3 +20,8 @@ def test_part_walk(tmp_path):
 @pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 3e38, -3e38, 2.0 ** 101, 2.0 ** -101, -1e-40])
 def test_attention_scales_that_are_refused(scale):
     T.refused("gp_launch_paged_attention", T.attend(scale=scale), "scale")
+
+
+@pytest.mark.parametrize("scale", [3e38, 2.0 ** 101, 2.0 ** -101, 1e-40, -0.5, -math.inf])
+def test_scales_of_logits_that_are_refused(scale):
+    T.refused("gp_launch_token_logprobs", T.logprobs(scale=scale), "scale")

@@ -85,3 +85,16 @@ def test_attention_to_many_unlikely_keys(gp, dt, cache, lens, news, heads, kv_he
     a.dev["q"].copy_(a.q)
     a.launch()
     a.check()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** 100])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_logprobs_at_the_borders_of_the_scale(gp, dt, scale):
+    """all tokens are alike, the type's lowest value among them; one takes everything"""
+    x = torch.randn((3, 40000), generator=T.gen(6)).to(S.TORCH[dt])
+    x[:, 7], x[1, 9] = 100.0, -torch.inf
+    if scale < 1:
+        x[2, 11] = torch.finfo(S.TORCH[dt]).min
+    a = T.Logprobs(gp, dt, x, torch.tensor([7, 8, 11]), 5, scale)
+    a.launch()
+    a.check()
