@@ -98,3 +98,74 @@ def test_logprobs_at_the_borders_of_the_scale(gp, dt, scale):
     a = T.Logprobs(gp, dt, x, torch.tensor([7, 8, 11]), 5, scale)
     a.launch()
     a.check()
+
+
+# ---- many query rows of 128 values -------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dt", T.DTS)
+@pytest.mark.parametrize("page", [16, 64])
+def test_many_rows_of_128_values_in_parts(gp, dt, cache, page):
+    """blocks whose keys are cut into two parts, and one of a single part"""
+    seqs = S.Sequences([1300, 1100, 900, 70], [70, 66, 80, 70], page, T.gen(10), tail=1)
+    a = T.Attend(gp, dt, dt if cache == "same" else cache, seqs, 16, 16, 128, True, 11)
+    info = a.launch()
+    assert tuple(info.shape)[:2] == (2, 64)
+    a.check()
+    first = a.left()
+    a.launch()
+    assert torch.equal(a.left(), first)
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dt", T.DTS)
+def test_many_rows_of_128_values_over_more_keys_than_a_window_of_pages(gp, dt, cache):
+    """one part of 22 tiles of keys, whose pages and scales are looked up sixteen at a time; pages that are not there in either window"""
+    seqs = S.Sequences([1400, 70], [67, 66], 64, T.gen(12), holes={(0, 3): -1, (0, 17): 10 ** 6})
+    a = T.Attend(gp, dt, dt if cache == "same" else cache, seqs, 130, 130, 128, True, 13)
+    info = a.launch()
+    assert tuple(info.shape)[:2] == (1, 260)
+    a.check()
+
+
+def test_many_rows_are_taken_in_blocks_of_128(gp):
+    """the cases of test_serving_gpu.py reach the kernel that they are about"""
+    shapes = []
+    for lens, news, page, heads, kv_heads, dim, causal in T.MANY:
+        seqs = S.Sequences(lens, news, page, T.gen(14), tail=1)
+        shapes.append(tuple(T.Attend(gp, "f16", "f16", seqs, heads, kv_heads, dim, causal, 15).launch().shape)[:2])
+    assert shapes == [(2, 64), (4, 64), (4, 64), (1, 64)]  # (blocks times parts, heads times sequences; the third: 390 rows, and 3 * 2 * 2 tiles are more than 700 keys)
+
+
+# ---- stopped with results that wait for the others' ------------------------------------------------------------------------------
+
+
+def joined_calls(gp):
+    """calls whose results are joined from parts, of more tiles than there are claim counters"""
+    rng = T.gen(20)
+    yield T.Attend(gp, "f16", "f16", S.Sequences([2000, 700, 1], None, 64, rng), 8, 4, 64, True, 21)
+    yield T.Attend(gp, "bf16", "e4m3", S.Sequences([1500, 300, 900], [6, 1, 8], 32, rng), 16, 4, 128, True, 22)
+    yield T.Attend(gp, "bf16", "e4m3", S.Sequences([1300, 1100, 900, 70], [70, 66, 80, 70], 64, rng), 16, 16, 128, True, 23)
+    yield T.Attend(gp, "f16", "f16", S.Sequences([1300, 1100, 900, 70], [70, 66, 80, 70], 16, rng), 16, 16, 128, True, 24)
+    yield T.Logprobs(gp, "bf16", torch.randn((40, 70000), generator=rng).bfloat16(), torch.arange(40), 20)
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_stopped_between_the_parts_of_a_result(gp, which):
+    """32 claim counters, served by a workgroup each: the first tile raises the flag, which its workgroup sees in front of its next one; the first result's other parts have
+    not been made then"""
+    call = list(joined_calls(gp))[which]
+    assert call.p.work_bytes and call.launch().total_tiles > 32
+    want = call.left()
+    T.clean(call)
+    flag = gp.Flag()
+    st = gp.BlpState(1, flag, 32)
+    call.launch(st.ctx(inject_at=0, max_workgroups=1, poll_every=1))
+    call.left()
+    counters = call.work[:1024].view(torch.int32)
+    assert flag.get() == 1 and st.stop_index() == 0 and int(counters[0]) > 0 and not T.same(call.left(), want)
+    flag.set(0)
+    st.clear_stop()
+    call.launch(st.ctx(max_workgroups=1, poll_every=1))
+    assert T.same(call.left(), want) and not counters.any()
