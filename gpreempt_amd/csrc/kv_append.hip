@@ -130,7 +130,7 @@ __device__ __forceinline__ void append_e4m3(const AppendArgs &a, const PageSpan 
     most = fmaxf(fmaxf(lds_most[0], lds_most[1]), fmaxf(lds_most[2], lds_most[3]));
     float *scale_at = (values ? p.cache.v_scale : p.cache.k_scale) + (long)page * p.cache.kv_heads + head;
     const float stored = span.lo ? *scale_at : 0.f;
-    const float before = stored > 0.f && stored < INFINITY ? within_scales(stored) : 0.f;  // (0: a scale that nobody has set)
+    const float before = stored > 0.f ? within_scales(stored) : 0.f;  // (0: a scale that nobody has set)
     const float scale = most > 448.f * before || before == 0.f ? scale_for(most) : before;
     const float inv = 1.f / scale;
     unsigned char *dst = (unsigned char *)(values ? p.cache.v : p.cache.k) + block;

@@ -11,10 +11,10 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["bf16"])
 def test_append_to_a_page_whose_scale_attention_takes_as_a_border(gp, dt):
     """8 bits: what append keeps, rescales and writes reads back on the scale that attention takes, 2^-60 .. 2^60, whatever scale the page came with or its values ask for"""
-    lens, page, dim = [5, 5, 5, 5, 1], 16, 64
+    lens, page, dim = [5, 5, 5, 5, 1, 5], 16, 64
     seqs = S.Sequences(lens, None, page, T.gen(1))
-    sizes = [0.0, 2.0 ** -64, 2.0 ** 62, 1.0, 2.0 ** 75]  # of the new tokens
-    before = [2.0 ** -130, 2.0 ** -70, 2.0 ** 70, 2.0 ** -126, 1.0]  # the scales of their pages (the last one begins)
+    sizes = [0.0, 2.0 ** -64, 2.0 ** 62, 1.0, 2.0 ** 75, 2.0 ** 60]  # of the new tokens
+    before = [2.0 ** -130, 2.0 ** -70, 2.0 ** 70, 2.0 ** -126, 1.0, float("inf")]  # the scales of their pages (the fifth begins)
 
     def change(a):
         for b, size in enumerate(sizes):
