@@ -582,8 +582,8 @@ typedef struct gp_kv_cache {
  * Row t of k (v, q) for head h is k + t * ld_qkv + h * head_dim (16-byte aligned rows).  Values are rounded once, to the cache's type.
  * GP_E4M3: a page's scale is set by the call that writes its slot 0, to the smallest power of two (2^-40 at least, 2^60 at most) that brings the
  * largest finite magnitude of its tokens to 448 or less; a later call raises it when larger values come.  Where that changes the scale of
- * the first page that a sequence's new tokens touch, what its other slots hold is rounded anew (nothing counts in a page whose
- * slot 0 is written: zeros); the other slots of further pages are left as they were.  Values beyond 448 scales (infinities)
+ * the first page that a sequence's new tokens touch, what its other slots hold is rounded anew, NaN staying NaN (nothing counts in a page whose
+ * slot 0 is written, so there every number becomes zero); the other slots of further pages are left as they were.  Values beyond 448 scales (infinities)
  * become the largest, NaN stays NaN.
  * No two positions of a call may share a page and a slot, nor, in GP_E4M3, may two entries of the table that are written to name one page.
  * q may be NULL (no queries); q_out may be q. */
