@@ -169,3 +169,29 @@ def test_stopped_between_the_parts_of_a_result(gp, which):
     st.clear_stop()
     call.launch(st.ctx(max_workgroups=1, poll_every=1))
     assert T.same(call.left(), want) and not counters.any()
+
+
+# ---- an append of so many tiles that a claim stands for several -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+def test_append_of_several_tiles_a_claim(gp, cache):
+    """64 sequences of a few new tokens each under a bound of 3000: most tiles find nothing to do, and those that do share a claim with others; as one launch, and stopped and resumed"""
+    news = [1 + i * 7 % 23 for i in range(64)]
+    seqs = S.Sequences([n + i * 11 % 40 for i, n in enumerate(news)], news, 16, T.gen(30), max_new=3000, tail=1)
+    a = T.Append(gp, "f16", cache, seqs, 4, 2, 64, 64, "halves", 31)
+    info = a.launch()
+    assert info.total_tiles < info.shape[0]  # (claims, tiles)
+    a.check()
+    want = a.left()
+    for limit in (1, 0):
+        T.clean(a)
+        flag = gp.Flag()
+        st = gp.BlpState(1, flag, 32)
+        a.launch(st.ctx(inject_at=1, max_workgroups=limit, poll_every=1))
+        a.left()
+        assert flag.get() == 1 and (limit == 0 or st.stop_index() == 0 and not T.same(a.left(), want))
+        flag.set(0)
+        st.clear_stop()
+        a.launch(st.ctx(max_workgroups=limit, poll_every=1))
+        assert T.same(a.left(), want)
