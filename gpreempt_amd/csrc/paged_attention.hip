@@ -33,8 +33,10 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
     if (a.p.scale == 0.f) a.p.scale = 1.f;
     const long rows = (long)a.p.max_new * a.group;
     GP_REQUIRE(rows < (1L << 30) && (long)p->batch * a.p.max_new < (1L << 31), "paged_attention: too large");
-    // Many rows: blocks of 128 of them over keys that come through LDS, if there are such blocks for a quarter of the compute units (128 rows of 8 heads of 128 over 4000 keys,
-    // e4m3: one sequence 34 us, blocks of 32 rows with the keys in parts 28; eight 48 and 44; with 256 rows each 58 and 81; 96 rows of 32 sequences over 2000 keys 63 and 97).
+    // Many rows: blocks of 128 of them over keys that come through LDS, if there are such blocks for a quarter of the compute units.  Us in such blocks / in blocks of 32 rows with
+    // the keys in parts, for rows of each of 8 cached heads of 128 over 4000 keys, e4m3: 128 rows of 1, 2, 4, 8 sequences 35 / 26, 36 / 27, 37 / 34, 38 / 43; 256 rows of 1, 2, 4, 8
+    // 36 / 27, 36 / 34, 38 / 43, 54 / 79; 96 rows of 4 (chosen: the second) 36 / 39, of 32 over 2000 keys 51 / 91.  Up to 64 rows are two blocks of 32 at most: 64 rows of 1, 8, and of 32
+    // sequences over 2000 keys 35 / 25, 37 / 38, 50 / 58.
     const long many_blocks = (rows + MANY_ROWS - 1) / MANY_ROWS, many_units = many_blocks * p->cache.kv_heads * p->batch;
     if (rows > 64 && 4 * many_units >= device_cus()) {
         const long blocks = many_blocks, tiles_y = (long)p->cache.kv_heads * p->batch, units = many_units;

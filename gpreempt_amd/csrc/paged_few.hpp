@@ -449,8 +449,9 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d, 64);
     total = __builtin_amdgcn_readfirstlane(total);
-    // (joining a part costs as much as a few units, more for more rows: 1 row of 8 heads of 128 over 1000 keys, bf16, 11.9 us in parts of two units, 14.5 in parts of four; 8 rows
-    // over 16000 keys, e4m3, 40.7 and 33.8)
+    // (joining a part costs as much as a few units, more for more rows.  Us in parts of two units / of four at least, 32 query heads over 8 cached ones of 128: one new token, which is 4 rows,
+    // over 1000 keys, bf16, 10.8 / 12.8; over 4000 and 16000, e4m3, 12.5 / 15.7 and 17.2 / 19.1; eight new tokens, which are 32 rows, 17.3 / 19.0, 22.7 / 25.2 and 39.3 / 33.2; over
+    // 131072 level, 50 and 82)
     constexpr int LEAST = NT == 1 ? 2 : 4;
     const int shares = total / LEAST < 1 ? 1 : total / LEAST < a.shares ? total / LEAST : a.shares;
     if (total == 0 || t.x >= shares) return;  // (no sequence has rows in this block)
