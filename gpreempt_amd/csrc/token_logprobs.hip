@@ -6,7 +6,7 @@
 // A few long rows are cut into parts, joined by whoever comes last.
 // Measured: 500 rows of 131001 bf16 logits, 20 alternatives: 35 us, 3.8 TB/s (a kernel that only reads: 7.1), bound by vector instructions:
 // a wavefront takes some 62 cycles of them per 64 logits (16 of these the exponential) for the maximum, the two sums and their exponents.  One row of 30522: 7.5 us, of which a launch is 4.5.
-// Rows that are walked once more for every alternative (below): the 500 rows with all logits equal 1980 us, with a NaN each 1930.
+// Rows that are walked once more for every alternative, since more logits are candidates than the list holds (below): the 500 rows with all logits equal 1980 us.
 //
 // The alternatives: every group of eight threads leaves the largest logit of each tile in LDS.  Of the 64 lanes' largest logits, all wavefronts together, the
 // top-th largest is a bound that at least `top` logits reach; the few groups and tiles that reach it are looked at again, what reaches it goes to a list
@@ -196,6 +196,10 @@ __device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, 
 
     // ---- the threads' sums ----
     const int kept = last - first < LP_KEPT ? last - first : LP_KEPT;
+    // A signalling NaN has made the instruction above forget the largest logit so far (making it a quiet one first is an instruction more for every logit of every row).  A thread that has
+    // seen one, whose sum is NaN then, has its group looked at again whatever that left.  (A bound that is too low only lets more candidates through)
+    if (top && s != s)
+        for (int i = 0; i < kept; ++i) l.groups[i][tid >> 3] = INFINITY;
     float M = max_of_wave(m);
     l.lanes[wave][tid & 63] = m;
     if ((tid & 63) == 0) l.red[0][wave] = M;
@@ -262,13 +266,11 @@ __device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, 
             p.top_logprobs[r * top + rank] = key ? (key_value(key) - M) * p.scale - log_sum : -INFINITY;
         });
     };
-    // more candidates than the list holds (equal logits, say): one after the other, each the largest behind the last one.  And so where there is a NaN (the sum is one then):
-    // a signalling one makes the instruction above forget the largest so far, which the groups' largest then do not name.  (Making it a quiet one first
-    // is an instruction more for every logit of every row)
-    if (top && (count > LP_LIST || s != s)) {
+    // more candidates than the list holds (equal logits, say): one after the other, each the largest behind the last one
+    if (top && count > LP_LIST) {
         const int from = first * LP_TILE, to = last * LP_TILE < vocab ? last * LP_TILE : vocab;
         unsigned long long before = ~0ull;
-        for (count = 0; count < top; ++count) {
+        for (int k = 0; k < top; ++k) {
             unsigned long long best = 0;
             for (int i = from + tid; i < to; i += LP_NT) {
                 const unsigned long long key = rank_key(Elem<T>::to_f(row[i]), i);
@@ -284,11 +286,11 @@ __device__ __forceinline__ void logprobs_tile(const LogprobsArgs &a, TileIdx t, 
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < LP_WAVES; ++i) best = l.list[1][i] > best ? l.list[1][i] : best;
-            if (best == 0) break;  // (no more alternatives)
-            if (tid == 0) l.list[0][count] = best;
+            if (tid == 0) l.list[0][k] = best;
             before = best;
         }
         __syncthreads();
+        count = top;
     }
     if (a.parts == 1) { finish(M, s, w, 0, count); return; }
 

@@ -637,7 +637,7 @@ int gp_launch_paged_attention(const gp_paged_attention_params *p, const gp_preem
  * Logits of -infinity have probability 0 and are no alternatives: where fewer than `top` are left, and for a row that has nothing else, the number is
  * -1 and the log probability -infinity; such an empty row has logprob -infinity and entropy 0.  A NaN or +infinity makes its row's log
  * probabilities and entropy NaN (NaN is no alternative either).  scale (one over the temperature): from 2^-100 to 2^100; 0 counts as 1.
- * A row is read once, but where more than some 1000 logits may be among its largest (equal ones, say), and where it has a NaN or +infinity, once more for each alternative.
+ * A row is read once, but where more than some 1000 logits may be among its largest (equal ones, say), once more for each alternative.
  * ld: elements from one row to the next.  work: as gp_paged_attention_params::work, of gp_token_logprobs_work_bytes(). */
 typedef struct gp_token_logprobs_params {
     int dtype;                /* of the logits: GP_F32, GP_F16 or GP_BF16 */

@@ -195,3 +195,20 @@ def test_append_of_several_tiles_a_claim(gp, cache):
         st.clear_stop()
         a.launch(st.ctx(max_workgroups=limit, poll_every=1))
         assert T.same(a.left(), want)
+
+
+@pytest.mark.parametrize("share", [0.1, 0.999])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [3, 9001, 140000])
+def test_alternatives_among_many_nans(gp, dt, vocab, share):
+    """signalling NaN for some or nearly all logits: the alternatives are what is left, also where that is fewer than are asked for"""
+    ints, bad = {"f32": (torch.int32, 0x7F800001), "bf16": (torch.int16, 0x7F81)}[dt]
+    rng = T.gen(40)
+    x = torch.randn((3, vocab), generator=rng).to(S.TORCH[dt])
+    x.view(ints)[torch.rand((3, vocab), generator=rng) < share] = bad
+    x.view(ints)[:, 1] = bad
+    a = T.Logprobs(gp, dt, x, torch.tensor([0, 1, 2]), 32)
+    a.launch()
+    got = a.left()
+    assert torch.equal(got["ids"], S.logprobs(x, torch.zeros(3), 1.0, 32)[2])
+    assert got["logprob"].isnan().all() and got["values"][got["ids"] >= 0].isnan().all() and (got["values"][got["ids"] < 0] == -torch.inf).all()
