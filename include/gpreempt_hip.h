@@ -571,8 +571,8 @@ typedef struct gp_kv_cache {
  *   page_table  batch x table_width page numbers: position p lies in page page_table[b][p / page_size], slot p % page_size
  *   tokens      rows that q, k, v and the outputs have.  Rows of no sequence are neither read nor written
  *   max_new     no sequence has more new tokens (the rows past that many of a sequence are left as they are)
- * The arrays may be written anew once the launch has run to its end (a stopped one: once it has been resumed and has).  Where lengths or row numbers change before,
- * results are wrong and a workspace has to be zeroed again, but the launch ends, and the next sentence holds.
+ * The arrays must stay as they are until the launch has run to its end (a stopped one: until it has been resumed and has): every wavefront reads them for itself, and
+ * the wavefronts of a workgroup have to agree.
  * Whatever the arrays hold, nothing outside these bounds is touched: a token at a negative position, past the table or in a page
  * that is not in the pool (a negative number marks one that is not there) is not stored, and is not among the keys. */
 
