@@ -118,6 +118,20 @@ class PagedAttentionParams(C.Structure):
                 ("work", vp), ("work_bytes", C.c_size_t)]
 
 
+class PrefixAttentionParams(C.Structure):
+    _fields_ = [("attention", PagedAttentionParams), ("shared_len", C.c_int), ("shared_table", vp)]
+
+
+class PackedAttentionParams(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("tokens", C.c_long), ("max_len", C.c_int), ("start", vp), ("heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("q", vp), ("ld_q", C.c_long), ("k", vp), ("v", vp), ("ld_kv", C.c_long), ("out", vp), ("ld_out", C.c_long), ("scale", C.c_float), ("causal", C.c_int)]
+
+
+class GemmW4Params(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("group", C.c_int), ("A", vp), ("lda", C.c_long), ("W", vp), ("ldw", C.c_long),
+                ("scales", vp), ("ld_scales", C.c_long), ("zeros", vp), ("ld_zeros", C.c_long), ("C", vp), ("ldc", C.c_long), ("bias", vp), ("residual", vp), ("act", C.c_int)]
+
+
 class TokenLogprobsParams(C.Structure):
     _fields_ = [("dtype", C.c_int), ("rows", C.c_long), ("vocab", C.c_int), ("logits", vp), ("ld", C.c_long), ("tokens", vp), ("scale", C.c_float),
                 ("logprob", vp), ("entropy", vp), ("top", C.c_int), ("top_ids", vp), ("top_logprobs", vp), ("work", vp), ("work_bytes", C.c_size_t)]
@@ -129,7 +143,7 @@ gp_stream_exists gp_stream_capturing gp_stream_query gp_stream_priority gp_strea
 gp_event_sync gp_event_query gp_event_elapsed_ms gp_malloc gp_malloc_capturing gp_free gp_host_alloc gp_host_alloc_coherent gp_host_free gp_memcpy_h2d gp_memcpy_d2h
 gp_memcpy_h2d_async gp_memcpy_d2h_async gp_memcpy_d2d_async gp_fill32_async gp_fetch gp_stage_create gp_stage_destroy gp_stage_upload_async gp_flag_create gp_flag_destroy gp_store_word_async gp_report_stop_async gp_flag_relay_start
 gp_launch_gemm gp_gemm_ln_supported gp_launch_gemm_noalloc gp_gemm_ckpt_bytes gp_conv_ckpt_bytes gp_ckpt_reset_async gp_launch_conv2d gp_conv2d_body gp_conv2d_group_supported gp_launch_conv2d_group gp_launch_nchw_to_nhwc gp_launch_pool2d gp_launch_eltwise gp_eltwise_conv2d_supported gp_launch_eltwise_conv2d gp_launch_softmax
-gp_launch_layernorm gp_launch_attention gp_launch_miniweather gp_launch_miniweather_sweep gp_launch_graph gp_launch_graph_iter gp_graph_pack_async gp_launch_embed gp_launch_kv_append gp_paged_attention_work_bytes gp_launch_paged_attention gp_token_logprobs_work_bytes gp_launch_token_logprobs gp_launch_gate gp_launch_noop gp_graph_begin gp_graph_end gp_graph_launch
+gp_launch_layernorm gp_launch_attention gp_launch_miniweather gp_launch_miniweather_sweep gp_launch_graph gp_launch_graph_iter gp_graph_pack_async gp_launch_embed gp_launch_kv_append gp_paged_attention_work_bytes gp_launch_paged_attention gp_prefix_attention_work_bytes gp_launch_prefix_attention gp_launch_packed_attention gp_launch_gemm_w4 gp_token_logprobs_work_bytes gp_launch_token_logprobs gp_launch_gate gp_launch_noop gp_graph_begin gp_graph_end gp_graph_launch
 gp_graph_destroy gp_program_create gp_program_destroy gp_program_add_gemm gp_program_add_conv2d
 gp_program_add_nchw_to_nhwc gp_program_add_pool2d gp_program_add_eltwise gp_program_add_softmax gp_program_add_layernorm
 gp_program_add_attention gp_program_add_embed gp_program_add_copy gp_program_finalize gp_program_launch gp_program_layers gp_program_read_state""".split()

@@ -1,0 +1,234 @@
+// Products of a few rows of activations with a matrix of 4-bit numbers: C = act(A W^T + bias + residual), W[n, k] = s[n, g] (q[n, k] - z[n, g]), g = k / group.
+//
+// Bound by memory for few rows: half a byte of W per 2 M flop.  So the numbers go from memory to the registers that the matrix instructions read, without LDS and
+// without a barrier in the loop.  A byte 0000qqqq is the e4m3 number 2^-9 q (fixed-point below 8, with an exponent from there on), so an instruction of the 8-bit
+// caches widens two of them to fp16 or bf16, exactly.  Scales and zeros come in once per group, in fp32, behind the products:
+//   C = sum_g s_g 2^9 (sum_k a 2^-9 q) - s_g z_g sum_k a,
+// the sums of a over a group from one more matrix instruction, whose other operand is ones.  Nothing is rounded to 16 bits but the result.
+//
+// A tile is 16 * NT rows of W and up to 16 * MT rows of A.  Its eight wavefronts take an eighth of the values of a row each, 128 at a time, and add their sums up in
+// LDS, in their order.
+//   v_mfma_f32_16x16x32   A as A: lane l has 8 values of row l % 16; W as B: lane l has 8 values of row l % 16 of W; the result's column l % 16 is a row of W, so a lane has one
+//                         scale per group.  A lane fetches 16 bytes of W: 32 neighbours, of which the four groups of 16 lanes have their own.  In groups of 128 it does not matter
+//                         which of the values meet in an instruction; for smaller ones the groups of lanes exchange what they have, so that an instruction takes 32 neighbours.
+#include "kv_cache.hpp"
+#include "paged_few.hpp"
+#include "launch_tiles.hpp"
+
+namespace gp {
+
+constexpr int W4_WAVES = 8, W4_NT = 64 * W4_WAVES;
+constexpr int W4_CHUNK = 128;  // values of a wavefront's step
+constexpr int W4_PANEL = 256;  // groups whose scales are in LDS at a time
+
+struct W4Args {
+    gp_gemm_w4_params p;
+    int groups;  // of a row
+    int panel;   // of them, at a time
+};
+inline __host__ __device__ int w4_scale_stride(int panel) { return panel + 1; }
+template <int MT, int NT> inline size_t w4_lds_bytes(int panel) {
+    return std::max((size_t)16 * NT * w4_scale_stride(panel) * sizeof(f32x2), (size_t)W4_WAVES * 256 * MT * NT * sizeof(float));
+}
+
+// rows r0 .. r3 of a 4 x 4 matrix of (registers, groups of 16 lanes) become its columns
+__device__ __forceinline__ void transpose_lane_groups(u32x4 &r) {
+    auto swap32 = [](unsigned &x, unsigned &y) { const auto s = __builtin_amdgcn_permlane32_swap(x, y, false, false); x = s[0]; y = s[1]; };
+    auto swap16 = [](unsigned &x, unsigned &y) { const auto s = __builtin_amdgcn_permlane16_swap(x, y, false, false); x = s[0]; y = s[1]; };
+    unsigned a = r[0], b = r[1], c = r[2], d = r[3];
+    swap32(a, c);
+    swap32(b, d);
+    swap16(a, b);
+    swap16(c, d);
+    r = u32x4{a, b, c, d};
+}
+
+// eight 4-bit numbers as 2^-9 times themselves, in their order
+template <typename T> __device__ __forceinline__ u32x4 widen_nibbles(unsigned raw) {
+    const unsigned even = raw & 0x0F0F0F0Fu, odd = (raw >> 4) & 0x0F0F0F0Fu;
+    const unsigned x = __builtin_amdgcn_perm(odd, even, 0x05010400u), y = __builtin_amdgcn_perm(odd, even, 0x07030602u);
+    return u32x4{widen<false>(x, T()), widen<true>(x, T()), widen<false>(y, T()), widen<true>(y, T())};
+}
+
+template <typename T, int G, int MT, int NT>
+__device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
+#pragma clang fp contract(off)  // (the plain and the preemptible kernels give the same bits)
+    const gp_gemm_w4_params &p = a.p;
+    constexpr bool WHOLE = G == W4_CHUNK;
+    constexpr int PER = G / 32;  // instructions to a group
+    constexpr int AHEAD = 4;     // steps that W is fetched ahead
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
+    const int n0 = t.x * 16 * NT, m0 = t.y * 16 * MT;
+    const unsigned char *w[NT];
+    const T *x[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int n = n0 + 16 * i + col;
+        w[i] = (const unsigned char *)p.W + (long)(n < p.N ? n : p.N - 1) * p.ldw;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int m = m0 + 16 * i + col;
+        x[i] = (const T *)p.A + (long)(m < p.M ? m : p.M - 1) * p.lda + (WHOLE ? 32 : 8) * g;
+    }
+    f32x4 total[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) total[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    typedef T tx8 __attribute__((ext_vector_type(8)));
+    tx8 one;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) one[e] = Elem<T>::from_f(1.f);
+    const u32x4 ones = __builtin_bit_cast(u32x4, one);
+    f32x2 *scales = (f32x2 *)lds;
+    const int stride = w4_scale_stride(a.panel);
+
+    for (int g0 = 0; g0 < a.groups; g0 += a.panel) {
+        const int gn = a.groups - g0 < a.panel ? a.groups - g0 : a.panel, len = gn * G;
+        const long k0 = (long)g0 * G;
+        const int chunks = (len + W4_CHUNK - 1) / W4_CHUNK, c0 = wave * chunks / W4_WAVES, c1 = (wave + 1) * chunks / W4_WAVES;
+        u32x4 raw[AHEAD][NT], act[MT][4];
+        auto load_w = [&](int c, u32x4 (&r)[NT]) {
+            const int at = 64 * c + 16 * g, last = len / 2 - 16;  // (what is behind the row's end is not multiplied)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) r[i] = load_cache<u32x4>((const char *)w[i] + k0 / 2 + (at < last ? at : last));
+        };
+        auto load_a = [&](int c, int j) {
+            const int at = c * W4_CHUNK + (WHOLE ? 8 : 32) * j;
+            if (!WHOLE && at >= len) return;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) act[i][j] = *(const u32x4 *)(x[i] + k0 + at);
+        };
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d)
+            if (c0 + d < c1) load_w(c0 + d, raw[d]);
+        if (c0 < c1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) load_a(c0, j);
+        }
+        __syncthreads();  // (what is in LDS is still being read)
+        for (int u = tid; u < 16 * NT * gn; u += W4_NT) {
+            const int r = u / gn, at = u - r * gn, n = n0 + r < p.N ? n0 + r : p.N - 1;
+            const float s = Elem<T>::to_f(((const T *)p.scales)[(long)n * p.ld_scales + g0 + at]);
+            const float z = p.zeros ? (float)p.zeros[(long)n * p.ld_zeros + g0 + at] : 8.f;
+            scales[r * stride + at] = f32x2{s * 512.f, -s * z};
+        }
+        __syncthreads();
+        auto chunk = [&](int c, u32x4 (&r)[NT]) {
+            f32x4 acc[MT][NT], sum[MT];
+            if constexpr (!WHOLE) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) transpose_lane_groups(r[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!WHOLE && c * W4_CHUNK + 32 * j >= len) break;
+                if (j % PER == 0) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int k = 0; k < NT; ++k) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < NT; ++k) {
+                    const u32x4 b = widen_nibbles<T>(r[k][j]);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) acc[i][k] = mma16(act[i][j], b, acc[i][k], T());
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) sum[i] = mma16(act[i][j], ones, sum[i], T());
+                if (c + 1 < c1) load_a(c + 1, j);
+                if (j % PER == PER - 1) {
+                    const int at = (c * W4_CHUNK + 32 * j) / G;
+#pragma unroll
+                    for (int k = 0; k < NT; ++k) {
+                        const f32x2 sz = scales[(16 * k + col) * stride + at];
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) total[i][k][e] = fmaf(sz[1], sum[i][e], fmaf(sz[0], acc[i][k][e], total[i][k][e]));
+                    }
+                }
+            }
+            if (c + AHEAD < c1) load_w(c + AHEAD, r);
+        };
+        for (int c = c0; c < c1; c += AHEAD)
+            static_for<0, AHEAD>([&](auto d) {
+                if (c + d < c1) chunk(c + d, raw[d]);
+            });
+    }
+
+    // ---- the wavefronts' sums, in their order ----
+    float *red = (float *)lds;
+    constexpr int COLS = 16 * NT, TILE = 16 * MT * COLS;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[wave * TILE + (16 * i + 4 * g + e) * COLS + 16 * k + col] = total[i][k][e];
+    __syncthreads();
+    const int rows = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT;
+    for (int u = tid; u < rows * COLS; u += W4_NT) {
+        const int m = m0 + u / COLS, n = n0 + u % COLS;
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < W4_WAVES; ++k) v += red[k * TILE + u];
+        if (n >= p.N) continue;
+        const long at = m * p.ldc + n;
+        if (p.bias) v += Elem<T>::to_f(((const T *)p.bias)[n]);
+        if (p.residual) v += Elem<T>::to_f(((const T *)p.residual)[at]);
+        ((T *)p.C)[at] = Elem<T>::from_f(rounded(apply_act(v, p.act)));
+    }
+}
+
+template <typename T, int G, int MT, int NT, int LOOP = LOOP_ANY>
+__global__ __launch_bounds__(W4_NT, MT * NT > 2 ? 2 : 4) void gemm_w4_kernel(W4Args a, BlpArgs blp) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char w4_lds[];
+    tiles<LOOP>(blp, [&](TileIdx t) { w4_tile<T, G, MT, NT>(a, t, (char *)w4_lds); });
+}
+
+template <typename T, int G, int MT, int NT>
+static int launch_w4(const W4Args &a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
+    const long nx = ((long)a.p.N + 16 * NT - 1) / (16 * NT), ny = ((long)a.p.M + 16 * MT - 1) / (16 * MT);
+    GP_REQUIRE(nx * ny < (1L << 31), "gemm_w4: too large");
+    return launch_tiles(GP_KSET(gemm_w4_kernel<T, G, MT, NT), (int)nx, (int)ny, ctx, s, info, a, w4_lds_bytes<MT, NT>(a.panel), 1, W4_NT);
+}
+
+template <typename T, int G>
+static int choose_w4(const W4Args &a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
+    if (a.p.M <= 16) return launch_w4<T, G, 1, 1>(a, ctx, s, info);
+    if (a.p.M <= 32) return launch_w4<T, G, 2, 2>(a, ctx, s, info);
+    return launch_w4<T, G, 4, 2>(a, ctx, s, info);
+}
+
+}  // namespace gp
+
+using namespace gp;
+
+extern "C" int gp_launch_gemm_w4(const gp_gemm_w4_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
+    GP_REQUIRE(p && p->A && p->W && p->scales && p->C, "null gemm_w4 params");
+    GP_REQUIRE(p->dtype == GP_F16 || p->dtype == GP_BF16, "gemm_w4: fp16 or bf16 only (dtype %d)", p->dtype);
+    GP_REQUIRE(p->M > 0 && p->N > 0 && p->K > 0, "gemm_w4: M, N and K must be positive");
+    GP_REQUIRE(p->group == 32 || p->group == 64 || p->group == 128, "gemm_w4: group must be 32, 64 or 128");
+    GP_REQUIRE(p->K % p->group == 0, "gemm_w4: K must be a multiple of the group");
+    GP_REQUIRE(p->lda % 8 == 0 && p->lda >= p->K, "gemm_w4: lda must be a multiple of 8 elements that holds a row");
+    GP_REQUIRE(p->ldw % 16 == 0 && p->ldw >= p->K / 2, "gemm_w4: ldw must be a multiple of 16 bytes that holds a row");
+    const int groups = p->K / p->group;
+    GP_REQUIRE(p->ld_scales >= groups && (!p->zeros || p->ld_zeros >= groups), "gemm_w4: row strides of scales and zeros must hold a row's groups");
+    GP_REQUIRE(p->ldc >= p->N, "gemm_w4: ldc must hold a row");
+    GP_REQUIRE(aligned16(p->A) && aligned16(p->W), "gemm_w4: A and W must be 16-byte aligned");
+    GP_REQUIRE(((uintptr_t)p->C | (uintptr_t)p->scales | (uintptr_t)p->bias | (uintptr_t)p->residual) % 2 == 0, "gemm_w4: C, scales, bias and residual must be aligned to their elements");
+    GP_REQUIRE(p->act == GP_ACT_NONE || p->act == GP_ACT_RELU || p->act == GP_ACT_GELU, "gemm_w4: act %d", p->act);
+    const W4Args a{*p, groups, std::min(groups, W4_PANEL)};
+    switch (p->group * 2 + (p->dtype == GP_F16)) {
+#define GP_W4(T, F16, G) case G * 2 + F16: return choose_w4<T, G>(a, ctx, s, info);
+        GP_W4(_Float16, 1, 32) GP_W4(__bf16, 0, 32) GP_W4(_Float16, 1, 64) GP_W4(__bf16, 0, 64) GP_W4(_Float16, 1, 128) GP_W4(__bf16, 0, 128)
+#undef GP_W4
+    }
+    return GP_OUTOFRANGE;
+}

@@ -38,30 +38,37 @@ __host__ __device__ inline int many_shares(long tiles, long most) {
 template <int D> constexpr int many_partial_floats() { return (D / 32 * 16 + 2) * MANY_NT; }  // every thread's sums as they are, its maximum and its sum
 template <int D> constexpr size_t many_lds_bytes() { return 2 * 2 * (size_t)MANY_KEYS * D * 2; }
 
-template <typename T, int D, bool E8>
-__device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *lds) {
+// Where the keys and values of one head lie: in the pages that row `b` of a table names, or (packed) in rows one behind the other
+struct PagedKeys {
+    static constexpr bool PAGED = true;
+    const gp_kv_cache &cache;
+    const int *table;
+    int width, b, kvh;
+};
+struct PackedKeys {
+    static constexpr bool PAGED = false;
+    const char *k, *v;  // of the first key
+    long ld;            // bytes from one to the next
+    int last;           // the last that there is
+};
+
+// A lane's query, and how many keys it sees (`there`: 0 .. kend; a lane without a query: nothing is asked of it)
+struct ManyRow { bool there; int seen; const void *q; };
+
+// The tiles [first_tile, tiles) of keys for 128 rows: adds up a lane's part of sum_j 2^(x_j - m) v_j in o (o[i][v] belongs to the lane's query and value
+// 32 i + 8 (v / 4) + 4 half + v % 4), sum_j 2^(x_j - m) over the lane's half of the keys in l, the reference in m.  kend: keys that some row of the block sees; the values from
+// `bound` on are taken as zeros.
+template <typename T, int D, bool E8, class Keys>
+__device__ __forceinline__ void many_keys(const Keys &keys, const ManyRow &row_of_lane, float score_scale, int kend, int bound, int first_tile, int tiles, char *lds, f32x16 (&o)[D / 32], float &m, float &l) {
 #pragma clang fp contract(off)  // (as in attend_stretch)
-    const gp_paged_attention_params &p = a.p;
     constexpr int ES = E8 ? 1 : 2, DB = D / 32, KSTEPS = D / 16;
     constexpr float ROOM = Reference<T>::room(8.f);
     constexpr int KCH = D / 8;                              // 16-byte chunks of a key's row in LDS
     constexpr int TILE_BYTES = MANY_KEYS * D * 2;           // of keys; values behind them
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5, P = p.cache.page_size;
-    const int rb = a.row_blocks - 1 - t.x / a.shares, share = t.x % a.shares, b = t.y % p.batch, kvh = t.y / p.batch;  // (the last rows see most keys: they come first)
-    const SeqTokens s = seq_tokens(p.start, p.kv_len, b, p.tokens, p.max_new);
-    const int nrows = s.rows * a.group - rb * MANY_ROWS;
-    if (nrows <= 0) return;
-    const int bound = (int)seq_bound(s, p.max_len, p.table_width, P);
-    const int last_token = (rb * MANY_ROWS + (nrows < MANY_ROWS ? nrows : MANY_ROWS) - 1) / a.group;
-    const int kend = (int)keys_seen(bound, s.first + last_token, p.causal), all_tiles = (kend + MANY_KEYS - 1) / MANY_KEYS;
-    const int shares = a.shares == 1 ? 1 : many_shares(all_tiles, a.shares);
-    if (share >= shares) return;
-    const int first_tile = (int)((long)share * all_tiles / shares), tiles = (int)((share + 1l) * all_tiles / shares);
-
-    // ---- this lane's query ----
-    const int r = wave * 32 + l32, token = (rb * MANY_ROWS + r) / a.group, hg = rb * MANY_ROWS + r - token * a.group;
-    const bool there = r < nrows;
-    const int seen = there ? (int)keys_seen(bound, s.first + token, p.causal) : 0;
+    constexpr bool PAGED = Keys::PAGED;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
+    const bool there = row_of_lane.there;
+    const int seen = row_of_lane.seen;
     int kmin = there ? seen : kend;  // what all rows of the wavefront see
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -71,8 +78,8 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
     kmin = __builtin_amdgcn_readfirstlane(kmin);
     u32x4 q[KSTEPS];
     {
-        const T *row = (const T *)p.q + (s.row0 + (there ? token : 0)) * p.ld_q + ((long)kvh * a.group + (there ? hg : 0)) * D;
-        const unsigned flip = p.scale < 0.f ? 0x80008000u : 0u;  // (so that the scale is positive from here on)
+        const T *row = (const T *)row_of_lane.q;
+        const unsigned flip = score_scale < 0.f ? 0x80008000u : 0u;  // (so that the scale is positive from here on)
 #pragma unroll
         for (int k = 0; k < KSTEPS; ++k) {
             q[k] = *(const u32x4 *)(row + 16 * k + 8 * half);
@@ -80,27 +87,29 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
             for (int e = 0; e < 4; ++e) q[k][e] = there ? q[k][e] ^ flip : 0u;
         }
     }
-    const float scale2 = fmaxf(fabsf(p.scale) * 1.44269504088896340736f, 0x1p-100f);
-    f32x16 o[DB];
+    const float scale2 = fmaxf(fabsf(score_scale) * 1.44269504088896340736f, 0x1p-100f);
 #pragma unroll
     for (int i = 0; i < DB; ++i)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[i][v] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    m = -INFINITY;
+    l = 0.f;
 
     // ---- pages: lane i has that of the i-th 16 keys of the sixteen tiles from `window` on; what a tile needs is read from there when it is needed (kept in
     // scalar registers over three steps there were too many of them: 608 us for the sequences named above, 593 so) ----
     int page_l = -1, window = first_tile;
     float ks_l = scale2, lv_l = 0.f, iv_l = 1.f;
     auto look_up = [&]() {
-        const int key = window * MANY_KEYS + lane * 16;
-        page_l = key < kend ? page_of(p.page_table, p.table_width, b, key / P, p.cache.pages) : -1;
-        if constexpr (E8) {
-            const long at = (long)(page_l < 0 ? 0 : page_l) * p.cache.kv_heads + kvh;
-            const float vs = page_scale(p.cache.v_scale, at);
-            ks_l = fmaxf(scale2 * page_scale(p.cache.k_scale, at), 0x1p-100f);  // (-infinity times it is that)
-            lv_l = __builtin_amdgcn_logf(vs);
-            iv_l = 1.f / vs;
+        if constexpr (PAGED) {
+            const int key = window * MANY_KEYS + lane * 16;
+            page_l = key < kend ? page_of(keys.table, keys.width, keys.b, key / keys.cache.page_size, keys.cache.pages) : -1;
+            if constexpr (E8) {
+                const long at = (long)(page_l < 0 ? 0 : page_l) * keys.cache.kv_heads + keys.kvh;
+                const float vs = page_scale(keys.cache.v_scale, at);
+                ks_l = fmaxf(scale2 * page_scale(keys.cache.k_scale, at), 0x1p-100f);  // (-infinity times it is that)
+                lv_l = __builtin_amdgcn_logf(vs);
+                iv_l = 1.f / vs;
+            }
         }
     };
     auto scalar = [](float v, int at) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), at)); };
@@ -113,19 +122,29 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
     static_assert(KROWS * KLOADS == MANY_KEYS, "the loads of a tile's keys");
     u32x4 kr[KLOADS];
     VRow vr[4];
-    auto block_at = [&](int page, int key) { return (((long)(page < 0 ? 0 : page) * p.cache.kv_heads + kvh) * P + (key & (P - 1))) * D * ES; };
+    auto block_at = [&](int page, int key) -> long {
+        if constexpr (PAGED) return (((long)(page < 0 ? 0 : page) * keys.cache.kv_heads + keys.kvh) * keys.cache.page_size + (key & (keys.cache.page_size - 1))) * D * ES;
+        else return (key < keys.last ? key : keys.last) * keys.ld;
+    };
+    auto cached_k = [&]() { if constexpr (PAGED) return (const char *)keys.cache.k; else return keys.k; };
+    auto cached_v = [&]() { if constexpr (PAGED) return (const char *)keys.cache.v; else return keys.v; };
     auto fetch = [&](int tile) {
         const int sub = (tile - window) * 4;
 #pragma unroll
         for (int i = 0; i < KLOADS; ++i) {
             const int row = i * KROWS + tid / (D * ES / 16), chunk = tid % (D * ES / 16);
             const int page = __builtin_amdgcn_readlane(page_l, sub + (i * KROWS + wave * (64 / (D * ES / 16))) / 16);  // (a wavefront's rows are 16 or part of them)
-            kr[i] = *(const u32x4 *)((const char *)p.cache.k + block_at(page, tile * MANY_KEYS + row) + chunk * 16);
+            kr[i] = *(const u32x4 *)(cached_k() + block_at(page, tile * MANY_KEYS + row) + chunk * 16);
         }
         const int page = __builtin_amdgcn_readlane(page_l, sub + wave), key0 = tile * MANY_KEYS + wave * 16 + lane / 16 * 4;
-        const char *at = (const char *)p.cache.v + block_at(page, key0) + lane % 16 * (VV * ES);
+        if constexpr (PAGED) {
+            const char *at = cached_v() + block_at(page, key0) + lane % 16 * (VV * ES);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) vr[e] = *(const VRow *)(at + e * D * ES);
+            for (int e = 0; e < 4; ++e) vr[e] = *(const VRow *)(at + e * D * ES);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vr[e] = *(const VRow *)(cached_v() + block_at(page, key0 + e) + lane % 16 * (VV * ES));
+        }
     };
     // ---- ... and on to LDS ----
     auto kslot = [&](int row, int chunk) { return row * (D * 2) + (chunk ^ (row & (KCH - 1))) * 16; };
@@ -148,7 +167,7 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
                 *(u32x4 *)(buf + kslot(row, chunk)) = kr[i];
             }
         }
-        const int vbound = __builtin_amdgcn_readlane(page_l, (tile - window) * 4 + wave) >= 0 ? bound : 0;
+        const int vbound = !PAGED || __builtin_amdgcn_readlane(page_l, (tile - window) * 4 + wave) >= 0 ? bound : 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (tile * MANY_KEYS + wave * 16 + lane / 16 * 4 + e >= vbound) vr[e] = VRow(0);
@@ -187,13 +206,13 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         constexpr int BUF = decltype(buffer)::value;
         const char *buf = lds + BUF * 2 * TILE_BYTES;
         const int key0 = tile * MANY_KEYS;
-        if (tile + 2 - window >= 16) { window = tile; look_up(); }  // (this tile, the one that is staged and the one that is fetched)
+        if (PAGED && tile + 2 - window >= 16) { window = tile; look_up(); }  // (this tile, the one that is staged and the one that is fetched)
         const int sub = (tile - window) * 4;
         int pages[4];
         float ks[4], lv[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            pages[u] = __builtin_amdgcn_readlane(page_l, sub + u);
+            pages[u] = PAGED ? __builtin_amdgcn_readlane(page_l, sub + u) : 0;
             ks[u] = E8 ? scalar(ks_l, sub + u) : scale2;
             lv[u] = E8 ? scalar(lv_l, sub + u) : 0.f;
         }
@@ -269,7 +288,33 @@ __device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *
         step(tile, IntC<0>());
         if (tile + 1 < tiles) step(tile + 1, IntC<1>());
     }
-    // ---- o[i][v] belongs to this lane's query and value 32 i + 8 (v / 4) + 4 half + v % 4 ----
+}
+
+template <typename T, int D, bool E8>
+__device__ __forceinline__ void attend_many(const ManyArgs &a, TileIdx t, char *lds) {
+#pragma clang fp contract(off)  // (as in attend_stretch)
+    const gp_paged_attention_params &p = a.p;
+    constexpr int DB = D / 32;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5, P = p.cache.page_size;
+    const int rb = a.row_blocks - 1 - t.x / a.shares, share = t.x % a.shares, b = t.y % p.batch, kvh = t.y / p.batch;  // (the last rows see most keys: they come first)
+    const SeqTokens s = seq_tokens(p.start, p.kv_len, b, p.tokens, p.max_new);
+    const int nrows = s.rows * a.group - rb * MANY_ROWS;
+    if (nrows <= 0) return;
+    const int bound = (int)seq_bound(s, p.max_len, p.table_width, P);
+    const int last_token = (rb * MANY_ROWS + (nrows < MANY_ROWS ? nrows : MANY_ROWS) - 1) / a.group;
+    const int kend = (int)keys_seen(bound, s.first + last_token, p.causal), all_tiles = (kend + MANY_KEYS - 1) / MANY_KEYS;
+    const int shares = a.shares == 1 ? 1 : many_shares(all_tiles, a.shares);
+    if (share >= shares) return;
+    const int first_tile = (int)((long)share * all_tiles / shares), tiles = (int)((share + 1l) * all_tiles / shares);
+
+    // ---- this lane's query ----
+    const int r = wave * 32 + l32, token = (rb * MANY_ROWS + r) / a.group, hg = rb * MANY_ROWS + r - token * a.group;
+    const bool there = r < nrows;
+    const int seen = there ? (int)keys_seen(bound, s.first + token, p.causal) : 0;
+    const T *q = (const T *)p.q + (s.row0 + (there ? token : 0)) * p.ld_q + ((long)kvh * a.group + (there ? hg : 0)) * D;
+    f32x16 o[DB];
+    float m, l;
+    many_keys<T, D, E8>(PagedKeys{p.cache, p.page_table, p.table_width, b, kvh}, ManyRow{there, seen, q}, p.scale, kend, bound, first_tile, tiles, lds, o, m, l);
     l += __shfl_xor(l, 32, 64);
     if (shares > 1) {
         // a part: every thread leaves what it has; the threads of whoever comes last take the parts, in their order, from where they left them

@@ -631,6 +631,66 @@ typedef struct gp_paged_attention_params {
 int gp_paged_attention_work_bytes(const gp_paged_attention_params *p, size_t *bytes);
 int gp_launch_paged_attention(const gp_paged_attention_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
 
+/* The same for sequences that all begin with the same shared_len tokens (a system prompt, a document), which lie in the same pages: whole pages, whose numbers
+ * shared_table (device memory, shared_len / page_size of them) has, and with which every sequence's row of the page table begins (either is read).  kv_len, positions and
+ * max_len count them.  They are read once for all sequences' rows together, not once for each.  A sequence that is shorter than
+ * shared_len sees its first kv_len tokens of them.  Results are those of gp_launch_paged_attention but for the order in which they are added up; all
+ * that is said there holds.  shared_len 0: nothing is shared.
+ * attention.work: gp_prefix_attention_work_bytes(), of a kind of its own: zeroed before its first use, serves these launches of any sizes one after the other, and no
+ * other operator's. */
+typedef struct gp_prefix_attention_params {
+    gp_paged_attention_params attention;
+    int shared_len;
+    const int *shared_table;
+} gp_prefix_attention_params;
+int gp_prefix_attention_work_bytes(const gp_prefix_attention_params *p, size_t *bytes);
+int gp_launch_prefix_attention(const gp_prefix_attention_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
+
+/* Attention over whole prompts without a cache: sequence b's tokens are the rows start[b] .. start[b + 1] - 1 of q, k, v and out (device memory, batch + 1 numbers,
+ * which must stay as they are until the launch has run to its end), and each row attends to its own sequence's rows, with `causal` to those up to itself:
+ *   out[row, h] = sum_j softmax_j(scale * <q[row, h], k_j>) v_j
+ * over keys and values of head h / (heads / kv_heads).  Beyond gp_launch_attention: sequences of any lengths side by side without padding, causal ones, several query heads to
+ * a head of keys, head_dim 128.
+ *   max_len   no sequence has more tokens (of one that has, the first max_len count and the other rows are left as they are); sizes the launch
+ *   tokens    rows that the tensors have.  Whatever `start` holds, no others are read or written, and rows of no sequence are left as they are
+ * Row t of q for head h is q + t * ld_q + h * head_dim, of k and v k (v) + t * ld_kv + h * head_dim (16-byte aligned rows); head_dim 64 or 128; GP_F16 or GP_BF16.
+ * Precision and scale: as gp_launch_paged_attention.  What is not finite among a sequence's values reaches its rows in front of it too.  out must not overlap q, k or v. */
+typedef struct gp_packed_attention_params {
+    int dtype;
+    int batch; long tokens; int max_len;
+    const int *start;
+    int heads, kv_heads, head_dim;
+    const void *q; long ld_q;
+    const void *k; const void *v; long ld_kv;
+    void *out; long ld_out;
+    float scale; int causal;
+} gp_packed_attention_params;
+int gp_launch_packed_attention(const gp_packed_attention_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
+
+/* Matrix products with weights in 4 bits: C[m, n] = act(sum_k A[m, k] W[n, k] + bias[n] + residual[m, n]), W[n, k] = scales[n, k / group] * (q[n, k] - zeros[n, k / group]).
+ *   W        N rows of K numbers q from 0 to 15, two to a byte, the even one in the lower half; ldw bytes from row to row (a multiple of 16; W 16-byte aligned)
+ *   scales   N rows of K / group numbers of the type `dtype`, ld_scales elements from row to row
+ *   zeros    the same of bytes (0 .. 255), ld_zeros; NULL: 8 everywhere
+ *   group    32, 64 or 128; K is a multiple of it
+ *   A        M rows of K values (lda a multiple of 8, A 16-byte aligned)
+ *   C, residual   M rows of N values, ldc from row to row; bias N values.  bias, residual may be NULL; residual may be C
+ * GP_F16 or GP_BF16; products and sums in fp32 (partial sums of A's values times up to 255 have to fit), one rounding at the end.  An infinity or NaN in a row of A or among the scales of a row of W makes
+ * the results it goes into infinite or NaN, which of these is not said.  C must not overlap A or W. */
+typedef struct gp_gemm_w4_params {
+    int dtype;
+    int M, N, K;
+    int group;
+    const void *A; long lda;
+    const void *W; long ldw;
+    const void *scales; long ld_scales;
+    const uint8_t *zeros; long ld_zeros;
+    void *C; long ldc;
+    const void *bias;
+    const void *residual;
+    int act;
+} gp_gemm_w4_params;
+int gp_launch_gemm_w4(const gp_gemm_w4_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
+
 /* Log probabilities under p = softmax(scale * logits[row]): for every row that of a given token, the entropy
  * (in nats), and the `top` (0 .. 32) largest with their token numbers, the lower number first among equals.
  * logprob, entropy, top_ids + top_logprobs may be NULL (not all).  A token number outside 0 .. vocab - 1 (padding) gets 0.
