@@ -16,6 +16,7 @@ ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
 MAT_AUTO, MAT_STAGED, MAT_PIPE, MAT_PIPE_SPLITK, MAT_WIDE, MAT_WIDE8 = 0, 1, 2, 3, 4, 5
 SUCC, FAIL, TIMEOUT, NOTFOUND, OUTOFRANGE, FULL = range(6)
 ROT_HALVES, ROT_NEIGHBOURS = 0, 1
+PREFIX_AUTO, PREFIX_TOGETHER, PREFIX_EACH = 0, 1, 2
 DTYPE_SIZE = {F32: 4, F16: 2, BF16: 2, I32: 4, I64: 8, E4M3: 1}
 DTYPE_BY_NAME = {"f32": F32, "f16": F16, "bf16": BF16}
 
@@ -119,7 +120,7 @@ class PagedAttentionParams(C.Structure):
 
 
 class PrefixAttentionParams(C.Structure):
-    _fields_ = [("attention", PagedAttentionParams), ("shared_len", C.c_int), ("shared_table", vp)]
+    _fields_ = [("attention", PagedAttentionParams), ("shared_len", C.c_int), ("shared_table", vp), ("variant", C.c_int)]
 
 
 class PackedAttentionParams(C.Structure):

@@ -11,6 +11,10 @@ namespace gp {
 // to its end leaves the workspace ready for any other.
 inline size_t join_counter_bytes() { return ((size_t)device_cus() * sizeof(int) + 255) / 256 * 256; }
 
+// Paged attention (paged_attention.hip) in a workspace whose first in_front bytes, join_counter_bytes() or more, are counters.
+int paged_work_bytes(const gp_paged_attention_params *p, size_t in_front, size_t *bytes);
+int launch_paged(const gp_paged_attention_params *p, size_t in_front, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
+
 // the three instantiations of one kernel: general dispatcher loop, no counters, fixed claims
 template <class Kernel> struct KernelSet { Kernel any, plain, fixed; bool long_tiles = false; };  // (long_tiles: see plan_launch)
 template <class Kernel> static KernelSet<Kernel> kernel_set(Kernel a, Kernel p, Kernel f) { return {a, p, f, false}; }

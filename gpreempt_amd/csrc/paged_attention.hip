@@ -14,7 +14,8 @@ struct PagedPlan {
     size_t work_bytes;
 };
 
-static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *pl) {
+// in_front: bytes in front of the parts of results in the workspace, the counters among them
+static int plan_paged_attention(const gp_paged_attention_params *p, size_t in_front, PagedPlan *pl) {
     GP_REQUIRE(p && p->kv_len && p->page_table && p->q && p->out, "null paged_attention params");
     if (int rc = check_kv_cache(p->cache, p->dtype, "paged_attention")) return rc;
     GP_REQUIRE(p->batch > 0 && p->tokens > 0 && p->max_new > 0 && p->max_len > 0 && p->table_width > 0, "paged_attention: batch, tokens, max_new, max_len and table_width must be positive");
@@ -44,7 +45,7 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
         GP_REQUIRE(units * want < (1L << 31), "paged_attention: too large");
         pl->many = ManyArgs{a.p, a.group, (int)blocks, (int)want, nullptr, nullptr};
         if (want > 1) {
-            const size_t counters = join_counter_bytes();  // (units: at most as many as compute units)
+            const size_t counters = in_front;  // (units: at most as many as compute units)
             pl->work_bytes = counters + (size_t)(units * want) * (p->cache.head_dim == 64 ? many_partial_floats<64>() : many_partial_floats<128>()) * sizeof(float);
             pl->many.arrived = (int *)p->work;
             pl->many.partial = (float *)((char *)p->work + counters);
@@ -67,7 +68,7 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
     pl->tiles_y = heads;
     if (most > 4) pl->tiles_x = a.shares = (int)std::min(std::max(1l, device_cus() / heads), most * p->batch);
     if (a.shares > 1) {
-        const size_t counters = join_counter_bytes();  // (heads * shares: at most as many as compute units)
+        const size_t counters = in_front;  // (heads * shares: at most as many as compute units)
         pl->work_bytes = counters + (size_t)heads * a.shares * 2 * 16 * pl->nt * (p->cache.head_dim + 2) * sizeof(float);
         a.arrived = (int *)p->work;
         a.partial = (float *)((char *)p->work + counters);
@@ -76,21 +77,16 @@ static int plan_paged_attention(const gp_paged_attention_params *p, PagedPlan *p
     return GP_SUCC;
 }
 
-}  // namespace gp
-
-using namespace gp;
-
-extern "C" int gp_paged_attention_work_bytes(const gp_paged_attention_params *p, size_t *bytes) {
+int paged_work_bytes(const gp_paged_attention_params *p, size_t in_front, size_t *bytes) {
     PagedPlan pl;
-    if (int rc = plan_paged_attention(p, &pl)) return rc;
-    GP_REQUIRE(bytes, "paged_attention: no place for the size");
+    if (int rc = plan_paged_attention(p, in_front, &pl)) return rc;
     *bytes = pl.work_bytes;
     return GP_SUCC;
 }
 
-extern "C" int gp_launch_paged_attention(const gp_paged_attention_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
+int launch_paged(const gp_paged_attention_params *p, size_t in_front, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
     PagedPlan pl;
-    if (int rc = plan_paged_attention(p, &pl)) return rc;
+    if (int rc = plan_paged_attention(p, in_front, &pl)) return rc;
     GP_REQUIRE(pl.work_bytes == 0 || (p->work && aligned16(p->work) && p->work_bytes >= pl.work_bytes), "paged_attention: needs a workspace of %zu bytes, 16-byte aligned", pl.work_bytes);
     const bool e8 = p->cache.dtype == GP_E4M3, f16 = p->dtype == GP_F16;
     if (pl.nt == 0) {
@@ -113,3 +109,17 @@ extern "C" int gp_launch_paged_attention(const gp_paged_attention_params *p, con
     }
     return GP_OUTOFRANGE;
 }
+
+}  // namespace gp
+
+using namespace gp;
+
+extern "C" int gp_paged_attention_work_bytes(const gp_paged_attention_params *p, size_t *bytes) {
+    size_t n;
+    if (int rc = paged_work_bytes(p, join_counter_bytes(), &n)) return rc;
+    GP_REQUIRE(bytes, "paged_attention: no place for the size");
+    *bytes = n;
+    return GP_SUCC;
+}
+
+extern "C" int gp_launch_paged_attention(const gp_paged_attention_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) { return launch_paged(p, join_counter_bytes(), ctx, s, info); }

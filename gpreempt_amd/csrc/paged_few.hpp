@@ -36,6 +36,7 @@ struct FewArgs {
     int shares;       // parts of the keys, per head and row block, at most; 0: every sequence is a part
     int *arrived;     // workspace: a counter for every (head, row block, part), 0 between launches
     float *partial;   // ... and for every tile two results: 16 * NT rows of D values, then their maxima and sums
+    int skip;         // keys at the beginning of every sequence that are left out
 };
 
 template <int NT, int D> constexpr int few_partial_floats() { return 16 * NT * (D + 2); }
@@ -91,14 +92,86 @@ __device__ __forceinline__ FewSequence few_sequence(const FewArgs &a, const SeqT
     const int last = (rb * ROWS + (f.nrows < ROWS ? f.nrows : ROWS) - 1) / a.group, first = rb * ROWS / a.group;
     f.kend = (int)keys_seen(f.bound, f.s.first + last, p.causal);
     f.kmin = (int)keys_seen(f.bound, f.s.first + first, p.causal);
-    f.units = f.nrows <= 0 ? 0 : f.kend <= UNIT ? 1 : (f.kend + UNIT - 1) / UNIT;
+    f.units = f.nrows <= 0 ? 0 : f.kend - a.skip <= UNIT ? 1 : (f.kend - a.skip + UNIT - 1) / UNIT;
     return f;
+}
+
+// What becomes of four values of a row's sum, v, behind its last part: here they are divided and stored
+template <typename T, int D, int ROWS> struct FewOut {
+    const FewArgs &a;
+    __device__ __forceinline__ void put(const FewSequence &f, int, int hr, int r, int d, f32x4 v, float, float sum) const {
+        const int rb = hr % a.row_blocks, kvh = hr / a.row_blocks, rr = rb * ROWS + r, token = rr / a.group, hg = rr - token * a.group;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        typedef T tx4 __attribute__((ext_vector_type(4)));
+        tx4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f(rounded(v[e] * inv));
+        *(tx4 *)((T *)a.p.out + (f.s.row0 + token) * a.p.ld_out + ((long)kvh * a.group + hg) * D + d) = y;
+    }
+    __device__ __forceinline__ void done(const FewSequence &, int, int) const {}  // all rows of the block
+};
+
+// Joins the results of `parts` parts of some rows, in their order: 16 * NT rows at most, `rows` of them there.  get(i, r, d): four values of row r of the i-th; get_ml(i, r): its reference
+// and sum; put(r, d, v, top, sum).  (up to FEW_JOIN of them at a time: first their factors, which every thread needs, then their values, eight loads of a thread in
+// flight.  A part that no row saw anything of has factor 0, and its values are zeros.)
+template <int D, int NT, int LDS_FLOATS, class Get, class GetMl, class Put>
+__device__ __forceinline__ void join_parts(int parts, int rows, float *lds, Get &&get, GetMl &&get_ml, Put &&put) {
+#pragma clang fp contract(off)
+    constexpr int ROWS = 16 * NT;
+    constexpr int FEW_JOIN = LDS_FLOATS / (2 * ROWS) < 256 ? LDS_FLOATS / (2 * ROWS) : 256;
+    constexpr int ITEMS = (ROWS * D / 4 + FEW_NT - 1) / FEW_NT;  // of a thread: four values of one row
+    const int tid = threadIdx.x;
+    f32x4 v[ITEMS];
+    float top[ITEMS], sum[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) { v[k] = f32x4{0.f, 0.f, 0.f, 0.f}; top[k] = -INFINITY; sum[k] = 0.f; }
+    for (int i0 = 0; i0 < parts; i0 += FEW_JOIN) {
+        const int n = parts - i0 < FEW_JOIN ? parts - i0 : FEW_JOIN;
+        __syncthreads();
+        for (int u = tid; u < n * rows; u += FEW_NT) {
+            const int i = u / rows, r = u - i * rows;
+            *(f32x2 *)(lds + 2 * (i * ROWS + r)) = get_ml(i0 + i, r);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
+            if (r >= rows) continue;
+            float now = top[k];
+            for (int i = 0; i < n; ++i) now = fmaxf(now, lds[2 * (i * ROWS + r)]);
+            const float base = now == -INFINITY ? 0.f : now, f0 = __builtin_amdgcn_exp2f(top[k] - base);
+            top[k] = now;
+            sum[k] *= f0;
+            v[k] *= f0;
+            for (int i = 0; i < n; i += 8) {
+                f32x4 y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    y[e] = get(i0 + (i + e < n ? i + e : i), r, d);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (i + e >= n) break;
+                    const f32x2 ms = *(const f32x2 *)(lds + 2 * ((i + e) * ROWS + r));
+                    const float f = __builtin_amdgcn_exp2f(ms[0] - base);
+                    sum[k] = fmaf(f, ms[1], sum[k]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[k][c] = fmaf(f, y[e][c], v[k][c]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
+        if (r < rows) put(r, d, v[k], top[k], sum[k]);
+    }
 }
 
 // Keys [c0, kend) of one sequence; then its rows are finished, or its part of them waits in slot `slot` for the others.
 // first_share, last_share: the parts that the sequence's keys are spread over.
-template <typename T, int D, bool E8, int NT>
-__device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequence &f, int b, int hr, int c0, int c1, float *slot, int first_share, int last_share, float *lds) {
+template <typename T, int D, bool E8, int NT, class Out>
+__device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequence &f, int b, int hr, int c0, int c1, float *slot, int first_share, int last_share, float *lds, const Out &out) {
     // (products and sums are contracted where the code says so and nowhere else, and rounded to fp32 before they are rounded to 16 bits, so that the
     // plain and the preemptible kernels give the same bits)
 #pragma clang fp contract(off)
@@ -327,15 +400,6 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
     }
     __syncthreads();
     const int rows = nrows < ROWS ? nrows : ROWS;
-    auto finish = [&](int r, int d, f32x4 v, float sum) {
-        const int rr = rb * ROWS + r, token = rr / a.group, hg = rr - token * a.group;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        typedef T tx4 __attribute__((ext_vector_type(4)));
-        tx4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = Elem<T>::from_f(rounded(v[e] * inv));
-        *(tx4 *)((T *)p.out + (s.row0 + token) * p.ld_out + ((long)kvh * a.group + hg) * D + d) = y;
-    };
     const int parts = last_share - first_share + 1;
     for (int u = tid; u < rows * (D / 4); u += FEW_NT) {
         const int r = u / (D / 4), d = u % (D / 4) * 4;
@@ -353,14 +417,17 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = fmaf(f, y[e], v[e]);
         }
-        if (parts == 1) finish(r, d, v, sum);
+        if (parts == 1) out.put(f, b, hr, r, d, v, top, sum);
         else {
             put_shared(slot + r * D + d, f32x2{v[0], v[1]});
             put_shared(slot + r * D + d + 2, f32x2{v[2], v[3]});
             if (d == 0) put_shared(slot + ROWS * D + 2 * r, f32x2{top, sum});
         }
     }
-    if (parts == 1) return;
+    if (parts == 1) {
+        out.done(f, b, hr);
+        return;
+    }
     // ---- whoever comes last joins the parts, in their order ----
     __shared__ int came;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above have reached the memory that all XCDs see
@@ -370,69 +437,24 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
     __syncthreads();
     if (came != parts - 1) return;
     if (tid == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // (up to FEW_JOIN of them at a time: first their factors, which every thread needs, then their values, eight loads of a thread in flight.
-    // A part that no row saw anything of has factor 0, and its values are zeros.)
     const float *all = a.partial + ((long)hr * a.shares + first_share) * 2 * few_partial_floats<NT, D>();
     auto part_at = [&](int i) { return all + (2l * i + (i == 0)) * few_partial_floats<NT, D>(); };  // the first part is what its tile did last
-    constexpr int FEW_JOIN = few_lds_floats<NT, D>() / (2 * ROWS) < 256 ? few_lds_floats<NT, D>() / (2 * ROWS) : 256;
-    constexpr int ITEMS = (ROWS * D / 4 + FEW_NT - 1) / FEW_NT;  // of a thread: four values of one row
-    f32x4 v[ITEMS];
-    float top[ITEMS], sum[ITEMS];
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) { v[k] = f32x4{0.f, 0.f, 0.f, 0.f}; top[k] = -INFINITY; sum[k] = 0.f; }
-    for (int i0 = 0; i0 < parts; i0 += FEW_JOIN) {
-        const int n = parts - i0 < FEW_JOIN ? parts - i0 : FEW_JOIN;
-        __syncthreads();
-        for (int u = tid; u < n * rows; u += FEW_NT) {
-            const int i = u / rows, r = u - i * rows;
-            *(f32x2 *)(lds + 2 * (i * ROWS + r)) = get_shared(part_at(i0 + i) + ROWS * D + 2 * r);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k) {
-            const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
-            if (r >= rows) continue;
-            float now = top[k];
-            for (int i = 0; i < n; ++i) now = fmaxf(now, lds[2 * (i * ROWS + r)]);
-            const float base = now == -INFINITY ? 0.f : now, f0 = __builtin_amdgcn_exp2f(top[k] - base);
-            top[k] = now;
-            sum[k] *= f0;
-            v[k] *= f0;
-            for (int i = 0; i < n; i += 8) {
-                f32x2 y[8][2];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float *from = part_at(i0 + (i + e < n ? i + e : i)) + r * D + d;
-                    y[e][0] = get_shared(from);
-                    y[e][1] = get_shared(from + 2);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (i + e >= n) break;
-                    const f32x2 ms = *(const f32x2 *)(lds + 2 * ((i + e) * ROWS + r));
-                    const float f = __builtin_amdgcn_exp2f(ms[0] - base);
-                    sum[k] = fmaf(f, ms[1], sum[k]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) v[k][c] = fmaf(f, y[e][c / 2][c % 2], v[k][c]);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-        const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
-        if (r < rows) finish(r, d, v[k], sum[k]);
-    }
+    join_parts<D, NT, few_lds_floats<NT, D>()>(parts, rows, lds, [&](int i, int r, int d) {
+        const float *from = part_at(i) + r * D + d;
+        const f32x2 x = get_shared(from), y = get_shared(from + 2);
+        return f32x4{x[0], x[1], y[0], y[1]};
+    }, [&](int i, int r) { return get_shared(part_at(i) + ROWS * D + 2 * r); }, [&](int r, int d, f32x4 v, float top, float sum) { out.put(f, b, hr, r, d, v, top, sum); });
+    out.done(f, b, hr);
 }
 
-template <typename T, int D, bool E8, int NT>
-__device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *lds) {
+template <typename T, int D, bool E8, int NT, class Out>
+__device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *lds, const Out &out) {
     const gp_paged_attention_params &p = a.p;
     constexpr int ROWS = 16 * NT, UNIT = few_unit<E8>();
     const int lane = threadIdx.x & 63, hr = t.y, rb = hr % a.row_blocks, batch = p.batch;
     if (a.shares == 0) {  // a tile per sequence
         const FewSequence f = few_sequence<ROWS, UNIT>(a, seq_tokens(p.start, p.kv_len, t.x, p.tokens, p.max_new), rb);
-        if (f.nrows > 0) attend_stretch<T, D, E8, NT>(a, f, t.x, hr, 0, f.kend, nullptr, 0, 0, lds);
+        if (f.nrows > 0) attend_stretch<T, D, E8, NT>(a, f, t.x, hr, a.skip, f.kend, nullptr, 0, 0, lds, out);
         return;
     }
     // ---- all units; then the sequence in which this part begins.  Every wavefront for itself, 64 sequences at a time, one to a lane ----
@@ -473,8 +495,8 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
         const FewSequence f = few_sequence<ROWS, UNIT>(a, seq_tokens_of(__builtin_amdgcn_readlane(r0, i), __builtin_amdgcn_readlane(r1, i), __builtin_amdgcn_readlane(len, i), p.tokens, p.max_new), rb);
         if (f.units == 0) return 0;
         const int u0 = lo > at ? lo - at : 0, u1 = hi - at < f.units ? hi - at : f.units;
-        attend_stretch<T, D, E8, NT>(a, f, b, hr, u0 * UNIT, u1 == f.units ? f.kend : u1 * UNIT, slots + (u0 == 0) * few_partial_floats<NT, D>(),
-                                     part_of(at, total, shares), part_of(at + f.units - 1l, total, shares), lds);
+        attend_stretch<T, D, E8, NT>(a, f, b, hr, a.skip + u0 * UNIT, u1 == f.units ? f.kend : a.skip + u1 * UNIT, slots + (u0 == 0) * few_partial_floats<NT, D>(),
+                                     part_of(at, total, shares), part_of(at + f.units - 1l, total, shares), lds, out);
         return f.units;
     });
 }
@@ -482,7 +504,7 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
 template <typename T, int D, bool E8, int NT, int LOOP = LOOP_ANY>
 __global__ __launch_bounds__(FEW_NT, 2) void paged_few_kernel(FewArgs a, BlpArgs blp) {
     extern __shared__ __attribute__((aligned(16))) unsigned char few_lds[];
-    tiles<LOOP>(blp, [&](TileIdx t) { attend_few<T, D, E8, NT>(a, t, (float *)few_lds); });
+    tiles<LOOP>(blp, [&](TileIdx t) { attend_few<T, D, E8, NT>(a, t, (float *)few_lds, FewOut<T, D, 16 * NT>{a}); });
 }
 
 }  // namespace gp

@@ -638,10 +638,12 @@ int gp_launch_paged_attention(const gp_paged_attention_params *p, const gp_preem
  * that is said there holds.  shared_len 0: nothing is shared.
  * attention.work: gp_prefix_attention_work_bytes(), of a kind of its own: zeroed before its first use, serves these launches of any sizes one after the other, and no
  * other operator's. */
+enum gp_prefix_variant { GP_PREFIX_AUTO = 0, GP_PREFIX_TOGETHER = 1, GP_PREFIX_EACH = 2 };
 typedef struct gp_prefix_attention_params {
     gp_paged_attention_params attention;
     int shared_len;
     const int *shared_table;
+    int variant;  /* 0 = chosen by the launcher: once for all sequences together, or for each as gp_launch_paged_attention does, which is quicker where little is shared by few */
 } gp_prefix_attention_params;
 int gp_prefix_attention_work_bytes(const gp_prefix_attention_params *p, size_t *bytes);
 int gp_launch_prefix_attention(const gp_prefix_attention_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);

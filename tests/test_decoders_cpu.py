@@ -43,8 +43,8 @@ def test_products_that_are_refused(change, says):
     refused("gp_launch_gemm_w4", w4(**change), says)
 
 
-def prefix(shared_len=32, shared_table=AT, **change):
-    return gp.PrefixAttentionParams(attention=attend(**change), shared_len=shared_len, shared_table=shared_table)
+def prefix(shared_len=32, shared_table=AT, variant=0, **change):
+    return gp.PrefixAttentionParams(attention=attend(**change), shared_len=shared_len, shared_table=shared_table, variant=variant)
 
 
 def refused_prefix(p, says):
@@ -62,10 +62,20 @@ def test_caches_that_are_refused(change, says):
     (dict(shared_len=-16), "whole pages"), (dict(shared_len=24), "whole pages"), (dict(shared_table=None), "shared pages"), (dict(dtype=gp.F32), "fp16 or bf16"), (dict(batch=0), "positive"),
     (dict(max_new=0), "positive"), (dict(max_len=0), "positive"), (dict(kv_len=None), "null"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(start=None, tokens=1), "a row for each"),
     (dict(heads=3), "multiple"), (dict(ld_q=252), "row strides"), (dict(ld_out=248), "row strides"), (dict(q=AT + 2), "alignment"), (dict(out=AT + 8), "alignment"), (dict(scale=math.nan), "scale"),
-    (dict(scale=2.0 ** -110), "scale"), (dict(scale=math.inf), "scale"),
+    (dict(scale=2.0 ** -110), "scale"), (dict(scale=math.inf), "scale"), (dict(variant=3), "variant"), (dict(variant=-1), "variant"), (dict(shared_len=1 << 30 | 16), "2^30"),
+    (dict(shared_len=0, variant=gp.PREFIX_TOGETHER), "together"), (dict(max_new=40, variant=gp.PREFIX_TOGETHER), "together"), (dict(batch=10000, tokens=20000, variant=gp.PREFIX_TOGETHER), "together"),
 ])
 def test_shared_beginnings_that_are_refused(change, says):
     refused_prefix(prefix(**change), says)
+
+
+def test_a_workspace_that_is_refused():
+    n, p = C.c_size_t(), prefix(variant=gp.PREFIX_TOGETHER)
+    gp.check(gp.lib().gp_prefix_attention_work_bytes(C.byref(p), C.byref(n)))
+    assert n.value > 0
+    for work, room in ((None, n.value), (AT, n.value - 1), (AT + 8, n.value)):
+        p.attention.work, p.attention.work_bytes = work, room
+        refused_prefix(p, "workspace")
 
 
 def packed(**change):

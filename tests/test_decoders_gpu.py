@@ -63,6 +63,7 @@ class W4:
         a, s = self.a.double(), self.scales.double().repeat_interleave(self.group, 1)
         z = 8.0 if self.zeros is None else self.zeros.double().repeat_interleave(self.group, 1)
         w, mass = (self.q.double() - z) * s, (self.q.double() + z) * s.abs()
+        self.weight_mass = a.abs() @ w.abs().t().contiguous()
         y, mass = a @ w.t().contiguous(), a.abs() @ mass.t().contiguous()
         for x in (self.bias, self.residual):
             if x is not None:
@@ -75,6 +76,8 @@ class W4:
         # each off by a unit at most.  (The activations are at most 1.13 times as steep, and off by a few units of their own.)
         deep = self.group + 2 * self.k // self.group + 32
         allowed = S.half_step(self.dt) * want.abs() + 1.13 * deep * 2.0 ** -23 * mass + (2.0 ** -25 if self.dt == "f16" else 0.0)
+        if self.m > 128:  # many rows: W is rounded to the type in front of the products: each of them is off by half a unit of |a| |w|, and fp16's smallest by half of their step
+            allowed += 1.13 * (S.half_step(self.dt) * self.weight_mass + (2.0 ** -25 if self.dt == "f16" else 0.0) * self.a.double().abs().sum(1, keepdim=True))
         err = (got[:, : self.n].double() - want).abs()
         # (from half a step above the type's largest on a value is rounded to infinity)
         border = float(torch.finfo(S.TORCH[self.dt]).max) * (1 + S.half_step(self.dt) / 2)
@@ -177,10 +180,17 @@ def begin_alike(seqs, shared):
 
 
 class Prefix(Attend):
-    def __init__(self, gp, dt, cache_dtype, seqs, *args, **kw):
+    """variant: None: together where that can be"""
+
+    def __init__(self, gp, dt, cache_dtype, seqs, *args, variant=None, **kw):
         super().__init__(gp, dt, cache_dtype, seqs, *args, **kw)
+        rows = seqs.max_new * self.heads // self.p.cache.kv_heads
+        self.together = seqs.shared > 0 and rows <= 64
+        if variant is None:
+            variant = gp.PREFIX_TOGETHER if self.together else gp.PREFIX_AUTO
         self.shared_table = seqs.table[0, : seqs.shared // seqs.page].contiguous().cuda()
-        self.prefix = gp.PrefixAttentionParams(attention=self.p, shared_len=seqs.shared, shared_table=self.shared_table.data_ptr() if seqs.shared else None)
+        self.prefix = gp.PrefixAttentionParams(attention=self.p, shared_len=seqs.shared, shared_table=self.shared_table.data_ptr() if seqs.shared else None,
+                                               variant=variant)
         self.p = self.prefix.attention
         n = gp.C.c_size_t()
         gp.check(gp.lib().gp_prefix_attention_work_bytes(gp.C.byref(self.prefix), gp.C.byref(n)))
@@ -226,6 +236,31 @@ def test_attention_behind_a_shared_beginning_matches_its_definition(gp, dt, cach
     first = a.left()
     a.clean()
     a.launch()  # the workspace is as it was
+    assert torch.equal(a.left(), first)
+
+
+@pytest.mark.parametrize("case", [1, 3, 5, 8])
+def test_for_each_sequence_as_if_nothing_were_shared(gp, case):
+    lens, news, page, shared, heads, kv_heads, dim, causal = PREFIXES[case]
+    seqs = begin_alike(S.Sequences(lens, news, page, gen(case), width=max(-(-max(lens) // page), shared // page)), shared)
+    a = Prefix(gp, "bf16", "e4m3", seqs, heads, kv_heads, dim, causal, 450 + case, variant=gp.PREFIX_EACH)
+    a.launch()
+    a.check()
+    b = Attend(gp, "bf16", "e4m3", seqs, heads, kv_heads, dim, causal, 450 + case)
+    b.launch()
+    assert torch.equal(a.left(), b.left())
+
+
+def test_what_the_launcher_chooses(gp):
+    """together where much is shared by many: more workgroups than sequences and heads; the result is what it is either way"""
+    seqs = begin_alike(S.Sequences([2048 + 1 + i % 9 for i in range(40)], None, 128, gen(21)), 2048)
+    a = Prefix(gp, "bf16", "bf16", seqs, 16, 8, 64, True, 22, variant=gp.PREFIX_AUTO)
+    assert a.launch().total_tiles > 8 * 40
+    a.check()
+    first = a.left()
+    a.prefix.variant = gp.PREFIX_TOGETHER
+    a.clean()
+    a.launch()
     assert torch.equal(a.left(), first)
 
 
@@ -476,7 +511,7 @@ def test_two_streams_at_once(gp):
 def test_one_workspace_for_batches_of_any_sizes(gp):
     made = []
     for lens, news, shared, heads, kv_heads, dim in (([1500, 1400], None, 1280, 2, 2, 64), ([1500 + i for i in range(60)], None, 1408, 8, 4, 64), ([1700, 900, 1000], [1, 9, 3], 832, 16, 8, 128),
-                                                     ([700 + i for i in range(5)], None, 640, 16, 16, 128), ([700 + i for i in range(300)], None, 640, 4, 4, 64)):
+                                                     ([700 + i for i in range(5)], None, 640, 16, 16, 128), ([700 + i for i in range(300)], None, 640, 4, 4, 64), ([2600] * 8, [70] * 8, 640, 16, 2, 64), ([1500], None, 640, 2, 2, 64)):
         made.append(Prefix(gp, "bf16", "bf16", begin_alike(S.Sequences(lens, news, 64, gen(30)), shared), heads, kv_heads, dim, True, 31 + len(made)))
     room = max(c.p.work_bytes for c in made)
     work = torch.zeros(room, dtype=torch.uint8, device="cuda")
@@ -485,6 +520,7 @@ def test_one_workspace_for_batches_of_any_sizes(gp):
         c.launch()
         want.append(c.left())
         c.p.work, c.p.work_bytes = work.data_ptr(), room
+    assert any(not c.together and c.p.work_bytes for c in made)
     for order in (made, made[::-1], made[::2] + made[1::2]):
         for c in order:
             c.clean()
@@ -556,7 +592,7 @@ def test_users_behind_one_prompt(gp, cache):
         torch.cuda.synchronize()
         gp.launch("gp_launch_gemm_w4", p, None, stream)
         stream.sync()
-        w.a, w.residual, w.c = a.cpu(), None if residual is None else residual.cpu(), c
+        w.m, w.a, w.residual, w.c = a.shape[0], a.cpu(), None if residual is None else residual.cpu(), c
         w.check()
         return c
 
