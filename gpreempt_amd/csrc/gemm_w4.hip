@@ -25,6 +25,7 @@ struct W4Args {
     gp_gemm_w4_params p;
     int groups;  // of a row
     int panel;   // of them, at a time
+    int rows, cols;  // tiles (many rows)
 };
 inline __host__ __device__ int w4_scale_stride(int panel) { return panel + 1; }
 template <int MT, int NT> inline size_t w4_lds_bytes(int panel) {
@@ -192,6 +193,157 @@ __global__ __launch_bounds__(W4_NT, MT * NT > 2 ? 2 : 4) void gemm_w4_kernel(W4A
     tiles<LOOP>(blp, [&](TileIdx t) { w4_tile<T, G, MT, NT>(a, t, (char *)w4_lds); });
 }
 
+// ---- many rows ----
+// Bound by the matrix instructions, and by the vector instructions that make 16-bit numbers of W's: two and a half for each of them, which 128 rows of A share.  A tile is 128 rows of A and
+// 256 of W, 64 to a wavefront, which has what it takes of W in registers; A comes through LDS, 128 values of a row at a time in two buffers.
+//   v_mfma_f32_32x32x16   A as A, W as B: lane l has 8 values of row l % 32; of 64 values the lanes below 32 take the first half, the others the second (16 bytes of W).
+// W's numbers are multiplied by their scale and rounded to the type in front of the products (the few rows' way, exact integers and a sum for each group, takes twice the registers and a vector instruction
+// for each result and group: there would be more of those than the matrix instructions hide).  So a result is off by half a unit of |A| |W| beside its own rounding, as if W had been kept in 16 bits.
+constexpr int W4M_NT = 256, W4M_ROWS = 128, W4M_COLS = 256, W4M_STEP = 128;
+constexpr int W4M_BUFFER = W4M_ROWS * W4M_STEP * 2;  // bytes
+constexpr int W4M_BAND = 8;  // rows of tiles that are worked on side by side
+
+// eight 4-bit numbers as scale * (number - zero); minus = -scale * zero
+template <typename T> __device__ __forceinline__ u32x4 dequantise(unsigned raw, float scale, float minus) {
+    const unsigned even = raw & 0x0F0F0F0Fu, odd = (raw >> 4) & 0x0F0F0F0Fu;
+    typedef T tx8 __attribute__((ext_vector_type(8)));
+    tx8 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        y[2 * i] = Elem<T>::from_f(fmaf((float)(even >> (8 * i) & 255u), scale, minus));
+        y[2 * i + 1] = Elem<T>::from_f(fmaf((float)(odd >> (8 * i) & 255u), scale, minus));
+    }
+    return __builtin_bit_cast(u32x4, y);
+}
+
+template <typename T>
+__device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int tile_n, char *lds) {
+#pragma clang fp contract(off)
+    const gp_gemm_w4_params &p = a.p;
+    constexpr int MB = W4M_ROWS / 32, NB = W4M_COLS / 4 / 32;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
+    const int m0 = tile_m * W4M_ROWS, n0 = tile_n * W4M_COLS + wave * 64;
+    const unsigned char *w[NB], *zero[NB];
+    const T *scale[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int n = n0 + 32 * i + l32 < p.N ? n0 + 32 * i + l32 : p.N - 1;
+        w[i] = (const unsigned char *)p.W + (long)n * p.ldw;
+        scale[i] = (const T *)p.scales + (long)n * p.ld_scales;
+        zero[i] = p.zeros ? p.zeros + (long)n * p.ld_zeros : nullptr;
+    }
+    f32x16 acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+    const int steps = (p.K + W4M_STEP - 1) / W4M_STEP;
+    // ---- A: thread (row tid / 16 + 16 i, 16 bytes tid % 16) ----
+    const int chunk = tid % 16, row = tid / 16;
+    const int slot = row * 256 + ((chunk ^ row) & 15) * 16;
+    const T *x0 = (const T *)p.A + chunk * 8;
+    u32x4 ar[8];
+    auto load_a = [&](int step) {
+        const int k = step * W4M_STEP + chunk * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int m = m0 + row + 16 * i;
+            ar[i] = *(const u32x4 *)(x0 + (long)(m < p.M ? m : p.M - 1) * p.lda + (k < p.K ? step * W4M_STEP : -chunk * 8));
+        }
+    };
+    auto store_a = [&](int step, char *buf) {
+        const bool there = step * W4M_STEP + chunk * 8 < p.K;  // (what is behind the rows' end counts as zeros)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *(u32x4 *)(buf + slot + i * 16 * 256) = there ? ar[i] : u32x4{0, 0, 0, 0};
+    };
+    // ---- W: of 64 values the lane's 32, and their scale and zero ----
+    u32x4 raw[2][NB];
+    float sc[2][NB], mi[2][NB];
+    auto load_w = [&](int step) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            int k = step * W4M_STEP + 64 * t + 32 * half;
+            if (k >= p.K) k = 0;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                raw[t][i] = *(const u32x4 *)(w[i] + k / 2);
+                const float s = Elem<T>::to_f(scale[i][k / p.group]), z = zero[i] ? (float)zero[i][k / p.group] : 8.f;
+                sc[t][i] = s;
+                mi[t][i] = -s * z;
+            }
+        }
+    };
+    load_a(0);
+    load_w(0);
+    __syncthreads();  // (the previous tile's buffers are still being read)
+    store_a(0, lds);
+    __syncthreads();
+    for (int step = 0; step < steps; ++step) {
+        const char *buf = lds + step % 2 * W4M_BUFFER;
+        const bool more = step + 1 < steps;
+        if (more) load_a(step + 1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u32x4 b[NB];
+#pragma unroll
+                for (int i = 0; i < NB; ++i) b[i] = dequantise<T>(raw[t][i][j], sc[t][i], mi[t][i]);
+#pragma unroll
+                for (int i = 0; i < MB; ++i) {
+                    const u32x4 x = *(const u32x4 *)(buf + (32 * i + l32) * 256 + (((8 * t + 4 * half + j) ^ l32) & 15) * 16);
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) Elem<T>::mma(x, b[k], acc[i][k]);
+                }
+            }
+        }
+        if (more) {
+            load_w(step + 1);
+            store_a(step + 1, lds + (step + 1) % 2 * W4M_BUFFER);
+        }
+        __syncthreads();
+    }
+    // ---- acc[i][j][v]: row 32 i + 8 (v / 4) + 4 half + v % 4 of the tile, row 32 j + l32 of the wavefront's of W ----
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int n = n0 + 32 * j + l32;
+        if (n >= p.N) continue;
+        const float bias = p.bias ? Elem<T>::to_f(((const T *)p.bias)[n]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int m = m0 + 32 * i + 8 * (v / 4) + 4 * half + v % 4;
+                if (m >= p.M) continue;
+                const long at = m * p.ldc + n;
+                float y = acc[i][j][v];
+                if (p.bias) y += bias;
+                if (p.residual) y += Elem<T>::to_f(((const T *)p.residual)[at]);
+                ((T *)p.C)[at] = Elem<T>::from_f(rounded(apply_act(y, p.act)));
+            }
+    }
+}
+
+template <typename T, int LOOP = LOOP_ANY>
+__global__ __launch_bounds__(W4M_NT, 2) void gemm_w4_many_kernel(W4Args a, BlpArgs blp) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char w4_lds[];
+    tiles<LOOP>(blp, [&](TileIdx t) {
+        // (bands of tiles: neighbours share rows of A and of W)
+        const int band = t.x / (W4M_BAND * a.cols), in = t.x - band * W4M_BAND * a.cols, high = a.rows - band * W4M_BAND < W4M_BAND ? a.rows - band * W4M_BAND : W4M_BAND;
+        w4_many_tile<T>(a, band * W4M_BAND + in % high, in / high, (char *)w4_lds);
+    });
+}
+
+template <typename T>
+static int launch_w4_many(W4Args a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
+    a.rows = (int)(((long)a.p.M + W4M_ROWS - 1) / W4M_ROWS);
+    a.cols = (int)(((long)a.p.N + W4M_COLS - 1) / W4M_COLS);
+    GP_REQUIRE((long)a.rows * a.cols < (1L << 31) && (long)a.cols * W4M_BAND < (1L << 31), "gemm_w4: too large");
+    return launch_tiles(GP_KSET(gemm_w4_many_kernel<T), a.rows * a.cols, 1, ctx, s, info, a, 2 * W4M_BUFFER, 1, W4M_NT);
+}
+
 template <typename T, int G, int MT, int NT>
 static int launch_w4(const W4Args &a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
     const long nx = ((long)a.p.N + 16 * NT - 1) / (16 * NT), ny = ((long)a.p.M + 16 * MT - 1) / (16 * MT);
@@ -201,6 +353,7 @@ static int launch_w4(const W4Args &a, const gp_preempt_ctx *ctx, gp_stream s, gp
 
 template <typename T, int G>
 static int choose_w4(const W4Args &a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
+    if (a.p.M > 128) return launch_w4_many<T>(a, ctx, s, info);
     if (a.p.M <= 16) return launch_w4<T, G, 1, 1>(a, ctx, s, info);
     if (a.p.M <= 32) return launch_w4<T, G, 2, 2>(a, ctx, s, info);
     return launch_w4<T, G, 4, 2>(a, ctx, s, info);
@@ -224,7 +377,7 @@ extern "C" int gp_launch_gemm_w4(const gp_gemm_w4_params *p, const gp_preempt_ct
     GP_REQUIRE(aligned16(p->A) && aligned16(p->W), "gemm_w4: A and W must be 16-byte aligned");
     GP_REQUIRE(((uintptr_t)p->C | (uintptr_t)p->scales | (uintptr_t)p->bias | (uintptr_t)p->residual) % 2 == 0, "gemm_w4: C, scales, bias and residual must be aligned to their elements");
     GP_REQUIRE(p->act == GP_ACT_NONE || p->act == GP_ACT_RELU || p->act == GP_ACT_GELU, "gemm_w4: act %d", p->act);
-    const W4Args a{*p, groups, std::min(groups, W4_PANEL)};
+    const W4Args a{*p, groups, std::min(groups, W4_PANEL), 0, 0};
     switch (p->group * 2 + (p->dtype == GP_F16)) {
 #define GP_W4(T, F16, G) case G * 2 + F16: return choose_w4<T, G>(a, ctx, s, info);
         GP_W4(_Float16, 1, 32) GP_W4(__bf16, 0, 32) GP_W4(_Float16, 1, 64) GP_W4(__bf16, 0, 64) GP_W4(_Float16, 1, 128) GP_W4(__bf16, 0, 128)
