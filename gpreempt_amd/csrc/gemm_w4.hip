@@ -1,23 +1,24 @@
 // Products of a few rows of activations with a matrix of 4-bit numbers: C = act(A W^T + bias + residual), W[n, k] = s[n, g] (q[n, k] - z[n, g]), g = k / group.
 //
-// Bound by memory for few rows: half a byte of W per 2 M flop.  So the numbers go from memory to the registers that the matrix instructions read, without LDS and
-// without a barrier in the loop.  A byte 0000qqqq is the e4m3 number 2^-9 q (fixed-point below 8, with an exponent from there on), so an instruction of the 8-bit
-// caches widens two of them to fp16 or bf16, exactly.  Scales and zeros come in once per group, in fp32, behind the products:
-//   C = sum_g s_g 2^9 (sum_k a 2^-9 q) - s_g z_g sum_k a,
-// the sums of a over a group from one more matrix instruction, whose other operand is ones.  Nothing is rounded to 16 bits but the result.
+// ---- few rows ----
+// Bound by memory: half a byte of W per 2 M flop.  So the numbers go from memory to the registers that the matrix instructions read, without LDS and without a barrier in the loop.  A byte 0000qqqq
+// is the e4m3 number 2^-9 q (fixed-point below 8, with an exponent from there on), so an instruction of the 8-bit caches widens two of them to fp16 or bf16, exactly.  Zeros are a second product,
+// with -2^-9 z everywhere in its other operand, and scales come in once per group, in fp32:
+//   C = sum_g 2^9 s_g (sum_k a 2^-9 q + sum_k a (-2^-9 z_g)).
+// Nothing is rounded to 16 bits but the result.
 //
-// A tile is 16 * NT rows of W and up to 16 * MT rows of A.  Its eight wavefronts take an eighth of the values of a row each, 128 at a time, and add their sums up in
-// LDS, in their order.
+// A tile is 16 * NT rows of W and up to 16 * MT rows of A.  Its wavefronts take an equal part of the values of a row each, 128 at a time, and add their sums up in LDS, in their order.
 //   v_mfma_f32_16x16x32   A as A: lane l has 8 values of row l % 16; W as B: lane l has 8 values of row l % 16 of W; the result's column l % 16 is a row of W, so a lane has one
-//                         scale per group.  A lane fetches 16 bytes of W: 32 neighbours, of which the four groups of 16 lanes have their own.  In groups of 128 it does not matter
-//                         which of the values meet in an instruction; for smaller ones the groups of lanes exchange what they have, so that an instruction takes 32 neighbours.
+//                         scale per group.  A lane fetches 16 bytes of W, 32 neighbours, and the four groups of 16 lanes exchange what they have, so that an instruction takes 32
+//                         neighbours of W and of A: within a group, and a row of A's in one piece.
+// Measured: 1 x 22528 x 4096, bf16, groups of 128: 16 us for 48 MB; 5 x 131001 x 4096, groups of 32, 97 us for 304 MB, 3.1 TB/s, of 128, 68 us, 4.2 TB/s: beside W, what is fetched of A and the vector
+// instructions (50 to 75 for 16 x 128 of W) take a share of the time that deeper prefetching, or A through LDS (a barrier a step: 68 -> 84 us), did not hide.
 #include "kv_cache.hpp"
 #include "paged_few.hpp"
 #include "launch_tiles.hpp"
 
 namespace gp {
 
-constexpr int W4_WAVES = 8, W4_NT = 64 * W4_WAVES;
 constexpr int W4_CHUNK = 128;  // values of a wavefront's step
 constexpr int W4_PANEL = 256;  // groups whose scales are in LDS at a time
 
@@ -26,10 +27,11 @@ struct W4Args {
     int groups;  // of a row
     int panel;   // of them, at a time
     int rows, cols;  // tiles (many rows)
+    int log2_group;
 };
 inline __host__ __device__ int w4_scale_stride(int panel) { return panel + 1; }
-template <int MT, int NT> inline size_t w4_lds_bytes(int panel) {
-    return std::max((size_t)16 * NT * w4_scale_stride(panel) * sizeof(f32x2), (size_t)W4_WAVES * 256 * MT * NT * sizeof(float));
+template <int MT, int NT, int WAVES> inline size_t w4_lds_bytes(int panel) {
+    return std::max((size_t)16 * NT * w4_scale_stride(panel) * sizeof(f32x2), (size_t)WAVES * 256 * MT * NT * sizeof(float));
 }
 
 // rows r0 .. r3 of a 4 x 4 matrix of (registers, groups of 16 lanes) become its columns
@@ -51,13 +53,13 @@ template <typename T> __device__ __forceinline__ u32x4 widen_nibbles(unsigned ra
     return u32x4{widen<false>(x, T()), widen<true>(x, T()), widen<false>(y, T()), widen<true>(y, T())};
 }
 
-template <typename T, int G, int MT, int NT>
+template <typename T, int G, int MT, int NT, int WAVES>
 __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
 #pragma clang fp contract(off)  // (the plain and the preemptible kernels give the same bits)
     const gp_gemm_w4_params &p = a.p;
-    constexpr bool WHOLE = G == W4_CHUNK;
+    constexpr bool WHOLE = G == W4_CHUNK;  // (K is a multiple of a step)
     constexpr int PER = G / 32;  // instructions to a group
-    constexpr int AHEAD = 4;     // steps that W is fetched ahead
+    constexpr int AHEAD_A = MT == 1 && NT == 4 ? 2 : 1, AHEAD = NT == 4 ? 2 : 4;  // steps that A and that W is fetched ahead
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
     const int n0 = t.x * 16 * NT, m0 = t.y * 16 * MT;
     const unsigned char *w[NT];
@@ -70,95 +72,108 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int m = m0 + 16 * i + col;
-        x[i] = (const T *)p.A + (long)(m < p.M ? m : p.M - 1) * p.lda + (WHOLE ? 32 : 8) * g;
+        x[i] = (const T *)p.A + (long)(m < p.M ? m : p.M - 1) * p.lda + 8 * g;
     }
     f32x4 total[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) total[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    typedef T tx8 __attribute__((ext_vector_type(8)));
-    tx8 one;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) one[e] = Elem<T>::from_f(1.f);
-    const u32x4 ones = __builtin_bit_cast(u32x4, one);
+    typedef T tx2 __attribute__((ext_vector_type(2)));
     f32x2 *scales = (f32x2 *)lds;
     const int stride = w4_scale_stride(a.panel);
 
     for (int g0 = 0; g0 < a.groups; g0 += a.panel) {
         const int gn = a.groups - g0 < a.panel ? a.groups - g0 : a.panel, len = gn * G;
         const long k0 = (long)g0 * G;
-        const int chunks = (len + W4_CHUNK - 1) / W4_CHUNK, c0 = wave * chunks / W4_WAVES, c1 = (wave + 1) * chunks / W4_WAVES;
-        u32x4 raw[AHEAD][NT], act[MT][4];
+        const int chunks = (len + W4_CHUNK - 1) / W4_CHUNK, c0 = wave * chunks / WAVES, c1 = (wave + 1) * chunks / WAVES;
+        u32x4 raw[AHEAD][NT], act[AHEAD_A][MT][4];
         auto load_w = [&](int c, u32x4 (&r)[NT]) {
             const int at = 64 * c + 16 * g, last = len / 2 - 16;  // (what is behind the row's end is not multiplied)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) r[i] = load_cache<u32x4>((const char *)w[i] + k0 / 2 + (at < last ? at : last));
+            for (int i = 0; i < NT; ++i) r[i] = *(const u32x4 *)(w[i] + k0 / 2 + (at < last ? at : last));
         };
-        auto load_a = [&](int c, int j) {
-            const int at = c * W4_CHUNK + (WHOLE ? 8 : 32) * j;
+        auto load_a = [&](int c, int j, u32x4 (&to)[MT][4]) {
+            const int at = c * W4_CHUNK + 32 * j;
             if (!WHOLE && at >= len) return;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) act[i][j] = *(const u32x4 *)(x[i] + k0 + at);
+            for (int i = 0; i < MT; ++i) to[i][j] = *(const u32x4 *)(x[i] + k0 + at);
         };
 #pragma unroll
         for (int d = 0; d < AHEAD; ++d)
             if (c0 + d < c1) load_w(c0 + d, raw[d]);
-        if (c0 < c1) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) load_a(c0, j);
-        }
+        for (int d = 0; d < AHEAD_A; ++d)
+            if (c0 + d < c1) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) load_a(c0 + d, j, act[d]);
+            }
         __syncthreads();  // (what is in LDS is still being read)
-        for (int u = tid; u < 16 * NT * gn; u += W4_NT) {
-            const int r = u / gn, at = u - r * gn, n = n0 + r < p.N ? n0 + r : p.N - 1;
-            const float s = Elem<T>::to_f(((const T *)p.scales)[(long)n * p.ld_scales + g0 + at]);
-            const float z = p.zeros ? (float)p.zeros[(long)n * p.ld_zeros + g0 + at] : 8.f;
-            scales[r * stride + at] = f32x2{s * 512.f, -s * z};
+        // (eight neighbouring groups of a row to a thread; rows start anywhere)
+        typedef T Eight __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+        typedef unsigned char Bytes __attribute__((ext_vector_type(8), aligned(1)));
+        const int per_row = (gn + 7) / 8;
+#pragma unroll 2
+        for (int u = tid; u < 16 * NT * per_row; u += 64 * WAVES) {
+            const int r = u / per_row, at = (u - r * per_row) * 8, n = n0 + r < p.N ? n0 + r : p.N - 1;
+            const T *from = (const T *)p.scales + (long)n * p.ld_scales + g0 + at;
+            const uint8_t *zero = p.zeros ? p.zeros + (long)n * p.ld_zeros + g0 + at : nullptr;
+            Eight s = {};
+            Bytes z = {8, 8, 8, 8, 8, 8, 8, 8};
+            if (at + 8 <= gn) {
+                s = *(const Eight *)from;
+                if (zero) z = *(const Bytes *)zero;
+            } else {
+                for (int e = 0; e < gn - at; ++e) {
+                    s[e] = from[e];
+                    if (zero) z[e] = zero[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const T minus = Elem<T>::from_f((float)z[e] * -0x1p-9f);  // (exact: a whole number of eight bits)
+                if (at + e < gn) scales[r * stride + at + e] = f32x2{Elem<T>::to_f(s[e]) * 512.f, __builtin_bit_cast(float, tx2{minus, minus})};
+            }
         }
         __syncthreads();
-        auto chunk = [&](int c, u32x4 (&r)[NT]) {
-            f32x4 acc[MT][NT], sum[MT];
-            if constexpr (!WHOLE) {
+        auto chunk = [&](int c, u32x4 (&r)[NT], u32x4 (&a)[MT][4]) {
+            f32x4 acc[MT][NT];
+            f32x2 sz[NT];
 #pragma unroll
-                for (int i = 0; i < NT; ++i) transpose_lane_groups(r[i]);
-            }
+            for (int i = 0; i < NT; ++i) transpose_lane_groups(r[i]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (!WHOLE && c * W4_CHUNK + 32 * j >= len) break;
                 if (j % PER == 0) {
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int k = 0; k < NT; ++k) acc[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    }
+                    for (int k = 0; k < NT; ++k) sz[k] = scales[(16 * k + col) * stride + (c * W4_CHUNK + 32 * j) / G];
                 }
 #pragma unroll
                 for (int k = 0; k < NT; ++k) {
                     const u32x4 b = widen_nibbles<T>(r[k][j]);
+                    const float second = sz[k][1];  // (a bit cast of a vector's element itself takes its first)
+                    const unsigned zero = __builtin_bit_cast(unsigned, second);
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) acc[i][k] = mma16(act[i][j], b, acc[i][k], T());
+                    for (int i = 0; i < MT; ++i) {
+                        acc[i][k] = mma16(a[i][j], u32x4{zero, zero, zero, zero}, j % PER == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][k], T());
+                        acc[i][k] = mma16(a[i][j], b, acc[i][k], T());
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < MT; ++i) sum[i] = mma16(act[i][j], ones, sum[i], T());
-                if (c + 1 < c1) load_a(c + 1, j);
+                if (c + AHEAD_A < c1) load_a(c + AHEAD_A, j, a);
                 if (j % PER == PER - 1) {
-                    const int at = (c * W4_CHUNK + 32 * j) / G;
 #pragma unroll
-                    for (int k = 0; k < NT; ++k) {
-                        const f32x2 sz = scales[(16 * k + col) * stride + at];
+                    for (int k = 0; k < NT; ++k)
 #pragma unroll
                         for (int i = 0; i < MT; ++i)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) total[i][k][e] = fmaf(sz[1], sum[i][e], fmaf(sz[0], acc[i][k][e], total[i][k][e]));
-                    }
+                            for (int e = 0; e < 4; ++e) total[i][k][e] = fmaf(sz[k][0], acc[i][k][e], total[i][k][e]);
                 }
             }
             if (c + AHEAD < c1) load_w(c + AHEAD, r);
         };
         for (int c = c0; c < c1; c += AHEAD)
             static_for<0, AHEAD>([&](auto d) {
-                if (c + d < c1) chunk(c + d, raw[d]);
+                if (c + d < c1) chunk(c + d, raw[d], act[d % AHEAD_A]);
             });
     }
 
@@ -174,11 +189,11 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
             for (int e = 0; e < 4; ++e) red[wave * TILE + (16 * i + 4 * g + e) * COLS + 16 * k + col] = total[i][k][e];
     __syncthreads();
     const int rows = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT;
-    for (int u = tid; u < rows * COLS; u += W4_NT) {
+    for (int u = tid; u < rows * COLS; u += 64 * WAVES) {
         const int m = m0 + u / COLS, n = n0 + u % COLS;
         float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < W4_WAVES; ++k) v += red[k * TILE + u];
+        for (int k = 0; k < WAVES; ++k) v += red[k * TILE + u];
         if (n >= p.N) continue;
         const long at = m * p.ldc + n;
         if (p.bias) v += Elem<T>::to_f(((const T *)p.bias)[n]);
@@ -187,10 +202,10 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
     }
 }
 
-template <typename T, int G, int MT, int NT, int LOOP = LOOP_ANY>
-__global__ __launch_bounds__(W4_NT, MT * NT > 2 ? 2 : 4) void gemm_w4_kernel(W4Args a, BlpArgs blp) {
+template <typename T, int G, int MT, int NT, int WAVES, int LOOP = LOOP_ANY>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : MT * NT > 2 ? 2 : 4) void gemm_w4_kernel(W4Args a, BlpArgs blp) {
     extern __shared__ __attribute__((aligned(16))) unsigned char w4_lds[];
-    tiles<LOOP>(blp, [&](TileIdx t) { w4_tile<T, G, MT, NT>(a, t, (char *)w4_lds); });
+    tiles<LOOP>(blp, [&](TileIdx t) { w4_tile<T, G, MT, NT, WAVES>(a, t, (char *)w4_lds); });
 }
 
 // ---- many rows ----
@@ -199,30 +214,31 @@ __global__ __launch_bounds__(W4_NT, MT * NT > 2 ? 2 : 4) void gemm_w4_kernel(W4A
 //   v_mfma_f32_32x32x16   A as A, W as B: lane l has 8 values of row l % 32; of 64 values the lanes below 32 take the first half, the others the second (16 bytes of W).
 // W's numbers are multiplied by their scale and rounded to the type in front of the products (the few rows' way, exact integers and a sum for each group, takes twice the registers and a vector instruction
 // for each result and group: there would be more of those than the matrix instructions hide).  So a result is off by half a unit of |A| |W| beside its own rounding, as if W had been kept in 16 bits.
-constexpr int W4M_NT = 256, W4M_ROWS = 128, W4M_COLS = 256, W4M_STEP = 128;
+constexpr int W4M_NT = 256, W4M_ROWS = 128, W4M_STEP = 128;
 constexpr int W4M_BUFFER = W4M_ROWS * W4M_STEP * 2;  // bytes
 constexpr int W4M_BAND = 8;  // rows of tiles that are worked on side by side
 
 // eight 4-bit numbers as scale * (number - zero); minus = -scale * zero
 template <typename T> __device__ __forceinline__ u32x4 dequantise(unsigned raw, float scale, float minus) {
-    const unsigned even = raw & 0x0F0F0F0Fu, odd = (raw >> 4) & 0x0F0F0F0Fu;
-    typedef T tx8 __attribute__((ext_vector_type(8)));
-    tx8 y;
+    unsigned even = raw & 0x0F0F0F0Fu, odd = (raw >> 4) & 0x0F0F0F0Fu;
+    asm("" : "+v"(even), "+v"(odd));  // (a byte to fp32 is one instruction; the compiler goes back to `raw`, and shifts and masks for each of them: 688 vector instructions a step for 400)
+    typedef T tx2 __attribute__((ext_vector_type(2)));
+    u32x4 y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        y[2 * i] = Elem<T>::from_f(fmaf((float)(even >> (8 * i) & 255u), scale, minus));
-        y[2 * i + 1] = Elem<T>::from_f(fmaf((float)(odd >> (8 * i) & 255u), scale, minus));
+        const f32x2 x = {fmaf((float)(even >> (8 * i) & 255u), scale, minus), fmaf((float)(odd >> (8 * i) & 255u), scale, minus)};
+        y[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, tx2));
     }
-    return __builtin_bit_cast(u32x4, y);
+    return y;
 }
 
-template <typename T>
+template <typename T, bool WHOLE, int NB>
 __device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int tile_n, char *lds) {
 #pragma clang fp contract(off)
     const gp_gemm_w4_params &p = a.p;
-    constexpr int MB = W4M_ROWS / 32, NB = W4M_COLS / 4 / 32;
+    constexpr int MB = W4M_ROWS / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
-    const int m0 = tile_m * W4M_ROWS, n0 = tile_n * W4M_COLS + wave * 64;
+    const int m0 = tile_m * W4M_ROWS, n0 = (tile_n * 4 + wave) * 32 * NB;
     const unsigned char *w[NB], *zero[NB];
     const T *scale[NB];
 #pragma unroll
@@ -230,7 +246,7 @@ __device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int ti
         const int n = n0 + 32 * i + l32 < p.N ? n0 + 32 * i + l32 : p.N - 1;
         w[i] = (const unsigned char *)p.W + (long)n * p.ldw;
         scale[i] = (const T *)p.scales + (long)n * p.ld_scales;
-        zero[i] = p.zeros ? p.zeros + (long)n * p.ld_zeros : nullptr;
+        zero[i] = p.zeros ? p.zeros + (long)n * p.ld_zeros : w[i];  // (where there are none, something is fetched all the same and left: no branch in the loop)
     }
     f32x16 acc[MB][NB];
 #pragma unroll
@@ -250,47 +266,56 @@ __device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int ti
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int m = m0 + row + 16 * i;
-            ar[i] = *(const u32x4 *)(x0 + (long)(m < p.M ? m : p.M - 1) * p.lda + (k < p.K ? step * W4M_STEP : -chunk * 8));
+            ar[i] = *(const u32x4 *)(x0 + (long)(m < p.M ? m : p.M - 1) * p.lda + (WHOLE || k < p.K ? step * W4M_STEP : -chunk * 8));
         }
     };
     auto store_a = [&](int step, char *buf) {
-        const bool there = step * W4M_STEP + chunk * 8 < p.K;  // (what is behind the rows' end counts as zeros)
+        const bool there = WHOLE || step * W4M_STEP + chunk * 8 < p.K;  // (what is behind the rows' end counts as zeros)
 #pragma unroll
         for (int i = 0; i < 8; ++i) *(u32x4 *)(buf + slot + i * 16 * 256) = there ? ar[i] : u32x4{0, 0, 0, 0};
     };
     // ---- W: of 64 values the lane's 32, and their scale and zero ----
     u32x4 raw[2][NB];
-    float sc[2][NB], mi[2][NB];
-    auto load_w = [&](int step) {
+    T sc[2][NB];
+    unsigned char ze[2][NB];
+    auto load_w = [&](int step, int t) {
+        int k = step * W4M_STEP + 64 * t + 32 * half;
+        if (!WHOLE && k >= p.K) k = 0;
+        const int g = k >> a.log2_group;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            int k = step * W4M_STEP + 64 * t + 32 * half;
-            if (k >= p.K) k = 0;
-#pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                raw[t][i] = *(const u32x4 *)(w[i] + k / 2);
-                const float s = Elem<T>::to_f(scale[i][k / p.group]), z = zero[i] ? (float)zero[i][k / p.group] : 8.f;
-                sc[t][i] = s;
-                mi[t][i] = -s * z;
+        for (int i = 0; i < NB; ++i) {
+            raw[t][i] = *(const u32x4 *)(w[i] + k / 2);
+            if (!WHOLE || t == 1) {
+                sc[t][i] = scale[i][g];
+                ze[t][i] = zero[i][g];
             }
         }
     };
     load_a(0);
-    load_w(0);
+    load_w(0, 0);
+    load_w(0, 1);
     __syncthreads();  // (the previous tile's buffers are still being read)
     store_a(0, lds);
     __syncthreads();
     for (int step = 0; step < steps; ++step) {
         const char *buf = lds + step % 2 * W4M_BUFFER;
-        const bool more = step + 1 < steps;
-        if (more) load_a(step + 1);
+        const int next = step + 1 < steps ? step + 1 : step;  // (behind the last step: the last one again, which nobody reads)
+        load_a(next);
+        float s[NB], minus[NB];  // (groups of 128: those of the whole step, else of the lane's 32 values)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            if (!WHOLE || t == 0) {
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    s[i] = Elem<T>::to_f(sc[WHOLE ? 1 : t][i]);
+                    minus[i] = -s[i] * (p.zeros ? (float)ze[WHOLE ? 1 : t][i] : 8.f);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 u32x4 b[NB];
 #pragma unroll
-                for (int i = 0; i < NB; ++i) b[i] = dequantise<T>(raw[t][i][j], sc[t][i], mi[t][i]);
+                for (int i = 0; i < NB; ++i) b[i] = dequantise<T>(raw[t][i][j], s[i], minus[i]);
 #pragma unroll
                 for (int i = 0; i < MB; ++i) {
                     const u32x4 x = *(const u32x4 *)(buf + (32 * i + l32) * 256 + (((8 * t + 4 * half + j) ^ l32) & 15) * 16);
@@ -298,11 +323,9 @@ __device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int ti
                     for (int k = 0; k < NB; ++k) Elem<T>::mma(x, b[k], acc[i][k]);
                 }
             }
+            load_w(next, t);
         }
-        if (more) {
-            load_w(step + 1);
-            store_a(step + 1, lds + (step + 1) % 2 * W4M_BUFFER);
-        }
+        store_a(next, lds + (step + 1) % 2 * W4M_BUFFER);
         __syncthreads();
     }
     // ---- acc[i][j][v]: row 32 i + 8 (v / 4) + 4 half + v % 4 of the tile, row 32 j + l32 of the wavefront's of W ----
@@ -326,37 +349,48 @@ __device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int ti
     }
 }
 
-template <typename T, int LOOP = LOOP_ANY>
+template <typename T, bool WHOLE, int NB, int LOOP = LOOP_ANY>
 __global__ __launch_bounds__(W4M_NT, 2) void gemm_w4_many_kernel(W4Args a, BlpArgs blp) {
     extern __shared__ __attribute__((aligned(16))) unsigned char w4_lds[];
     tiles<LOOP>(blp, [&](TileIdx t) {
         // (bands of tiles: neighbours share rows of A and of W)
         const int band = t.x / (W4M_BAND * a.cols), in = t.x - band * W4M_BAND * a.cols, high = a.rows - band * W4M_BAND < W4M_BAND ? a.rows - band * W4M_BAND : W4M_BAND;
-        w4_many_tile<T>(a, band * W4M_BAND + in % high, in / high, (char *)w4_lds);
+        w4_many_tile<T, WHOLE, NB>(a, band * W4M_BAND + in % high, in / high, (char *)w4_lds);
     });
 }
 
-template <typename T>
+template <typename T, bool WHOLE, int NB>
 static int launch_w4_many(W4Args a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
     a.rows = (int)(((long)a.p.M + W4M_ROWS - 1) / W4M_ROWS);
-    a.cols = (int)(((long)a.p.N + W4M_COLS - 1) / W4M_COLS);
+    a.cols = (int)(((long)a.p.N + 128 * NB - 1) / (128 * NB));
     GP_REQUIRE((long)a.rows * a.cols < (1L << 31) && (long)a.cols * W4M_BAND < (1L << 31), "gemm_w4: too large");
-    return launch_tiles(GP_KSET(gemm_w4_many_kernel<T), a.rows * a.cols, 1, ctx, s, info, a, 2 * W4M_BUFFER, 1, W4M_NT);
+    return launch_tiles(GP_KSET(gemm_w4_many_kernel<T, WHOLE, NB), a.rows * a.cols, 1, ctx, s, info, a, 2 * W4M_BUFFER, 1, W4M_NT);
 }
 
-template <typename T, int G, int MT, int NT>
+template <typename T, int G, int MT, int NT, int WAVES>
 static int launch_w4(const W4Args &a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
     const long nx = ((long)a.p.N + 16 * NT - 1) / (16 * NT), ny = ((long)a.p.M + 16 * MT - 1) / (16 * MT);
     GP_REQUIRE(nx * ny < (1L << 31), "gemm_w4: too large");
-    return launch_tiles(GP_KSET(gemm_w4_kernel<T, G, MT, NT), (int)nx, (int)ny, ctx, s, info, a, w4_lds_bytes<MT, NT>(a.panel), 1, W4_NT);
+    return launch_tiles(GP_KSET(gemm_w4_kernel<T, G, MT, NT, WAVES), (int)nx, (int)ny, ctx, s, info, a, w4_lds_bytes<MT, NT, WAVES>(a.panel), 1, 64 * WAVES);
 }
 
 template <typename T, int G>
 static int choose_w4(const W4Args &a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
-    if (a.p.M > 128) return launch_w4_many<T>(a, ctx, s, info);
-    if (a.p.M <= 16) return launch_w4<T, G, 1, 1>(a, ctx, s, info);
-    if (a.p.M <= 32) return launch_w4<T, G, 2, 2>(a, ctx, s, info);
-    return launch_w4<T, G, 4, 2>(a, ctx, s, info);
+    // Many rows' tiles of 128 x 128 or 128 x 256, or few rows at a time.  Us, few / 128 x 128 / 128 x 256, bf16, K = 4096 (768 where N is 2304), groups of 128: 128 x 4096 24 / 55 / 86,
+    // 256 x 4096 48 / 56 / 86, 512 x 4096 96 / 68 / 97, 1024 x 1024 43 / 67 / 95, 300 x 2304 14.5 / 17.4 / 29, 600 x 2304 20.9 / 17.9 / 29, 64 x 22528 65 / 70 / 94, 128 x 22528 130 / 69 / 95,
+    // 2048 x 4096 355 / 90 / 106, 512 x 22528 469 / 145 / 133.
+    const long tiles = ((long)a.p.M + W4M_ROWS - 1) / W4M_ROWS * (((long)a.p.N + 127) / 128);
+    if (a.p.M > 64 && 3 * tiles >= device_cus())
+        return tiles > 2 * device_cus() ? launch_w4_many<T, G == W4M_STEP, 2>(a, ctx, s, info) : launch_w4_many<T, G == W4M_STEP, 1>(a, ctx, s, info);
+    // Rows of W for each wavefront, and wavefronts: what is fetched of A counts as much as W does, so a wavefront takes several rows' sixteens at once where there are enough of them for all compute
+    // units.  Us (K = 4096, groups of 128, bf16) in tiles of 16 rows for 8 wavefronts / 32 for 4 / 64 for 4: 1 x 4096 6.0 / 8.2 / 10.6, 1 x 22528 19 / 16.2 / 17.0, 5 x 131001 104 / 87 / 68,
+    // 24 x 4096 10.6 / 12 / 15, 24 x 22528 48 / 35 / 27, 24 x 131001 246 / 178 / 107, 64 x 4096 19 / 24, 64 x 22528 106 / 57.
+    const long sixteens = ((long)a.p.N + 15) / 16;
+    if (sixteens < 4l * device_cus())
+        return a.p.M <= 16 ? launch_w4<T, G, 1, 1, 8>(a, ctx, s, info) : a.p.M <= 32 ? launch_w4<T, G, 2, 1, 8>(a, ctx, s, info) : launch_w4<T, G, 4, 1, 8>(a, ctx, s, info);
+    if (a.p.M > 32) return launch_w4<T, G, 4, 2, 4>(a, ctx, s, info);
+    if (a.p.M > 16) return launch_w4<T, G, 2, 4, 4>(a, ctx, s, info);
+    return sixteens < 16l * device_cus() ? launch_w4<T, G, 1, 2, 4>(a, ctx, s, info) : launch_w4<T, G, 1, 4, 4>(a, ctx, s, info);
 }
 
 }  // namespace gp
@@ -377,7 +411,7 @@ extern "C" int gp_launch_gemm_w4(const gp_gemm_w4_params *p, const gp_preempt_ct
     GP_REQUIRE(aligned16(p->A) && aligned16(p->W), "gemm_w4: A and W must be 16-byte aligned");
     GP_REQUIRE(((uintptr_t)p->C | (uintptr_t)p->scales | (uintptr_t)p->bias | (uintptr_t)p->residual) % 2 == 0, "gemm_w4: C, scales, bias and residual must be aligned to their elements");
     GP_REQUIRE(p->act == GP_ACT_NONE || p->act == GP_ACT_RELU || p->act == GP_ACT_GELU, "gemm_w4: act %d", p->act);
-    const W4Args a{*p, groups, std::min(groups, W4_PANEL), 0, 0};
+    const W4Args a{*p, groups, std::min(groups, W4_PANEL), 0, 0, p->group == 32 ? 5 : p->group == 64 ? 6 : 7};
     switch (p->group * 2 + (p->dtype == GP_F16)) {
 #define GP_W4(T, F16, G) case G * 2 + F16: return choose_w4<T, G>(a, ctx, s, info);
         GP_W4(_Float16, 1, 32) GP_W4(__bf16, 0, 32) GP_W4(_Float16, 1, 64) GP_W4(__bf16, 0, 64) GP_W4(_Float16, 1, 128) GP_W4(__bf16, 0, 128)
