@@ -124,9 +124,11 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
                 s = *(const Eight *)from;
                 if (zero) z = *(const Bytes *)zero;
             } else {
-                for (int e = 0; e < gn - at; ++e) {
-                    s[e] = from[e];
-                    if (zero) z[e] = zero[e];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {  // (behind the last one that one again, so that all are fetched at once)
+                    const int i = at + e < gn ? e : gn - 1 - at;
+                    s[e] = from[i];
+                    if (zero) z[e] = zero[i];
                 }
             }
 #pragma unroll

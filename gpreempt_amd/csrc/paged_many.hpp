@@ -128,7 +128,29 @@ __device__ __forceinline__ void many_keys(const Keys &keys, const ManyRow &row_o
     };
     auto cached_k = [&]() { if constexpr (PAGED) return (const char *)keys.cache.k; else return keys.k; };
     auto cached_v = [&]() { if constexpr (PAGED) return (const char *)keys.cache.v; else return keys.v; };
+    // (packed: a lane's rows of a tile as offsets of 32 bits from the tile's first, which the wavefront shares; in the tile where the sequence ends they stop at its last row.  A multiplication of 64 bits
+    // for each load instead: 1540 us for 1520)
+    unsigned krow[KLOADS], vrow[4];
+    auto look_at_rows = [&](int last) {
+        if constexpr (!PAGED) {
+            auto row = [&](int r) { return (unsigned)(r < last ? r : last) * (unsigned)keys.ld; };
+#pragma unroll
+            for (int i = 0; i < KLOADS; ++i) krow[i] = row(i * KROWS + tid / (D * ES / 16)) + tid % (D * ES / 16) * 16;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vrow[e] = row(wave * 16 + lane / 16 * 4 + e) + lane % 16 * (VV * ES);
+        }
+    };
+    look_at_rows(MANY_KEYS);
     auto fetch = [&](int tile) {
+        if constexpr (!PAGED) {
+            if (tile * MANY_KEYS + MANY_KEYS > keys.last) look_at_rows(keys.last - tile * MANY_KEYS);
+            const char *k = keys.k + tile * MANY_KEYS * keys.ld, *v = keys.v + tile * MANY_KEYS * keys.ld;
+#pragma unroll
+            for (int i = 0; i < KLOADS; ++i) kr[i] = *(const u32x4 *)(k + krow[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vr[e] = *(const VRow *)(v + vrow[e]);
+            return;
+        }
         const int sub = (tile - window) * 4;
 #pragma unroll
         for (int i = 0; i < KLOADS; ++i) {

@@ -88,7 +88,7 @@ def packed(**change):
     (dict(dtype=gp.F32), "fp16 or bf16"), (dict(dtype=gp.E4M3), "fp16 or bf16"), (dict(batch=0), "positive"), (dict(tokens=0), "positive"), (dict(max_len=0), "positive"), (dict(max_len=-5), "positive"),
     (dict(start=None), "null"), (dict(q=None), "null"), (dict(k=None), "null"), (dict(v=None), "null"), (dict(out=None), "null"), (dict(heads=3), "multiple"), (dict(heads=0), "multiple"),
     (dict(kv_heads=0), "multiple"), (dict(head_dim=96), "head_dim"), (dict(head_dim=256), "head_dim"), (dict(ld_q=252), "row strides"), (dict(ld_q=248), "row strides"), (dict(ld_kv=120), "row strides"),
-    (dict(ld_out=248), "row strides"), (dict(ld_out=-256), "row strides"), (dict(q=AT + 8), "alignment"), (dict(k=AT + 2), "alignment"), (dict(v=AT + 8), "alignment"), (dict(out=2 * AT + 8), "alignment"),
+    (dict(ld_out=248), "row strides"), (dict(ld_out=-256), "row strides"), (dict(ld_kv=(1 << 25) + 8), "2^25"), (dict(q=AT + 8), "alignment"), (dict(k=AT + 2), "alignment"), (dict(v=AT + 8), "alignment"), (dict(out=2 * AT + 8), "alignment"),
     (dict(scale=math.nan), "scale"), (dict(scale=2.0 ** 101), "scale"), (dict(tokens=1 << 30, max_len=1 << 30), "too large"),
     (dict(tokens=1 << 29, max_len=1 << 28, batch=1 << 20), "too large"),
 ])
