@@ -4,7 +4,7 @@
 // Bound by memory: half a byte of W per 2 M flop.  So the numbers go from memory to the registers that the matrix instructions read, without LDS and without a barrier in the loop.  A byte 0000qqqq
 // is the e4m3 number 2^-9 q (fixed-point below 8, with an exponent from there on), so an instruction of the 8-bit caches widens two of them to fp16 or bf16, exactly.  Zeros are a second product,
 // with -2^-9 z everywhere in its other operand, and scales come in once per group, in fp32:
-//   C = sum_g 2^9 s_g (sum_k a 2^-9 q + sum_k a (-2^-9 z_g)).
+//   C = 2^9 sum_g s_g (sum_k a 2^-9 q + sum_k a (-2^-9 z_g)).
 // Nothing is rounded to 16 bits but the result.
 //
 // A tile is 16 * NT rows of W and up to 16 * MT rows of A.  Its wavefronts take an equal part of the values of a row each, 128 at a time, and add their sums up in LDS, in their order.
@@ -31,7 +31,7 @@ struct W4Args {
 };
 inline __host__ __device__ int w4_scale_stride(int panel) { return panel + 1; }
 template <int MT, int NT, int WAVES> inline size_t w4_lds_bytes(int panel) {
-    return std::max((size_t)16 * NT * w4_scale_stride(panel) * sizeof(f32x2), (size_t)WAVES * 256 * MT * NT * sizeof(float));
+    return std::max((size_t)16 * NT * w4_scale_stride(panel) * sizeof(unsigned), (size_t)WAVES * 256 * MT * NT * sizeof(float));
 }
 
 // rows r0 .. r3 of a 4 x 4 matrix of (registers, groups of 16 lanes) become its columns
@@ -80,7 +80,7 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) total[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     typedef T tx2 __attribute__((ext_vector_type(2)));
-    f32x2 *scales = (f32x2 *)lds;
+    unsigned *scales = (unsigned *)lds;  // a group's scale, and -2^-9 times its zero
     const int stride = w4_scale_stride(a.panel);
 
     for (int g0 = 0; g0 < a.groups; g0 += a.panel) {
@@ -134,13 +134,13 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const T minus = Elem<T>::from_f((float)z[e] * -0x1p-9f);  // (exact: a whole number of eight bits)
-                if (at + e < gn) scales[r * stride + at + e] = f32x2{Elem<T>::to_f(s[e]) * 512.f, __builtin_bit_cast(float, tx2{minus, minus})};
+                if (at + e < gn) scales[r * stride + at + e] = __builtin_bit_cast(unsigned, tx2{s[e], minus});
             }
         }
         __syncthreads();
         auto chunk = [&](int c, u32x4 (&r)[NT], u32x4 (&a)[MT][4]) {
             f32x4 acc[MT][NT];
-            f32x2 sz[NT];
+            unsigned sz[NT];
 #pragma unroll
             for (int i = 0; i < NT; ++i) transpose_lane_groups(r[i]);
 #pragma unroll
@@ -153,8 +153,7 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
 #pragma unroll
                 for (int k = 0; k < NT; ++k) {
                     const u32x4 b = widen_nibbles<T>(r[k][j]);
-                    const float second = sz[k][1];  // (a bit cast of a vector's element itself takes its first)
-                    const unsigned zero = __builtin_bit_cast(unsigned, second);
+                    const unsigned zero = __builtin_amdgcn_perm(sz[k], sz[k], 0x07060706u);
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
                         acc[i][k] = mma16(a[i][j], u32x4{zero, zero, zero, zero}, j % PER == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][k], T());
@@ -164,11 +163,14 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
                 if (c + AHEAD_A < c1) load_a(c + AHEAD_A, j, a);
                 if (j % PER == PER - 1) {
 #pragma unroll
-                    for (int k = 0; k < NT; ++k)
+                    for (int k = 0; k < NT; ++k) {
+                        const tx2 both = __builtin_bit_cast(tx2, sz[k]);
+                        const float scale = Elem<T>::to_f(both[0]);
 #pragma unroll
                         for (int i = 0; i < MT; ++i)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) total[i][k][e] = fmaf(sz[k][0], acc[i][k][e], total[i][k][e]);
+                            for (int e = 0; e < 4; ++e) total[i][k][e] = fmaf(scale, acc[i][k][e], total[i][k][e]);
+                    }
                 }
             }
             if (c + AHEAD < c1) load_w(c + AHEAD, r);
@@ -197,6 +199,7 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
 #pragma unroll
         for (int k = 0; k < WAVES; ++k) v += red[k * TILE + u];
         if (n >= p.N) continue;
+        v *= 512.f;
         const long at = m * p.ldc + n;
         if (p.bias) v += Elem<T>::to_f(((const T *)p.bias)[n]);
         if (p.residual) v += Elem<T>::to_f(((const T *)p.residual)[at]);
@@ -403,6 +406,7 @@ extern "C" int gp_launch_gemm_w4(const gp_gemm_w4_params *p, const gp_preempt_ct
     GP_REQUIRE(p && p->A && p->W && p->scales && p->C, "null gemm_w4 params");
     GP_REQUIRE(p->dtype == GP_F16 || p->dtype == GP_BF16, "gemm_w4: fp16 or bf16 only (dtype %d)", p->dtype);
     GP_REQUIRE(p->M > 0 && p->N > 0 && p->K > 0, "gemm_w4: M, N and K must be positive");
+    GP_REQUIRE(p->M <= (1 << 30) && p->N <= (1 << 30) && p->K <= (1 << 30), "gemm_w4: M, N and K must be at most 2^30");
     GP_REQUIRE(p->group == 32 || p->group == 64 || p->group == 128, "gemm_w4: group must be 32, 64 or 128");
     GP_REQUIRE(p->K % p->group == 0, "gemm_w4: K must be a multiple of the group");
     GP_REQUIRE(p->lda % 8 == 0 && p->lda >= p->K, "gemm_w4: lda must be a multiple of 8 elements that holds a row");

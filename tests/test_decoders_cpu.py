@@ -33,7 +33,7 @@ def w4(**change):
 
 
 @pytest.mark.parametrize("change,says", [
-    (dict(dtype=gp.F32), "fp16 or bf16"), (dict(dtype=gp.E4M3), "fp16 or bf16"), (dict(M=0), "positive"), (dict(N=-1), "positive"), (dict(K=0), "positive"), (dict(group=0), "group"),
+    (dict(dtype=gp.F32), "fp16 or bf16"), (dict(dtype=gp.E4M3), "fp16 or bf16"), (dict(M=0), "positive"), (dict(N=-1), "positive"), (dict(K=0), "positive"), (dict(M=(1 << 30) + 1), "2^30"), (dict(N=(1 << 30) + 1, ldc=1 << 31), "2^30"), (dict(K=(1 << 30) + 64, lda=1 << 31, ldw=1 << 30, ld_scales=1 << 30, ld_zeros=1 << 30), "2^30"), (dict(group=0), "group"),
     (dict(group=16), "group"), (dict(group=256), "group"), (dict(K=224, lda=224), "multiple of the group"), (dict(lda=248), "lda"), (dict(lda=260), "lda"), (dict(ldw=120), "ldw"), (dict(ldw=112), "ldw"),
     (dict(ld_scales=3), "row strides"), (dict(ld_zeros=3), "row strides"), (dict(ldc=49), "ldc"), (dict(A=None), "null"), (dict(W=None), "null"), (dict(scales=None), "null"), (dict(C=None), "null"),
     (dict(A=AT + 8), "16-byte"), (dict(W=AT + 4), "16-byte"), (dict(C=2 * AT + 1), "elements"), (dict(scales=AT + 1), "elements"), (dict(bias=AT + 1), "elements"), (dict(residual=AT + 1), "elements"),
