@@ -655,7 +655,7 @@ int gp_launch_prefix_attention(const gp_prefix_attention_params *p, const gp_pre
  * a head of keys, head_dim 128.
  *   max_len   no sequence has more tokens (of one that has, the first max_len count and the other rows are left as they are); sizes the launch
  *   tokens    rows that the tensors have.  Whatever `start` holds, no others are read or written, and rows of no sequence are left as they are
- * Row t of q for head h is q + t * ld_q + h * head_dim, of k and v k (v) + t * ld_kv + h * head_dim (16-byte aligned rows); head_dim 64 or 128; GP_F16 or GP_BF16.
+ * Row t of q for head h is q + t * ld_q + h * head_dim, of k and v k (v) + t * ld_kv + h * head_dim (16-byte aligned rows, ld_kv at most 2^25); head_dim 64 or 128; GP_F16 or GP_BF16.
  * Precision and scale: as gp_launch_paged_attention.  What is not finite among a sequence's values reaches its rows in front of it too.  out must not overlap q, k or v. */
 typedef struct gp_packed_attention_params {
     int dtype;
@@ -676,8 +676,9 @@ int gp_launch_packed_attention(const gp_packed_attention_params *p, const gp_pre
  *   group    32, 64 or 128; K is a multiple of it
  *   A        M rows of K values (lda a multiple of 8, A 16-byte aligned)
  *   C, residual   M rows of N values, ldc from row to row; bias N values.  bias, residual may be NULL; residual may be C
- * GP_F16 or GP_BF16; products and sums in fp32 (partial sums of A's values times up to 255 have to fit), one rounding at the end.  An infinity or NaN in a row of A or among the scales of a row of W makes
- * the results it goes into infinite or NaN, which of these is not said.  C must not overlap A or W. */
+ * GP_F16 or GP_BF16; M, N and K at most 2^30; sums in fp32 (A's values times up to 255 have to fit).  Up to 64 rows of A nothing but the result is rounded to 16 bits; for more, W may be rounded to the type in
+ * front of the products, as if it had been kept in 16 bits.  An infinity or NaN in a row of A or among the scales of a row of W makes the results it goes into infinite or NaN, which of these is not
+ * said.  C must not overlap A, W, scales, zeros or bias. */
 typedef struct gp_gemm_w4_params {
     int dtype;
     int M, N, K;

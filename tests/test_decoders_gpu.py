@@ -92,6 +92,9 @@ W4S = [
     (17, 40, 448, 64), (31, 65, 1280, 128), (32, 7, 160, 32), (33, 100, 256, 64), (63, 130, 384, 128), (64, 32, 224, 32), (65, 257, 512, 128), (100, 31, 320, 64),
     (129, 130, 352, 32), (130, 300, 1152, 128), (200, 515, 576, 64), (257, 256, 256, 128),
     (2, 20, 32 * 300, 32), (20, 20, 64 * 258, 64), (40, 9, 32 * 513, 32),  # scales in several panels
+    (3, 16400, 96, 32), (20, 16401, 160, 32), (50, 16400, 128, 64), (2, 65600, 128, 128),  # more rows of W to a wavefront
+    (1101, 1303, 160, 32), (1101, 1303, 192, 64), (1100, 1302, 384, 128), (1025, 1281, 32, 32),  # tiles of 128 x 128
+    (2945, 3001, 96, 32), (2945, 3001, 320, 64), (3000, 2945, 256, 128),  # ... of 128 x 256
 ]
 
 
@@ -110,7 +113,7 @@ def test_products_match_their_definition(gp, dt, case):
 
 @pytest.mark.parametrize("dt", DTS)
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("m", [16, 48, 128, 384])
+@pytest.mark.parametrize("m", [16, 48, 128, 384, 1100])
 def test_every_number_is_where_it_belongs(gp, dt, group, m):
     """rows of A with a single one: a column of W each, exactly"""
     k = 384
@@ -118,14 +121,14 @@ def test_every_number_is_where_it_belongs(gp, dt, group, m):
     def one_hot(w):
         w.a.zero_()
         w.a[torch.arange(m), torch.arange(m) * 5 % k] = 1.0
-    w = W4(gp, dt, m, 77, k, group, 3, bias=False, residual=False, spread=256, change=one_hot)
+    w = W4(gp, dt, m, 77 if m < 1000 else 1301, k, group, 3, bias=False, residual=False, spread=256, change=one_hot)
     w.launch()
     exact = ((w.q.double() - w.zeros.double().repeat_interleave(group, 1)) * w.scales.double().repeat_interleave(group, 1))[:, torch.arange(m) * 5 % k].t()
     assert torch.equal(w.left(), exact.to(S.TORCH[dt]))
 
 
 @pytest.mark.parametrize("dt", DTS)
-@pytest.mark.parametrize("m", [3, 40, 200])
+@pytest.mark.parametrize("m", [3, 40, 200, 1200])
 def test_rows_of_large_and_of_no_size(gp, dt, m):
     """rows of zeros, of one sign and far from zero, of the type's smallest and of large values; a row with a NaN and one with an infinity, which nobody else sees"""
     def change(w):
@@ -137,7 +140,7 @@ def test_rows_of_large_and_of_no_size(gp, dt, m):
             w.a[m - 2, 17], w.a[m - 1, 5] = math.nan, math.inf
         w.scales[1], w.scales[2, 1] = 0.0, -0.5
         w.scales[3] *= 2.0 ** -9
-    w = W4(gp, dt, m, 150, 512, 64, 5, residual=False, change=change)
+    w = W4(gp, dt, m, 150 if m < 1000 else 1301, 512, 64, 5, residual=False, change=change)
     w.launch()
     got = w.left()
     if m > 3:
@@ -147,26 +150,23 @@ def test_rows_of_large_and_of_no_size(gp, dt, m):
     w.check()
 
 
-def test_weights_and_rows_behind_four_gigabytes(gp):
+@pytest.mark.parametrize("m, n", [(3, 40), (200, 40), (1101, 1301)])
+def test_weights_and_rows_behind_four_gigabytes(gp, m, n):
     """the last rows of W, A and C lie behind 2^32 bytes (2^31 elements); the bits of the same call close together"""
-    for m in (3, 200):
-        small = W4(gp, "f16", m, 40, 256, 128, 8, residual=False)
-        small.launch()
-        want = small.left()
-        far, p = W4(gp, "f16", m, 40, 256, 128, 8, residual=False), None
-        p = far.p
-        ldw = (1 << 32) // 39 // 16 * 16 + 16
-        lda = (1 << 32) // (m - 1) // 8 * 8 + 8
-        w, a, c = (torch.empty(n, dtype=t, device="cuda") for n, t in ((ldw * 39 + 128, torch.uint8), (lda * (m - 1) + 256, torch.half), (lda * (m - 1) + 40, torch.half)))
-        for n in range(40):
-            w[n * ldw: n * ldw + 128] = far.dev["w"][n]
-        for r in range(m):
-            a[r * lda: r * lda + 256] = far.dev["a"][r]
-        p.W, p.ldw, p.A, p.lda, p.C, p.ldc = w.data_ptr(), ldw, a.data_ptr(), lda, c.data_ptr(), lda
-        far.launch()
-        torch.cuda.synchronize()
-        for r in range(m):
-            assert torch.equal(c[r * lda: r * lda + 40].cpu(), want[r]), (m, r)
+    small = W4(gp, "f16", m, n, 256, 128, 8, residual=False)
+    small.launch()
+    want = small.left()
+    far = W4(gp, "f16", m, n, 256, 128, 8, residual=False)
+    p = far.p
+    ldw, ld = (1 << 32) // (n - 1) // 16 * 16 + 16, (1 << 32) // (m - 1) // 8 * 8 + 8
+    ld = max(ld, (n + 7) // 8 * 8)
+    w, a, c = (torch.empty(size, dtype=t, device="cuda") for size, t in ((ldw * (n - 1) + 128, torch.uint8), (ld * (m - 1) + 256, torch.half), (ld * (m - 1) + n, torch.half)))
+    w.as_strided((n, 128), (ldw, 1)).copy_(far.dev["w"])
+    a.as_strided((m, 256), (ld, 1)).copy_(far.dev["a"])
+    p.W, p.ldw, p.A, p.lda, p.C, p.ldc = w.data_ptr(), ldw, a.data_ptr(), ld, c.data_ptr(), ld
+    far.launch()
+    torch.cuda.synchronize()
+    assert torch.equal(c.as_strided((m, n), (ld, 1)).cpu(), want)
 
 
 # ---- sequences that begin alike -------------------------------------------------------------------------------------------
@@ -221,6 +221,10 @@ PREFIXES = [
     ([400, 500, 700], None, 64, 0, 8, 2, 64, True),                 # nothing is shared
     ([2100, 2050], None, 128, 2048, 16, 1, 128, True),
     ([600, 700], [90, 70], 64, 512, 8, 2, 64, True),                # many rows of each
+    ([1900, 1810, 1801], [8, 7, 8], 128, 1792, 8, 1, 128, True),    # 64 rows, the most that go together; seven parts
+    ([800, 790, 781, 800, 770], [11, 4, 11, 1, 2], 16, 768, 8, 2, 128, True),  # 44 rows, two blocks of 32; three parts
+    ([640 + 2600, 640 + 40, 640 + 1300, 640 + 1], None, 64, 640, 4, 2, 64, True),  # own keys in parts
+    ([640 + 2600, 640 + 40, 640 + 1300], [6, 6, 5], 64, 640, 8, 2, 128, False),
 ]
 
 
@@ -453,7 +457,7 @@ def test_packed_rows_behind_four_gigabytes(gp):
 
 
 def calls(gp):
-    got = [W4(gp, "bf16", 1, 300, 512, 128, 600), W4(gp, "f16", 20, 200, 384, 64, 601), W4(gp, "f16", 300, 520, 256, 32, 602, in_place=True, act="gelu"), W4(gp, "bf16", 600, 600, 512, 128, 603)]
+    got = [W4(gp, "bf16", 1, 300, 512, 128, 600), W4(gp, "f16", 20, 200, 384, 64, 601), W4(gp, "f16", 1100, 1300, 256, 32, 602, in_place=True, act="gelu"), W4(gp, "bf16", 3000, 2900, 256, 128, 603)]
     got.append(Prefix(gp, "f16", "f16", begin_alike(S.Sequences([2000, 1700, 1600], None, 64, gen(62)), 1536), 8, 4, 64, True, 63))
     got.append(Prefix(gp, "bf16", "e4m3", begin_alike(S.Sequences([900, 800, 1500], [3, 1, 4], 32, gen(64)), 768), 8, 4, 128, True, 65))
     got.append(Prefix(gp, "bf16", "bf16", begin_alike(S.Sequences([1300 + i for i in range(70)], None, 64, gen(66)), 1280), 8, 2, 64, True, 67))
