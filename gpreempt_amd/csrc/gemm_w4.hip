@@ -11,8 +11,8 @@
 //   v_mfma_f32_16x16x32   A as A: lane l has 8 values of row l % 16; W as B: lane l has 8 values of row l % 16 of W; the result's column l % 16 is a row of W, so a lane has one
 //                         scale per group.  A lane fetches 16 bytes of W, 32 neighbours, and the four groups of 16 lanes exchange what they have, so that an instruction takes 32
 //                         neighbours of W and of A: within a group, and a row of A's in one piece.
-// Measured: 1 x 22528 x 4096, bf16, groups of 128: 16 us for 48 MB; 5 x 131001 x 4096, groups of 32, 97 us for 304 MB, 3.1 TB/s, of 128, 68 us, 4.2 TB/s: beside W, what is fetched of A and the vector
-// instructions (50 to 75 for 16 x 128 of W) take a share of the time that deeper prefetching, or A through LDS (a barrier a step: 68 -> 84 us), did not hide.
+// Measured: 1 x 22528 x 4096, bf16, groups of 128: 15 us for 48 MB; 5 x 131001 x 4096, groups of 32, 85 us for 304 MB, 3.6 TB/s, of 128, 64 us, 4.4 TB/s: beside W, what is fetched of A and the vector
+// instructions (50 to 75 for 16 x 128 of W) take a share of the time that deeper prefetching, or A through LDS (a barrier a step: 68 -> 84 us, of 128), did not hide.
 #include "kv_cache.hpp"
 #include "paged_few.hpp"
 #include "launch_tiles.hpp"
@@ -215,10 +215,11 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : MT * NT > 2 ? 2 : 4) 
 
 // ---- many rows ----
 // Bound by the matrix instructions, and by the vector instructions that make 16-bit numbers of W's: two and a half for each of them, which 128 rows of A share.  A tile is 128 rows of A and
-// 256 of W, 64 to a wavefront, which has what it takes of W in registers; A comes through LDS, 128 values of a row at a time in two buffers.
+// 256 or 128 of W, a quarter to a wavefront, which has what it takes of W in registers; A comes through LDS, 128 values of a row at a time in two buffers.
 //   v_mfma_f32_32x32x16   A as A, W as B: lane l has 8 values of row l % 32; of 64 values the lanes below 32 take the first half, the others the second (16 bytes of W).
 // W's numbers are multiplied by their scale and rounded to the type in front of the products (the few rows' way, exact integers and a sum for each group, takes twice the registers and a vector instruction
 // for each result and group: there would be more of those than the matrix instructions hide).  So a result is off by half a unit of |A| |W| beside its own rounding, as if W had been kept in 16 bits.
+// Measured: 4001 x 8192 x 8192, bf16, groups of 128: 553 to 581 us on different days, 925 to 970 TFLOP/s (a large matrix product of 16 bits: 1150); the matrix instructions take 50 % of the cycles.
 constexpr int W4M_NT = 256, W4M_ROWS = 128, W4M_STEP = 128;
 constexpr int W4M_BUFFER = W4M_ROWS * W4M_STEP * 2;  // bytes
 constexpr int W4M_BAND = 8;  // rows of tiles that are worked on side by side
