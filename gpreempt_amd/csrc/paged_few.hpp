@@ -36,7 +36,7 @@ struct FewArgs {
     int shares;       // parts of the keys, per head and row block, at most; 0: every sequence is a part
     int *arrived;     // workspace: a counter for every (head, row block, part), 0 between launches
     float *partial;   // ... and for every tile two results: 16 * NT rows of D values, then their maxima and sums
-    int skip;         // keys at the beginning of every sequence that are left out
+    int skip;         // keys at the beginning that are left out, of the sequences all of whose rows see them
 };
 
 template <int NT, int D> constexpr int few_partial_floats() { return 16 * NT * (D + 2); }
@@ -79,10 +79,11 @@ template <typename V> __device__ __forceinline__ V load_cache(const char *p) { r
 struct FewSequence {
     SeqTokens s;
     int nrows;       // of the block and those behind it
+    int skip;        // the first key
     int bound, kmin, kend;  // keys; those that every row of the block sees, and that some row does
     int units;       // of few_unit keys: what the parts are made of (a sequence that sees nothing counts as one: it gets its zeros)
 };
-template <int ROWS, int UNIT>
+template <int ROWS, int UNIT, bool SKIPS>
 __device__ __forceinline__ FewSequence few_sequence(const FewArgs &a, const SeqTokens &s, int rb) {
     const gp_paged_attention_params &p = a.p;
     FewSequence f;
@@ -92,12 +93,14 @@ __device__ __forceinline__ FewSequence few_sequence(const FewArgs &a, const SeqT
     const int last = (rb * ROWS + (f.nrows < ROWS ? f.nrows : ROWS) - 1) / a.group, first = rb * ROWS / a.group;
     f.kend = (int)keys_seen(f.bound, f.s.first + last, p.causal);
     f.kmin = (int)keys_seen(f.bound, f.s.first + first, p.causal);
-    f.units = f.nrows <= 0 ? 0 : f.kend - a.skip <= UNIT ? 1 : (f.kend - a.skip + UNIT - 1) / UNIT;
+    f.skip = SKIPS && keys_seen(f.bound, f.s.first, p.causal) >= a.skip ? a.skip : 0;
+    f.units = f.nrows <= 0 ? 0 : f.kend - f.skip <= UNIT ? 1 : (f.kend - f.skip + UNIT - 1) / UNIT;
     return f;
 }
 
 // What becomes of four values of a row's sum, v, behind its last part: here they are divided and stored
 template <typename T, int D, int ROWS> struct FewOut {
+    static constexpr bool SKIPS = false;
     const FewArgs &a;
     __device__ __forceinline__ void put(const FewSequence &f, int, int hr, int r, int d, f32x4 v, float, float sum) const {
         const int rb = hr % a.row_blocks, kvh = hr / a.row_blocks, rr = rb * ROWS + r, token = rr / a.group, hg = rr - token * a.group;
@@ -453,8 +456,8 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
     constexpr int ROWS = 16 * NT, UNIT = few_unit<E8>();
     const int lane = threadIdx.x & 63, hr = t.y, rb = hr % a.row_blocks, batch = p.batch;
     if (a.shares == 0) {  // a tile per sequence
-        const FewSequence f = few_sequence<ROWS, UNIT>(a, seq_tokens(p.start, p.kv_len, t.x, p.tokens, p.max_new), rb);
-        if (f.nrows > 0) attend_stretch<T, D, E8, NT>(a, f, t.x, hr, a.skip, f.kend, nullptr, 0, 0, lds, out);
+        const FewSequence f = few_sequence<ROWS, UNIT, Out::SKIPS>(a, seq_tokens(p.start, p.kv_len, t.x, p.tokens, p.max_new), rb);
+        if (f.nrows > 0) attend_stretch<T, D, E8, NT>(a, f, t.x, hr, f.skip, f.kend, nullptr, 0, 0, lds, out);
         return;
     }
     // ---- all units; then the sequence in which this part begins.  Every wavefront for itself, 64 sequences at a time, one to a lane ----
@@ -464,7 +467,7 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
         r0 = p.start ? p.start[b] : b;
         r1 = p.start ? p.start[b + 1] : b + 1;
         len = p.kv_len[b];
-        return b0 + lane < batch ? few_sequence<ROWS, UNIT>(a, seq_tokens_of(r0, r1, len, p.tokens, p.max_new), rb).units : 0;
+        return b0 + lane < batch ? few_sequence<ROWS, UNIT, Out::SKIPS>(a, seq_tokens_of(r0, r1, len, p.tokens, p.max_new), rb).units : 0;
     };
     int total = 0, n = 0;
     for (int b0 = batch <= 64 ? 0 : (batch - 1) / 64 * 64; b0 >= 0; b0 -= 64) total += n = look(b0);  // (the first 64 last: they are looked at next)
@@ -492,10 +495,10 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
         at += behind ? __builtin_amdgcn_readlane(upto - n, i) : __builtin_amdgcn_readlane(upto, 63);
         return behind != 0;
     }, look, [&](int b, int i, int at) {
-        const FewSequence f = few_sequence<ROWS, UNIT>(a, seq_tokens_of(__builtin_amdgcn_readlane(r0, i), __builtin_amdgcn_readlane(r1, i), __builtin_amdgcn_readlane(len, i), p.tokens, p.max_new), rb);
+        const FewSequence f = few_sequence<ROWS, UNIT, Out::SKIPS>(a, seq_tokens_of(__builtin_amdgcn_readlane(r0, i), __builtin_amdgcn_readlane(r1, i), __builtin_amdgcn_readlane(len, i), p.tokens, p.max_new), rb);
         if (f.units == 0) return 0;
         const int u0 = lo > at ? lo - at : 0, u1 = hi - at < f.units ? hi - at : f.units;
-        attend_stretch<T, D, E8, NT>(a, f, b, hr, a.skip + u0 * UNIT, u1 == f.units ? f.kend : a.skip + u1 * UNIT, slots + (u0 == 0) * few_partial_floats<NT, D>(),
+        attend_stretch<T, D, E8, NT>(a, f, b, hr, f.skip + u0 * UNIT, u1 == f.units ? f.kend : f.skip + u1 * UNIT, slots + (u0 == 0) * few_partial_floats<NT, D>(),
                                      part_of(at, total, shares), part_of(at + f.units - 1l, total, shares), lds, out);
         return f.units;
     });

@@ -2,7 +2,8 @@
 //
 // What they share is read once for the rows of all sequences: a tile takes a head of the cache, the rows of as many whole sequences as 128 rows hold, and one of `shares` parts of the shared
 // keys (many_keys in paged_many.hpp).  What a sequence has of its own is attended to as in a step without anything shared (attend_few in paged_few.hpp, behind the first shared_len
-// keys).  Both are tiles of one launch, the shared ones first, and leave a reference, a sum and a weighted sum per row.  The parts of the shared keys are joined two by two, and whoever comes second to a
+// keys).  A sequence with a row that does not see all of the shared keys attends to everything for itself: behind what it sees may lie NaN, and a probability of 0 times that is no 0.
+// Both are tiles of one launch, the shared ones first, and leave a reference, a sum and a weighted sum per row.  The parts of the shared keys are joined two by two, and whoever comes second to a
 // sequence's rows, with what its own or what the shared keys come to, joins both; in one order whoever that is.
 //
 // Measured (32 heads of queries over 8 of 128; each sequence for itself in brackets): 64 sequences behind 8192 tokens, up to 2048 of their own, e4m3: 62 us (152) for 169 MB; 5 with 4 new tokens behind 131072, bf16:
@@ -69,7 +70,7 @@ __device__ __forceinline__ void join_prefix(const PrefixArgs &a, int block, int 
         place[u] = at;
         const float top = fmaxf(x[0], y[0]), base = top == -INFINITY ? 0.f : top;
         const float f = __builtin_amdgcn_exp2f(x[0] - base), g = __builtin_amdgcn_exp2f(y[0] - base), sum = fmaf(g, y[1], f * x[1]), inv = sum == 0.f ? 0.f : 1.f / sum;
-        factors[u] = f32x2{f * inv, g * inv};
+        factors[u] = f32x2{f * inv, y[1] == 0.f ? -1.f : g * inv};  // (-1: none of the shared keys counts, and their sum may be NaN)
     }
     __syncthreads();
     const auto own_buffer = shared_buffer(own), shared_result = shared_buffer(shared);
@@ -91,7 +92,7 @@ __device__ __forceinline__ void join_prefix(const PrefixArgs &a, int block, int 
             typedef T tx4 __attribute__((ext_vector_type(4)));
             tx4 out;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) out[e] = Elem<T>::from_f(rounded(fmaf(f[1], y[k][e], f[0] * x[k][e])));
+            for (int e = 0; e < 4; ++e) out[e] = Elem<T>::from_f(rounded(f[1] < 0.f ? f[0] * x[k][e] : fmaf(f[1], y[k][e], f[0] * x[k][e])));
             *(tx4 *)((T *)p.out + place[r] + d) = out;
         }
     }
@@ -99,6 +100,7 @@ __device__ __forceinline__ void join_prefix(const PrefixArgs &a, int block, int 
 
 // a sequence's own keys: the result waits for those of the shared keys, or joins them
 template <typename T, int D, int NT> struct PrefixOut {
+    static constexpr bool SKIPS = true;
     const PrefixArgs &a;
     float *lds;
     __device__ __forceinline__ void put(const FewSequence &, int b, int hr, int r, int d, f32x4 v, float top, float sum) const {
@@ -131,9 +133,9 @@ __device__ __forceinline__ void attend_shared(const PrefixArgs &a, int at, char 
     const int r = wave * 32 + l32, b = block * a.per_block + r / a.rows, in = r % a.rows, token = in / a.few.group, hg = in - token * a.few.group;
     bool there = r < a.per_block * a.rows && b < p.batch;
     const SeqTokens s = seq_tokens(p.start, p.kv_len, there ? b : 0, p.tokens, p.max_new);
-    there = there && token < s.rows;
-    int seen = there ? (int)keys_seen(seq_bound(s, p.max_len, p.table_width, p.cache.page_size), s.first + token, p.causal) : 0;
-    if (seen > a.shared_len) seen = a.shared_len;
+    // (all shared keys or none: few_sequence)
+    there = there && token < s.rows && keys_seen(seq_bound(s, p.max_len, p.table_width, p.cache.page_size), s.first, p.causal) >= a.shared_len;
+    const int seen = there ? a.shared_len : 0;
     const T *q = (const T *)p.q + (there ? s.row0 + token : 0) * p.ld_q + ((long)kvh * a.few.group + (there ? hg : 0)) * D;
     const int tiles = (a.shared_len + MANY_KEYS - 1) / MANY_KEYS;
     f32x16 o[DB];
@@ -141,6 +143,7 @@ __device__ __forceinline__ void attend_shared(const PrefixArgs &a, int at, char 
     many_keys<T, D, E8>(PagedKeys{p.cache, a.table, a.shared_len / p.cache.page_size, 0, kvh}, ManyRow{there, seen, q}, p.scale, a.shared_len, a.shared_len,
                         part_begin(share, tiles, a.shares), part_begin(share + 1, tiles, a.shares), lds, o, m, l);
     l += __shfl_xor(l, 32, 64);
+    if (!there) { m = -INFINITY; l = 0.f; }  // (what has come together here is of no row)
     // ---- the parts' results meet two by two: whoever of a pair comes second goes on with both, in their order ----
     const long unit = (long)block * p.cache.kv_heads + kvh;
     float *slots = a.shared + unit * a.shares * many_partial_floats<D>();

@@ -634,7 +634,7 @@ int gp_launch_paged_attention(const gp_paged_attention_params *p, const gp_preem
 /* The same for sequences that all begin with the same shared_len tokens (a system prompt, a document), which lie in the same pages: whole pages, whose numbers
  * shared_table (device memory, shared_len / page_size of them) has, and with which every sequence's row of the page table begins (either is read).  kv_len, positions and
  * max_len count them.  They are read once for all sequences' rows together, not once for each.  A sequence that is shorter than
- * shared_len sees its first kv_len tokens of them.  Results are those of gp_launch_paged_attention but for the order in which they are added up; all
+ * shared_len, or has new tokens among them, sees those of them that gp_launch_paged_attention would show it, and is not among those that read them together.  Results are those of gp_launch_paged_attention but for the order in which they are added up; all
  * that is said there holds.  shared_len 0: nothing is shared.
  * attention.work: gp_prefix_attention_work_bytes(), of a kind of its own: zeroed before its first use, serves these launches of any sizes one after the other, and no
  * other operator's. */

@@ -310,6 +310,39 @@ def test_shared_pages_with_scales_far_apart(gp, batch):
     a.check()
 
 
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+@pytest.mark.parametrize("case", [([100, 37, 1], None), ([90, 100, 60], [7, 1, 3]), ([2, 0, 33] * 30, None)])
+def test_sequences_that_end_in_front_of_what_nobody_has_written_yet(gp, cache, case):
+    """the shared pages' last slots are no sequence's, and hold NaN"""
+    for causal in (True, False):
+        a = Prefix(gp, "f16", cache, begin_alike(S.Sequences(*case, 64, gen(31), width=3), 128), 8, 2, 64, causal, 32)
+        a.launch()
+        a.check()
+
+
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+def test_what_is_not_finite_reaches_only_who_sees_it(gp, cache):
+    """NaN among the shared keys and values from token 300 on; who has 300 tokens or fewer, or 300 at his new one, is as if it were not there"""
+    seqs = begin_alike(S.Sequences([2000, 300, 299, 1950, 17, 0, 305, 310], [1, 1, 4, 2, 3, 0, 1, 11], 64, gen(33), width=32), 1920)
+    for causal in (True, False):
+        a = Prefix(gp, "f16", cache, seqs, 8, 2, 128, causal, 34)
+        a.launch()
+        finite = a.left()
+        for pos in range(300, 1920):
+            page, slot = seqs.place(0, pos)
+            for name in ("k", "v"):
+                a.dev[name].view(torch.uint8 if cache == "e4m3" else torch.int16)[page, :, slot] = 0x7F if cache == "e4m3" else 0x7FFF
+        a.clean()
+        a.launch()
+        got = a.left()
+        for b in range(seqs.batch):
+            for row, pos in seqs.rows(b):
+                if seqs.lens[b] <= 300:
+                    assert torch.equal(got[row], finite[row]), (b, pos)
+                elif (pos if causal else seqs.lens[b] - 1) >= 300:
+                    assert got[row].isnan().all(), (b, pos)
+
+
 def test_bounds_on_what_is_new_are_only_bounds(gp):
     """sequences with fewer new tokens than max_new, none among them, rows behind the last"""
     for news in ([1, 2, 0], [0, 0, 0]):
