@@ -34,6 +34,11 @@ template <int MT, int NT, int WAVES> inline size_t w4_lds_bytes(int panel) {
     return std::max((size_t)16 * NT * w4_scale_stride(panel) * sizeof(unsigned), (size_t)WAVES * 256 * MT * NT * sizeof(float));
 }
 
+// What is not finite must not come out as a number: apply_act's ReLU takes NaN to 0, and an infinite scale times a group's negative sum to 0 too, where scale * (q - zero) in front of the sum has both
+// signs.  So NaN stays NaN, and an infinite scale is one.
+template <typename T> __device__ __forceinline__ T finite_or_nan(T scale) { return Elem<T>::from_f(fmaf(Elem<T>::to_f(scale), 0.f, Elem<T>::to_f(scale))); }
+__device__ __forceinline__ float act_of_sum(float v, int act) { return act == GP_ACT_RELU ? (v <= 0.f ? 0.f : v) : apply_act(v, act); }
+
 // rows r0 .. r3 of a 4 x 4 matrix of (registers, groups of 16 lanes) become its columns
 __device__ __forceinline__ void transpose_lane_groups(u32x4 &r) {
     auto swap32 = [](unsigned &x, unsigned &y) { const auto s = __builtin_amdgcn_permlane32_swap(x, y, false, false); x = s[0]; y = s[1]; };
@@ -134,7 +139,7 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const T minus = Elem<T>::from_f((float)z[e] * -0x1p-9f);  // (exact: a whole number of eight bits)
-                if (at + e < gn) scales[r * stride + at + e] = __builtin_bit_cast(unsigned, tx2{s[e], minus});
+                if (at + e < gn) scales[r * stride + at + e] = __builtin_bit_cast(unsigned, tx2{finite_or_nan((T)s[e]), minus});
             }
         }
         __syncthreads();
@@ -203,7 +208,7 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
         const long at = m * p.ldc + n;
         if (p.bias) v += Elem<T>::to_f(((const T *)p.bias)[n]);
         if (p.residual) v += Elem<T>::to_f(((const T *)p.residual)[at]);
-        ((T *)p.C)[at] = Elem<T>::from_f(rounded(apply_act(v, p.act)));
+        ((T *)p.C)[at] = Elem<T>::from_f(rounded(act_of_sum(v, p.act)));
     }
 }
 
@@ -313,7 +318,7 @@ __device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int ti
             if (!WHOLE || t == 0) {
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
-                    s[i] = Elem<T>::to_f(sc[WHOLE ? 1 : t][i]);
+                    s[i] = Elem<T>::to_f(finite_or_nan(sc[WHOLE ? 1 : t][i]));
                     minus[i] = -s[i] * (p.zeros ? (float)ze[WHOLE ? 1 : t][i] : 8.f);
                 }
             }
@@ -350,7 +355,7 @@ __device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int ti
                 float y = acc[i][j][v];
                 if (p.bias) y += bias;
                 if (p.residual) y += Elem<T>::to_f(((const T *)p.residual)[at]);
-                ((T *)p.C)[at] = Elem<T>::from_f(rounded(apply_act(y, p.act)));
+                ((T *)p.C)[at] = Elem<T>::from_f(rounded(act_of_sum(y, p.act)));
             }
     }
 }

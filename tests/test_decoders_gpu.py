@@ -695,3 +695,34 @@ def test_users_behind_one_prompt(gp, cache):
         stream.sync()
         lp.check()
     stream.destroy()
+
+
+# ---- 4-bit weights: what is not finite, and one precision for all sizes ---------------------------------------------------------
+
+
+EVERY_SIZE = [(3, 150, 512, 64), (40, 150, 512, 64), (200, 150, 512, 64), (1200, 1301, 512, 64), (1200, 1301, 512, 128), (1200, 1301, 544, 32), (65, 11009, 96, 32), (2945, 3001, 192, 64)]
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("m, n, k, group", EVERY_SIZE)
+def test_what_is_not_finite_stays_so_behind_every_activation(gp, dt, act, m, n, k, group):
+    """NaN and infinities in rows of A, among the scales, in bias and residual: a sum that is NaN comes out as NaN, one that is infinite as infinite or NaN (ReLU and GELU take minus infinity to 0)"""
+    def change(w):
+        w.a[0, 3] = math.nan
+        w.a[1, 5], w.a[2, 5] = math.inf, -math.inf
+        w.scales[7, 1], w.scales[8, 0] = math.nan, math.inf
+        w.bias[9], w.bias[10], w.bias[11] = math.nan, math.inf, -math.inf
+        w.residual[m - 1, 12], w.residual[m - 1, 13], w.residual[m - 1, 14] = math.nan, math.inf, -math.inf
+    w = W4(gp, dt, m, n, k, group, 71, act=act, change=change)
+    w.launch()
+    got = w.left()[:, :n]
+    w.act = "none"
+    total, _ = w.definition()
+    plain = torch.isfinite(total)
+    assert torch.isfinite(got[plain]).all()
+    assert got[total.isnan()].isnan().all() and got[:, 8].isnan().all()
+    up, down = got[total == math.inf], got[total == -math.inf]
+    assert (up.isnan() | (up == math.inf)).all()
+    assert (down.isnan() | (down == (-math.inf if act == "none" else 0.0)) | ((down == -math.inf) if act == "gelu" else False)).all()
+    assert (total == math.inf).any() and (total == -math.inf).any() and total.isnan().any()
