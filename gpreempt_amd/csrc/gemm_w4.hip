@@ -27,7 +27,6 @@ struct W4Args {
     int groups;  // of a row
     int panel;   // of them, at a time
     int rows, cols;  // tiles (many rows)
-    int log2_group;
 };
 inline __host__ __device__ int w4_scale_stride(int panel) { return panel + 1; }
 template <int MT, int NT, int WAVES> inline size_t w4_lds_bytes(int panel) {
@@ -219,60 +218,64 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : MT * NT > 2 ? 2 : 4) 
 }
 
 // ---- many rows ----
-// Bound by the matrix instructions, and by the vector instructions that make 16-bit numbers of W's: two and a half for each of them, which 128 rows of A share.  A tile is 128 rows of A and
-// 256 or 128 of W, a quarter to a wavefront, which has what it takes of W in registers; A comes through LDS, 128 values of a row at a time in two buffers.
-//   v_mfma_f32_32x32x16   A as A, W as B: lane l has 8 values of row l % 32; of 64 values the lanes below 32 take the first half, the others the second (16 bytes of W).
-// W's numbers are multiplied by their scale and rounded to the type in front of the products (the few rows' way, exact integers and a sum for each group, takes twice the registers and a vector instruction
-// for each result and group: there would be more of those than the matrix instructions hide).  So a result is off by half a unit of |A| |W| beside its own rounding, as if W had been kept in 16 bits.
-// Measured: 4001 x 8192 x 8192, bf16, groups of 128: 553 to 581 us on different days, 925 to 970 TFLOP/s (a large matrix product of 16 bits: 1150); the matrix instructions take 50 % of the cycles.
-constexpr int W4M_NT = 256, W4M_ROWS = 128, W4M_STEP = 128;
+// Bound by the vector instructions that make 16-bit numbers of W's (23 for eight numbers in bf16, 13 in fp16, which 128 rows of A share) and scale the groups' sums (16 for 32 x 32 results and a group),
+// and by the matrix instructions, which seldom overlap with them.  A tile is 128 rows of A and 128 of W, a quarter of these to a wavefront, which has what it takes of W in registers; A comes through
+// LDS, 128 values of a row at a time in two buffers.
+//   v_mfma_f32_32x32x16   A as A, W as B: lane l has 8 values of row l % 32.
+// The products are of A with q - z, whole numbers of eight bits and exact; a group's sum meets its scale in fp32: nothing is rounded to 16 bits but the result, as for few rows.
+// Measured (rounding scale * (q - z) to 16 bits in front of the products in brackets): 4001 x 8192 x 8192, bf16, groups of 128: 663 to 706 us, 760 to 810 TFLOP/s (571); fp16 633 (568); of 64 736 (614); of 32 885 to 901 (622);
+// 2048 x 4096 x 4096 82 to 92 (88 to 92), 128 x 22528 x 4096 58 (68).  Tiles of 256 x 256 in eight wavefronts, one to a compute unit: 645, of 64 642, of 32 797, 2048 x 4096 x 4096 174.  Widening W a step
+// ahead between the matrix instructions: 687.
+constexpr int W4M_ROWS = 128, W4M_NT = 256, W4M_STEP = 128;
 constexpr int W4M_BUFFER = W4M_ROWS * W4M_STEP * 2;  // bytes
 constexpr int W4M_BAND = 8;  // rows of tiles that are worked on side by side
 
-// eight 4-bit numbers as scale * (number - zero); minus = -scale * zero
-template <typename T> __device__ __forceinline__ u32x4 dequantise(unsigned raw, float scale, float minus) {
+// eight 4-bit numbers minus `zero`, in their order: whole numbers of eight bits, exact in either type
+__device__ __forceinline__ u32x4 less_zero(unsigned raw, float zero, __bf16) {
     unsigned even = raw & 0x0F0F0F0Fu, odd = (raw >> 4) & 0x0F0F0F0Fu;
-    asm("" : "+v"(even), "+v"(odd));  // (a byte to fp32 is one instruction; the compiler goes back to `raw`, and shifts and masks for each of them: 688 vector instructions a step for 400)
-    typedef T tx2 __attribute__((ext_vector_type(2)));
+    asm("" : "+v"(even), "+v"(odd));  // (a byte to fp32 is one instruction; the compiler goes back to `raw`, and shifts and masks for each of them)
+    typedef __bf16 tx2 __attribute__((ext_vector_type(2)));
     u32x4 y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const f32x2 x = {fmaf((float)(even >> (8 * i) & 255u), scale, minus), fmaf((float)(odd >> (8 * i) & 255u), scale, minus)};
+        const f32x2 x = {(float)(even >> (8 * i) & 255u) - zero, (float)(odd >> (8 * i) & 255u) - zero};
         y[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, tx2));
     }
     return y;
 }
+__device__ __forceinline__ u32x4 less_zero(unsigned raw, float zero, _Float16) {
+    const unsigned even = raw & 0x0F0F0F0Fu, odd = (raw >> 4) & 0x0F0F0F0Fu;
+    const unsigned x = __builtin_amdgcn_perm(odd, even, 0x05010400u), y = __builtin_amdgcn_perm(odd, even, 0x07030602u);
+    const _Float16 z = (_Float16)(1024.f + zero);
+    const f16x2 zz = {z, z};
+    // (the bits 0x6400 + n are 1024 + n)
+    auto pair = [&](unsigned bytes, unsigned pick) { return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, bytes, pick)) - zz); };
+    return u32x4{pair(x, 0x04010400u), pair(x, 0x04030402u), pair(y, 0x04010400u), pair(y, 0x04030402u)};
+}
 
-template <typename T, bool WHOLE, int NB>
+template <typename T, int G>
 __device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int tile_n, char *lds) {
 #pragma clang fp contract(off)
     const gp_gemm_w4_params &p = a.p;
-    constexpr int MB = W4M_ROWS / 32;
+    constexpr bool WHOLE = G == W4M_STEP;  // (K is a multiple of a step)
+    constexpr int MB = W4M_ROWS / 32, GROUPS = W4M_STEP / G, SLICES = G / 16;  // of a step; instructions of a group
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
-    const int m0 = tile_m * W4M_ROWS, n0 = (tile_n * 4 + wave) * 32 * NB;
-    const unsigned char *w[NB], *zero[NB];
-    const T *scale[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        const int n = n0 + 32 * i + l32 < p.N ? n0 + 32 * i + l32 : p.N - 1;
-        w[i] = (const unsigned char *)p.W + (long)n * p.ldw;
-        scale[i] = (const T *)p.scales + (long)n * p.ld_scales;
-        zero[i] = p.zeros ? p.zeros + (long)n * p.ld_zeros : w[i];  // (where there are none, something is fetched all the same and left: no branch in the loop)
-    }
-    f32x16 acc[MB][NB];
+    const int m0 = tile_m * W4M_ROWS, n = (tile_n * 4 + wave) * 32 + l32, row_of_w = n < p.N ? n : p.N - 1;
+    const unsigned char *w = (const unsigned char *)p.W + (long)row_of_w * p.ldw;
+    const T *scale = (const T *)p.scales + (long)row_of_w * p.ld_scales;
+    const unsigned char *zero = p.zeros ? p.zeros + (long)row_of_w * p.ld_zeros : w;  // (where there are none, something is fetched all the same and left: no branch in the loop)
+    f32x16 total[MB];
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+        for (int v = 0; v < 16; ++v) total[i][v] = 0.f;
     const int steps = (p.K + W4M_STEP - 1) / W4M_STEP;
     // ---- A: thread (row tid / 16 + 16 i, 16 bytes tid % 16) ----
     const int chunk = tid % 16, row = tid / 16;
     const int slot = row * 256 + ((chunk ^ row) & 15) * 16;
     const T *x0 = (const T *)p.A + chunk * 8;
     u32x4 ar[8];
-    auto load_a = [&](int step) {
+    auto load_a = [&](int step) {  // (what is behind the rows' end is not multiplied: the row's first values instead)
         const int k = step * W4M_STEP + chunk * 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -280,102 +283,104 @@ __device__ __forceinline__ void w4_many_tile(const W4Args &a, int tile_m, int ti
             ar[i] = *(const u32x4 *)(x0 + (long)(m < p.M ? m : p.M - 1) * p.lda + (WHOLE || k < p.K ? step * W4M_STEP : -chunk * 8));
         }
     };
-    auto store_a = [&](int step, char *buf) {
-        const bool there = WHOLE || step * W4M_STEP + chunk * 8 < p.K;  // (what is behind the rows' end counts as zeros)
+    auto store_a = [&](char *buf) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) *(u32x4 *)(buf + slot + i * 16 * 256) = there ? ar[i] : u32x4{0, 0, 0, 0};
+        for (int i = 0; i < 8; ++i) *(u32x4 *)(buf + slot + i * 16 * 256) = ar[i];
     };
-    // ---- W: of 64 values the lane's 32, and their scale and zero ----
-    u32x4 raw[2][NB];
-    T sc[2][NB];
-    unsigned char ze[2][NB];
-    auto load_w = [&](int step, int t) {
-        int k = step * W4M_STEP + 64 * t + 32 * half;
-        if (!WHOLE && k >= p.K) k = 0;
-        const int g = k >> a.log2_group;
+    // ---- W: of 64 values the lane's 32; the step's scales and zeros ----
+    u32x4 raw[2];
+    T sc[GROUPS];
+    unsigned char ze[GROUPS];
+    auto load_w = [&](int step) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            raw[t][i] = *(const u32x4 *)(w[i] + k / 2);
-            if (!WHOLE || t == 1) {
-                sc[t][i] = scale[i][g];
-                ze[t][i] = zero[i][g];
-            }
+        for (int t = 0; t < 2; ++t) {
+            const int k = step * W4M_STEP + 64 * t + 32 * half;
+            raw[t] = *(const u32x4 *)(w + (WHOLE || k < p.K ? k / 2 : 0));
+        }
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const int at = step * GROUPS + g < a.groups ? step * GROUPS + g : 0;
+            sc[g] = scale[at];
+            ze[g] = zero[at];
         }
     };
     load_a(0);
-    load_w(0, 0);
-    load_w(0, 1);
+    load_w(0);
     __syncthreads();  // (the previous tile's buffers are still being read)
-    store_a(0, lds);
+    store_a(lds);
     __syncthreads();
     for (int step = 0; step < steps; ++step) {
         const char *buf = lds + step % 2 * W4M_BUFFER;
         const int next = step + 1 < steps ? step + 1 : step;  // (behind the last step: the last one again, which nobody reads)
         load_a(next);
-        float s[NB], minus[NB];  // (groups of 128: those of the whole step, else of the lane's 32 values)
+        float s[GROUPS], z[GROUPS];
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            s[g] = Elem<T>::to_f(finite_or_nan(sc[g]));
+            z[g] = p.zeros ? (float)ze[g] : 8.f;
+        }
+        // (the halves of a wavefront exchange what they have, so that an instruction takes 16 neighbours: within a group)
+        unsigned mine[2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            if (!WHOLE || t == 0) {
-#pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    s[i] = Elem<T>::to_f(finite_or_nan(sc[WHOLE ? 1 : t][i]));
-                    minus[i] = -s[i] * (p.zeros ? (float)ze[WHOLE ? 1 : t][i] : 8.f);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4 b[NB];
-#pragma unroll
-                for (int i = 0; i < NB; ++i) b[i] = dequantise<T>(raw[t][i][j], s[i], minus[i]);
-#pragma unroll
-                for (int i = 0; i < MB; ++i) {
-                    const u32x4 x = *(const u32x4 *)(buf + (32 * i + l32) * 256 + (((8 * t + 4 * half + j) ^ l32) & 15) * 16);
-#pragma unroll
-                    for (int k = 0; k < NB; ++k) Elem<T>::mma(x, b[k], acc[i][k]);
-                }
-            }
-            load_w(next, t);
+            const auto x = __builtin_amdgcn_permlane32_swap(raw[t][0], raw[t][1], false, false), y = __builtin_amdgcn_permlane32_swap(raw[t][2], raw[t][3], false, false);
+            mine[t][0] = x[0]; mine[t][1] = y[0]; mine[t][2] = x[1]; mine[t][3] = y[1];
         }
-        store_a(next, lds + (step + 1) % 2 * W4M_BUFFER);
+        load_w(next);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            if (!WHOLE && step * GROUPS + g >= a.groups) break;
+            u32x4 b[SLICES];
+#pragma unroll
+            for (int j = 0; j < SLICES; ++j) b[j] = less_zero(mine[(g * SLICES + j) / 4][(g * SLICES + j) % 4], z[g], T());
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+                f32x16 acc;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+#pragma unroll
+                for (int j = 0; j < SLICES; ++j)
+                    Elem<T>::mma(*(const u32x4 *)(buf + (32 * i + l32) * 256 + (((2 * (g * SLICES + j) + half) ^ l32) & 15) * 16), b[j], acc);
+#pragma unroll
+                for (int v = 0; v < 16; ++v) total[i][v] = fmaf(s[g], acc[v], total[i][v]);
+            }
+        }
+        store_a(lds + (step + 1) % 2 * W4M_BUFFER);
         __syncthreads();
     }
-    // ---- acc[i][j][v]: row 32 i + 8 (v / 4) + 4 half + v % 4 of the tile, row 32 j + l32 of the wavefront's of W ----
+    // ---- total[i][v]: row 32 i + 8 (v / 4) + 4 half + v % 4 of the tile, the lane's row of W ----
+    if (n >= p.N) return;
+    const float bias = p.bias ? Elem<T>::to_f(((const T *)p.bias)[n]) : 0.f;
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        const int n = n0 + 32 * j + l32;
-        if (n >= p.N) continue;
-        const float bias = p.bias ? Elem<T>::to_f(((const T *)p.bias)[n]) : 0.f;
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int m = m0 + 32 * i + 8 * (v / 4) + 4 * half + v % 4;
-                if (m >= p.M) continue;
-                const long at = m * p.ldc + n;
-                float y = acc[i][j][v];
-                if (p.bias) y += bias;
-                if (p.residual) y += Elem<T>::to_f(((const T *)p.residual)[at]);
-                ((T *)p.C)[at] = Elem<T>::from_f(rounded(act_of_sum(y, p.act)));
-            }
-    }
+        for (int v = 0; v < 16; ++v) {
+            const int m = m0 + 32 * i + 8 * (v / 4) + 4 * half + v % 4;
+            if (m >= p.M) continue;
+            const long at = m * p.ldc + n;
+            float y = total[i][v];
+            if (p.bias) y += bias;
+            if (p.residual) y += Elem<T>::to_f(((const T *)p.residual)[at]);
+            ((T *)p.C)[at] = Elem<T>::from_f(rounded(act_of_sum(y, p.act)));
+        }
 }
 
-template <typename T, bool WHOLE, int NB, int LOOP = LOOP_ANY>
+template <typename T, int G, int LOOP = LOOP_ANY>
 __global__ __launch_bounds__(W4M_NT, 2) void gemm_w4_many_kernel(W4Args a, BlpArgs blp) {
     extern __shared__ __attribute__((aligned(16))) unsigned char w4_lds[];
     tiles<LOOP>(blp, [&](TileIdx t) {
         // (bands of tiles: neighbours share rows of A and of W)
         const int band = t.x / (W4M_BAND * a.cols), in = t.x - band * W4M_BAND * a.cols, high = a.rows - band * W4M_BAND < W4M_BAND ? a.rows - band * W4M_BAND : W4M_BAND;
-        w4_many_tile<T, WHOLE, NB>(a, band * W4M_BAND + in % high, in / high, (char *)w4_lds);
+        w4_many_tile<T, G>(a, band * W4M_BAND + in % high, in / high, (char *)w4_lds);
     });
 }
 
-template <typename T, bool WHOLE, int NB>
+template <typename T, int G>
 static int launch_w4_many(W4Args a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
     a.rows = (int)(((long)a.p.M + W4M_ROWS - 1) / W4M_ROWS);
-    a.cols = (int)(((long)a.p.N + 128 * NB - 1) / (128 * NB));
+    a.cols = (int)(((long)a.p.N + 127) / 128);
     GP_REQUIRE((long)a.rows * a.cols < (1L << 31) && (long)a.cols * W4M_BAND < (1L << 31), "gemm_w4: too large");
-    return launch_tiles(GP_KSET(gemm_w4_many_kernel<T, WHOLE, NB), a.rows * a.cols, 1, ctx, s, info, a, 2 * W4M_BUFFER, 1, W4M_NT);
+    return launch_tiles(GP_KSET(gemm_w4_many_kernel<T, G), a.rows * a.cols, 1, ctx, s, info, a, 2 * W4M_BUFFER, 1, W4M_NT);
 }
 
 template <typename T, int G, int MT, int NT, int WAVES>
@@ -387,12 +392,11 @@ static int launch_w4(const W4Args &a, const gp_preempt_ctx *ctx, gp_stream s, gp
 
 template <typename T, int G>
 static int choose_w4(const W4Args &a, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info) {
-    // Many rows' tiles of 128 x 128 or 128 x 256, or few rows at a time.  Us, few / 128 x 128 / 128 x 256, bf16, K = 4096 (768 where N is 2304), groups of 128: 128 x 4096 24 / 55 / 86,
-    // 256 x 4096 48 / 56 / 86, 512 x 4096 96 / 68 / 97, 1024 x 1024 43 / 67 / 95, 300 x 2304 14.5 / 17.4 / 29, 600 x 2304 20.9 / 17.9 / 29, 64 x 22528 65 / 70 / 94, 128 x 22528 130 / 69 / 95,
-    // 2048 x 4096 355 / 90 / 106, 512 x 22528 469 / 145 / 133.
-    const long tiles = ((long)a.p.M + W4M_ROWS - 1) / W4M_ROWS * (((long)a.p.N + 127) / 128);
-    if (a.p.M > 64 && 3 * tiles >= device_cus())
-        return tiles > 2 * device_cus() ? launch_w4_many<T, G == W4M_STEP, 2>(a, ctx, s, info) : launch_w4_many<T, G == W4M_STEP, 1>(a, ctx, s, info);
+    // Many rows' tiles of 128 x 128, or few rows at a time, in tiles of up to 64 x 16: the first takes 50 (groups of 128), 60 (64), 90 us (32) for K = 4096 as long as the chip is not full, the second goes by how
+    // many there are.  Us, many / few, bf16 (fp16 within 5 %), K = 4096, tiles of 64 x 16 in brackets: groups of 128: 128 x 4096 (512) 51 / 38, 400 x 1400 (616) 52 / 53, 600 x 1000 (630) 57 / 53, 65 x 6700
+    // (838) 49 / 71, 256 x 4096 (1024) 51 / 72, 72 x 22528 (2816) 56 / 103; of 64: 616 61 / 54, 838 60 / 74, 1024 61 / 75; of 32: 838 88 / 72, 1024 89 / 72, 128 x 9200 (1150) 92 / 90, 128 x 11000 (1376) 97 / 108.
+    const long tiles = ((long)a.p.M + 63) / 64 * (((long)a.p.N + 15) / 16);
+    if (a.p.M > 64 && 4 * tiles >= (G == 128 ? 10l : G == 64 ? 12l : 18l) * device_cus()) return launch_w4_many<T, G>(a, ctx, s, info);
     // Rows of W for each wavefront, and wavefronts: what is fetched of A counts as much as W does, so a wavefront takes several rows' sixteens at once where there are enough of them for all compute
     // units.  Us (K = 4096, groups of 128, bf16) in tiles of 16 rows for 8 wavefronts / 32 for 4 / 64 for 4: 1 x 4096 6.0 / 8.2 / 10.6, 1 x 22528 19 / 16.2 / 17.0, 5 x 131001 104 / 87 / 68,
     // 24 x 4096 10.6 / 12 / 15, 24 x 22528 48 / 35 / 27, 24 x 131001 246 / 178 / 107, 64 x 4096 19 / 24, 64 x 22528 106 / 57.
@@ -423,7 +427,7 @@ extern "C" int gp_launch_gemm_w4(const gp_gemm_w4_params *p, const gp_preempt_ct
     GP_REQUIRE(aligned16(p->A) && aligned16(p->W), "gemm_w4: A and W must be 16-byte aligned");
     GP_REQUIRE(((uintptr_t)p->C | (uintptr_t)p->scales | (uintptr_t)p->bias | (uintptr_t)p->residual) % 2 == 0, "gemm_w4: C, scales, bias and residual must be aligned to their elements");
     GP_REQUIRE(p->act == GP_ACT_NONE || p->act == GP_ACT_RELU || p->act == GP_ACT_GELU, "gemm_w4: act %d", p->act);
-    const W4Args a{*p, groups, std::min(groups, W4_PANEL), 0, 0, p->group == 32 ? 5 : p->group == 64 ? 6 : 7};
+    const W4Args a{*p, groups, std::min(groups, W4_PANEL), 0, 0};
     switch (p->group * 2 + (p->dtype == GP_F16)) {
 #define GP_W4(T, F16, G) case G * 2 + F16: return choose_w4<T, G>(a, ctx, s, info);
         GP_W4(_Float16, 1, 32) GP_W4(__bf16, 0, 32) GP_W4(_Float16, 1, 64) GP_W4(__bf16, 0, 64) GP_W4(_Float16, 1, 128) GP_W4(__bf16, 0, 128)

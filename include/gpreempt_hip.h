@@ -676,8 +676,8 @@ int gp_launch_packed_attention(const gp_packed_attention_params *p, const gp_pre
  *   group    32, 64 or 128; K is a multiple of it
  *   A        M rows of K values (lda a multiple of 8, A 16-byte aligned)
  *   C, residual   M rows of N values, ldc from row to row; bias N values.  bias, residual may be NULL; residual may be C
- * GP_F16 or GP_BF16; M, N and K at most 2^30; sums in fp32 (A's values times up to 255 have to fit).  Up to 64 rows of A nothing but the result is rounded to 16 bits; for more, W may be rounded to the type in
- * front of the products, as if it had been kept in 16 bits.  A NaN in a row of A, in bias or residual, and a scale that is not finite, make
+ * GP_F16 or GP_BF16; M, N and K at most 2^30; sums in fp32 (A's values times up to 255 have to fit).  Nothing but the result is rounded to 16 bits, whatever the sizes.
+ * A NaN in a row of A, in bias or residual, and a scale that is not finite, make
  * the results they go into NaN, behind every activation; an infinity in a row of A makes the sums it goes into infinite or NaN, which of these is not said (of minus infinity ReLU makes 0).  C must not overlap A, W, scales, zeros or bias. */
 typedef struct gp_gemm_w4_params {
     int dtype;

@@ -726,3 +726,55 @@ def test_what_is_not_finite_stays_so_behind_every_activation(gp, dt, act, m, n, 
     assert (up.isnan() | (up == math.inf)).all()
     assert (down.isnan() | (down == (-math.inf if act == "none" else 0.0)) | ((down == -math.inf) if act == "gelu" else False)).all()
     assert (total == math.inf).any() and (total == -math.inf).any() and total.isnan().any()
+
+
+class ExactW4(W4):
+    """... whatever the size: nothing but the result is rounded to 16 bits"""
+
+    def check(self):
+        got, (want, mass) = self.left(), self.definition()
+        deep = self.group + 2 * self.k // self.group + 32
+        allowed = S.half_step(self.dt) * want.abs() + 1.13 * deep * 2.0 ** -23 * mass + (2.0 ** -25 if self.dt == "f16" else 0.0)
+        err = (got[:, : self.n].double() - want).abs()
+        assert (err <= allowed).all(), (float((err / allowed).max()), (err / allowed).argmax())
+        assert (got[:, self.n:] == 7.0).all()
+
+
+EXACT = [
+    (65, 11009, 96, 32), (100, 11009, 256, 128), (128, 23000, 192, 64),  # one tile of rows, partly empty, of many columns
+    (129, 130, 352, 32), (130, 300, 1152, 128), (200, 515, 576, 64), (257, 256, 256, 128),
+    (1101, 1303, 160, 32), (1101, 1303, 192, 64), (1100, 1302, 384, 128), (1025, 1281, 32, 32), (700, 2000, 2048, 128), (2945, 3001, 96, 32), (2945, 3001, 320, 64), (3000, 2945, 256, 128),
+]
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("case", range(len(EXACT)))
+def test_only_the_result_is_rounded_whatever_the_size(gp, dt, case):
+    m, n, k, group = EXACT[case]
+    w = ExactW4(gp, dt, m, n, k, group, 500 + case, zeros=case % 3 != 0, bias=case % 2 == 0, residual=case % 4 < 2, act=list(ACTS)[case % 3], pad=case % 3, in_place=case % 4 == 1, spread=256 if case % 2 else 16)
+    w.launch()
+    w.check()
+    first = w.left()
+    w.clean()
+    w.launch()
+    assert torch.equal(w.left(), first)
+
+
+@pytest.mark.parametrize("m, n", [(3, 150), (200, 150), (1200, 1301)])
+def test_weights_beyond_the_largest_of_16_bits(gp, m, n):
+    """fp16: a scale of 8000 times numbers up to 15 less 0: weights up to 120000, sums that fit"""
+    def change(w):
+        w.a *= 2.0 ** -9
+        w.scales[5], w.zeros[5] = 8000.0, 0
+    w = ExactW4(gp, "f16", m, n, 256, 64, 73, bias=False, residual=False, change=change)
+    assert float((w.q[5].double() * 8000).max()) > 65504
+    w.launch()
+    w.check()
+
+
+def test_rows_are_as_exact_among_many_as_alone(gp):
+    many = ExactW4(gp, "bf16", 1200, 1301, 512, 64, 74)
+    for m in (1, 40, 1200):
+        w = ExactW4(gp, "bf16", m, 1301, 512, 64, 75, change=lambda w: [getattr(w, x).copy_(getattr(many, x)[: m] if x in ("a", "residual") else getattr(many, x)) for x in ("a", "residual", "q", "scales", "zeros", "bias")])
+        w.launch()
+        w.check()
