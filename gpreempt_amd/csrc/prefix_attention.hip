@@ -12,11 +12,11 @@
 #include "paged_few.hpp"
 #include "paged_many.hpp"
 #include "launch_tiles.hpp"
+#include "../../include/util/join_counters.h"
 
 namespace gp {
 
-constexpr int PREFIX_ROWS = 64;      // of a sequence and a head of the cache, at most
-constexpr int PREFIX_UNITS = 16384;  // counters: sequences times blocks of their rows times heads, at most
+constexpr int PREFIX_ROWS = 64;  // of a sequence and a head of the cache, at most
 
 struct PrefixArgs {
     FewArgs few;              // of the sequences' own keys
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(FEW_NT, 2) void prefix_kernel(PrefixArgs a, BlpArgs
 }
 
 // in front of everything else, whatever the launch: so one workspace serves launches of any sizes
-static size_t prefix_counter_bytes() { return (PREFIX_UNITS + 4 * (size_t)device_cus()) * sizeof(int); }
+static size_t prefix_counter_bytes() { return prefix_counters(device_cus()).bytes; }
 
 struct PrefixPlan {
     PrefixArgs a;
@@ -288,11 +288,12 @@ static int plan_prefix(const gp_prefix_attention_params *p, PrefixPlan *pl) {
     GP_REQUIRE(pl->tiles < (1L << 31), "prefix_attention: too large");
     const size_t part = (size_t)16 * pl->nt * (q.cache.head_dim + 2) * sizeof(float), many = (size_t)(q.cache.head_dim / 2 + 2) * MANY_NT * sizeof(float);
     char *at = (char *)q.work;
-    auto take = [&](size_t bytes) { char *x = at + pl->work_bytes; pl->work_bytes += (bytes + 255) / 256 * 256; return x; };
-    pl->work_bytes = 0;
-    few.arrived = (int *)take(2 * device_cus() * sizeof(int));  // (parts of the own keys, and of the shared ones: at most so many where there are any)
-    a.arrived = (int *)take(PREFIX_UNITS * sizeof(int));
-    a.met = (int *)take(2 * device_cus() * sizeof(int));
+    auto take = [&](size_t bytes) { char *x = at + pl->work_bytes; pl->work_bytes += join_aligned(bytes); return x; };
+    const PrefixCounters counters = prefix_counters(device_cus());
+    few.arrived = (int *)(at + counters.parts);  // (parts of the own keys, and of the shared ones: at most two to a compute unit where there are any)
+    a.arrived = (int *)(at + counters.arrived);
+    a.met = (int *)(at + counters.met);
+    pl->work_bytes = counters.bytes;
     a.own = (float *)take(heads * q.batch * part);
     a.shared = (float *)take((size_t)a.shared_tiles * many);
     few.partial = (float *)take(few.shares > 1 ? (size_t)heads * few.shares * 2 * part : 0);

@@ -103,3 +103,9 @@ def test_null_params():
     assert gp.lib().gp_prefix_attention_work_bytes(None, C.byref(n)) == gp.OUTOFRANGE
     assert gp.lib().gp_prefix_attention_work_bytes(C.byref(prefix()), None) == gp.OUTOFRANGE
     assert gp.lib().gp_prefix_attention_work_bytes(C.byref(prefix()), C.byref(n)) == gp.SUCC
+
+
+def test_counters_in_front_of_a_workspace(tmp_path):
+    exe = str(tmp_path / "check")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "include"), os.path.join(ROOT, "tests", "join_counters_check.cpp"), "-o", exe])
+    assert subprocess.run([exe], capture_output=True, text=True).stdout == "ok\n"
