@@ -37,6 +37,7 @@ struct FewArgs {
     int *arrived;     // workspace: a counter for every (head, row block, part), 0 between launches
     float *partial;   // ... and for every tile two results: 16 * NT rows of D values, then their maxima and sums
     int skip;         // keys at the beginning that are left out, of the sequences all of whose rows see them
+    int whole;        // not 0: sequences of up to so many units have a tile each, in front of the parts, which are of the others' keys
 };
 
 template <int NT, int D> constexpr int few_partial_floats() { return 16 * NT * (D + 2); }
@@ -455,9 +456,10 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
     const gp_paged_attention_params &p = a.p;
     constexpr int ROWS = 16 * NT, UNIT = few_unit<E8>();
     const int lane = threadIdx.x & 63, hr = t.y, rb = hr % a.row_blocks, batch = p.batch;
-    if (a.shares == 0) {  // a tile per sequence
+    const int whole = Out::SKIPS ? a.whole : 0, part = t.x - (whole ? batch : 0);
+    if (a.shares == 0 || part < 0) {  // a tile per sequence
         const FewSequence f = few_sequence<ROWS, UNIT, Out::SKIPS>(a, seq_tokens(p.start, p.kv_len, t.x, p.tokens, p.max_new), rb);
-        if (f.nrows > 0) attend_stretch<T, D, E8, NT>(a, f, t.x, hr, f.skip, f.kend, nullptr, 0, 0, lds, out);
+        if (f.nrows > 0 && (whole == 0 || f.units <= whole)) attend_stretch<T, D, E8, NT>(a, f, t.x, hr, f.skip, f.kend, nullptr, 0, 0, lds, out);
         return;
     }
     // ---- all units; then the sequence in which this part begins.  Every wavefront for itself, 64 sequences at a time, one to a lane ----
@@ -467,7 +469,8 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
         r0 = p.start ? p.start[b] : b;
         r1 = p.start ? p.start[b + 1] : b + 1;
         len = p.kv_len[b];
-        return b0 + lane < batch ? few_sequence<ROWS, UNIT, Out::SKIPS>(a, seq_tokens_of(r0, r1, len, p.tokens, p.max_new), rb).units : 0;
+        const int units = few_sequence<ROWS, UNIT, Out::SKIPS>(a, seq_tokens_of(r0, r1, len, p.tokens, p.max_new), rb).units;
+        return b0 + lane < batch && units > whole ? units : 0;
     };
     int total = 0, n = 0;
     for (int b0 = batch <= 64 ? 0 : (batch - 1) / 64 * 64; b0 >= 0; b0 -= 64) total += n = look(b0);  // (the first 64 last: they are looked at next)
@@ -479,9 +482,9 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
     // 131072 level, 50 and 82)
     constexpr int LEAST = NT == 1 ? 2 : 4;
     const int shares = total / LEAST < 1 ? 1 : total / LEAST < a.shares ? total / LEAST : a.shares;
-    if (total == 0 || t.x >= shares) return;  // (no sequence has rows in this block)
-    const int lo = part_begin(t.x, total, shares), hi = part_begin(t.x + 1, total, shares);
-    float *slots = a.partial + ((long)hr * a.shares + t.x) * 2 * few_partial_floats<NT, D>();
+    if (total == 0 || part >= shares) return;  // (no sequence has rows in this block)
+    const int lo = part_begin(part, total, shares), hi = part_begin(part + 1, total, shares);
+    float *slots = a.partial + ((long)hr * a.shares + part) * 2 * few_partial_floats<NT, D>();
     walk_part(batch, 64, lo, hi, [&](int b0, int unit, int &at, int &i) {
         if (b0) n = look(b0);
         int upto = n;
@@ -496,7 +499,7 @@ __device__ __forceinline__ void attend_few(const FewArgs &a, TileIdx t, float *l
         return behind != 0;
     }, look, [&](int b, int i, int at) {
         const FewSequence f = few_sequence<ROWS, UNIT, Out::SKIPS>(a, seq_tokens_of(__builtin_amdgcn_readlane(r0, i), __builtin_amdgcn_readlane(r1, i), __builtin_amdgcn_readlane(len, i), p.tokens, p.max_new), rb);
-        if (f.units == 0) return 0;
+        if (f.units <= whole) return 0;
         const int u0 = lo > at ? lo - at : 0, u1 = hi - at < f.units ? hi - at : f.units;
         attend_stretch<T, D, E8, NT>(a, f, b, hr, f.skip + u0 * UNIT, u1 == f.units ? f.kend : f.skip + u1 * UNIT, slots + (u0 == 0) * few_partial_floats<NT, D>(),
                                      part_of(at, total, shares), part_of(at + f.units - 1l, total, shares), lds, out);

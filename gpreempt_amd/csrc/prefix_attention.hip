@@ -260,9 +260,10 @@ static int plan_prefix(const gp_prefix_attention_params *p, PrefixPlan *pl) {
     GP_REQUIRE(p->shared_len <= (1 << 30), "prefix_attention: shared_len must be at most 2^30");
     GP_REQUIRE(p->variant >= GP_PREFIX_AUTO && p->variant <= GP_PREFIX_EACH, "prefix_attention: variant %d", p->variant);
     const bool can = p->shared_len > 0 && rows <= PREFIX_ROWS && heads * q.batch <= PREFIX_UNITS;
+    const long reach = std::min((long)q.max_len, (long)q.table_width * q.cache.page_size);  // (what is shared behind it nobody sees)
     GP_REQUIRE(can || p->variant != GP_PREFIX_TOGETHER, "prefix_attention: together only behind shared tokens, up to %d query rows of a sequence to a head of the cache and %d blocks of 16 or 32 of them", PREFIX_ROWS, PREFIX_UNITS);
     const double megabytes = 0x1p-19 * p->shared_len * q.cache.kv_heads * q.cache.head_dim * (q.cache.dtype == GP_E4M3 ? 1 : 2);
-    pl->shared = can && (p->variant == GP_PREFIX_AUTO ? (q.batch - 1) * megabytes >= std::min(80 + 5 * megabytes, 280.) : p->variant == GP_PREFIX_TOGETHER);
+    pl->shared = can && reach >= p->shared_len && (p->variant == GP_PREFIX_AUTO ? (q.batch - 1) * megabytes >= std::min(80 + 5 * megabytes, 280.) : p->variant == GP_PREFIX_TOGETHER);
     if (!pl->shared) return GP_SUCC;
     a.table = p->shared_table;
     a.shared_len = few.skip = p->shared_len;
@@ -272,18 +273,28 @@ static int plan_prefix(const gp_prefix_attention_params *p, PrefixPlan *pl) {
     const long units = (long)a.blocks * q.cache.kv_heads, key_tiles = (p->shared_len + MANY_KEYS - 1l) / MANY_KEYS;
     // Own keys: a tile for each sequence, or in equal parts, two per compute unit, where there are few sequences or long ones.  (e4m3, 8 heads of 128, behind 8192 shared ones; us, a tile each / parts:
     // 64 sequences of up to 2048 own keys 74 / 83, of up to 7808 161 / 138; 16 of up to 7232 behind 32768 82 / 74.  One part per compute unit: 88, 176, 82)
+    // A sequence that does not see all of what is shared has keys of its own from the first on: where that may be more than a tile of the others has, its keys are dealt out in parts, one for each compute unit,
+    // behind the others' tiles.  (A tile is not stopped half-way, and reads 25 to 30 GB/s.  Us, in one tile / in parts (8 heads of 128), of which
+    // none / one / eight end 100 to 1000 tokens within what is shared: 64 sequences behind 8192, e4m3, 71 / 103 / 141 and 71 / 68 / 74; 64 behind 32768 79 / 244 / 478 and 76 / 84 / 179; 8 behind 131072, bf16, one: 1623
+    // and 229)
     const int unit = q.cache.dtype == GP_E4M3 ? few_unit<true>() : few_unit<false>();
-    const long most = std::max(1l, ((long)q.max_len - p->shared_len + unit - 1) / unit);
+    const long most = std::max(1l, (reach - p->shared_len + unit - 1) / unit), whole = heads * q.batch < 2l * device_cus() ? 4 : 16;
+    const long all = std::max(most, (std::min(reach, p->shared_len + few.p.max_new - 1l) + unit - 1) / unit);  // of a sequence that ends within what is shared, or begins there
     a.own_x = q.batch;
-    if (most > (heads * q.batch < 2l * device_cus() ? 4 : 16)) a.own_x = few.shares = (int)std::min(std::max(1l, 2l * device_cus() / heads), most * q.batch);
+    if (most > whole) a.own_x = few.shares = (int)std::min(std::max(1l, 2l * device_cus() / heads), all * q.batch);
+    else if (all > whole) {
+        few.whole = (int)whole;
+        few.shares = (int)std::min(std::max(1l, device_cus() / heads), all * q.batch);
+        a.own_x += few.shares;
+    }
     // Shared tiles, one to a compute unit beside the sequences' own, whose loads then have their arithmetic to hide behind, or two where there is little else to do.  Us, one / two (8 heads of 128): 64 sequences
     // of up to 2048 own tokens behind 8192, e4m3, 61 / 71, of 1 to 2 42 / 47; 256 of up to 316 behind 16384, fp16, 124 / 134; 128 of up to 404 behind 4096 47 / 58; 128 of up to 232 behind 32768, e4m3,
     // 127 / 113; 64 of the same, fp16, 83 / 79.
-    const long own_tiles = heads * a.own_x, per_unit = own_tiles >= 2l * device_cus() && units * key_tiles <= 8 * own_tiles ? 1 : 2;
+    const long own_tiles = heads * (few.whole ? q.batch : a.own_x), per_unit = own_tiles >= 2l * device_cus() && units * key_tiles <= 8 * own_tiles ? 1 : 2;
     a.shares = (int)std::max(1l, std::min(per_unit * device_cus() / units, key_tiles / 4));
     a.shared_tiles = (int)(units * a.shares);
     a.shared_slice = (a.shared_tiles + 7) / 8;
-    a.own_slice = (int)((own_tiles + 7) / 8);
+    a.own_slice = (int)((heads * a.own_x + 7) / 8);
     pl->tiles = 8l * a.shared_slice + 8l * a.own_slice;
     GP_REQUIRE(pl->tiles < (1L << 31), "prefix_attention: too large");
     const size_t part = (size_t)16 * pl->nt * (q.cache.head_dim + 2) * sizeof(float), many = (size_t)(q.cache.head_dim / 2 + 2) * MANY_NT * sizeof(float);

@@ -778,3 +778,67 @@ def test_rows_are_as_exact_among_many_as_alone(gp):
         w = ExactW4(gp, "bf16", m, 1301, 512, 64, 75, change=lambda w: [getattr(w, x).copy_(getattr(many, x)[: m] if x in ("a", "residual") else getattr(many, x)) for x in ("a", "residual", "q", "scales", "zeros", "bias")])
         w.launch()
         w.check()
+
+
+# ---- sequences that end within a long shared beginning ----------------------------------------------------------------------------
+
+
+def long_beginning(lens, news, page, shared, rng):
+    """as begin_alike, without pages in the pool that nobody names"""
+    seqs = S.Sequences(lens, news, page, rng, width=max(1, -(-(max(lens) - shared) // page)))
+    pages = shared // page
+    seqs.table = torch.cat([torch.arange(seqs.pages, seqs.pages + pages, dtype=torch.int32).repeat(seqs.batch, 1), seqs.table], 1)
+    seqs.pages, seqs.width, seqs.shared = seqs.pages + pages, seqs.width + pages, shared
+    return seqs
+
+
+LONG_BEGINNINGS = [
+    # lens, news, page, shared, heads, kv_heads, dim: keys of a sequence that does not see all of what is shared are more than a tile's
+    ([16384 + 9 + i for i in range(6)] + [16000, 9000, 16384, 1, 0], None, 128, 16384, 8, 2, 64),
+    ([8192 + 40 + 3 * i for i in range(8)] + [8190, 8192 + 2, 5000], [3] * 8 + [3, 5, 1], 64, 8192, 8, 2, 64),  # one has new tokens in front of the end of what is shared
+    ([4096 + 17] * 64 + [4000, 3999, 17] + [4096 + 2] * 3, None, 128, 4096, 8, 8, 64),  # many sequences, and parts of several of them
+    ([4096 + 17] * 64 + [4095] * 6, [2] * 70, 128, 4096, 64, 8, 64),
+    ([8192 + 700, 8192 + 30, 8000], None, 128, 8192, 8, 1, 128),  # own keys in parts anyway
+    ([3000, 2999], None, 128, 4096, 8, 1, 128),  # nobody sees all of it
+]
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("case", range(len(LONG_BEGINNINGS)))
+def test_sequences_that_end_within_a_long_beginning(gp, dt, cache, case):
+    lens, news, page, shared, heads, kv_heads, dim = LONG_BEGINNINGS[case]
+    a = Prefix(gp, dt, dt if cache == "same" else cache, long_beginning(lens, news, page, shared, gen(80 + case)), heads, kv_heads, dim, True, 600 + case)
+    a.launch()
+    a.check()
+    first = a.left()
+    a.clean()
+    a.launch()
+    assert torch.equal(a.left(), first)
+
+
+def test_a_sequence_that_ends_within_a_long_beginning_is_not_left_to_one_workgroup(gp):
+    """its 256 units of keys in one tile took 20 times what the others' call takes"""
+    def took(lens):
+        a = Prefix(gp, "bf16", "bf16", long_beginning(lens, None, 128, 32768, gen(90)), 4, 1, 64, True, 91)
+        times = []
+        for _ in range(9):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            for _ in range(20):
+                a.launch()
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        return sorted(times)[4]
+    assert took([32768 + 20 + i for i in range(5)] + [32700]) < 6 * took([32768 + 20 + i for i in range(6)])
+
+
+def test_what_nobody_sees_is_not_read_for_all(gp):
+    """max_len, or the table, ends in front of the end of what is shared: each sequence for itself, whoever asks"""
+    seqs = begin_alike(S.Sequences([300, 210, 330], None, 64, gen(13)), 192)
+    for max_len, tiles in ((191, 3), (192, None)):
+        a = Prefix(gp, "bf16", "bf16", seqs, 8, 2, 128, True, 14, max_len=max_len)
+        got = a.launch().total_tiles
+        assert (got == 2 * 3) if tiles else got >= 16
+        a.check()
