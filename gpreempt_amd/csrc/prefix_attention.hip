@@ -271,8 +271,9 @@ static int plan_prefix(const gp_prefix_attention_params *p, PrefixPlan *pl) {
     a.per_block = MANY_ROWS / a.rows;
     a.blocks = (q.batch + a.per_block - 1) / a.per_block;
     const long units = (long)a.blocks * q.cache.kv_heads, key_tiles = (p->shared_len + MANY_KEYS - 1l) / MANY_KEYS;
-    // Own keys: a tile for each sequence, or in equal parts, two per compute unit, where there are few sequences or long ones.  (e4m3, 8 heads of 128, behind 8192 shared ones; us, a tile each / parts:
-    // 64 sequences of up to 2048 own keys 74 / 83, of up to 7808 161 / 138; 16 of up to 7232 behind 32768 82 / 74.  One part per compute unit: 88, 176, 82)
+    // Own keys: a tile for each sequence, or in equal parts, two per compute unit, where there are few sequences or long ones.  Us, a tile each / parts (8 heads of 128, 512 of a sequence's tiles fill the chip
+    // once), up to 2048 own keys behind 8192 shared ones, e4m3: 16 sequences 39 / 38, 32 47 / 43, 48 55 / 53, 63 60 / 61, 64 63 / 69, 80 62 / 76; behind 4096 63 65 / 65; up to 4096 own keys 63 sequences 101 / 88,
+    // 64 88 / 86; behind 4096 up to 512 own keys 48 sequences 35.8 / 35.
     // A sequence that does not see all of what is shared has keys of its own from the first on: where that may be more than a tile of the others has, its keys are dealt out in parts, one for each compute unit,
     // behind the others' tiles.  (A tile is not stopped half-way, and reads 25 to 30 GB/s.  Us, in one tile / in parts (8 heads of 128), of which
     // none / one / eight end 100 to 1000 tokens within what is shared: 64 sequences behind 8192, e4m3, 71 / 103 / 141 and 71 / 68 / 74; 64 behind 32768 79 / 244 / 478 and 76 / 84 / 179; 8 behind 131072, bf16, one: 1623
@@ -287,10 +288,10 @@ static int plan_prefix(const gp_prefix_attention_params *p, PrefixPlan *pl) {
         few.shares = (int)std::min(std::max(1l, device_cus() / heads), all * q.batch);
         a.own_x += few.shares;
     }
-    // Shared tiles, one to a compute unit beside the sequences' own, whose loads then have their arithmetic to hide behind, or two where there is little else to do.  Us, one / two (8 heads of 128): 64 sequences
-    // of up to 2048 own tokens behind 8192, e4m3, 61 / 71, of 1 to 2 42 / 47; 256 of up to 316 behind 16384, fp16, 124 / 134; 128 of up to 404 behind 4096 47 / 58; 128 of up to 232 behind 32768, e4m3,
-    // 127 / 113; 64 of the same, fp16, 83 / 79.
-    const long own_tiles = heads * (few.whole ? q.batch : a.own_x), per_unit = own_tiles >= 2l * device_cus() && units * key_tiles <= 8 * own_tiles ? 1 : 2;
+    // Shared tiles: one to a compute unit, beside the sequences' own, whose loads then have their arithmetic to hide behind, or two where the shared keys are most of the work.  Us, one / two (8 heads of 128), with
+    // 4, 8, 16 and 32 tiles of shared keys to a tile of own ones, or to half a compute unit: 63 sequences of up to 100 own keys, e4m3, 39 / 46, 51 / 53, 73 / 71; 256 of up to 316 78 / 89, 119 / 117, 203 / 183,
+    // 385 / 322; 64 of up to 2048 63 / 72, 62 / 75, 80 / 91, 125 / 120; fp16 96 / 104, 86 / 107, 108 / 127, 149 / 157; 256 of up to 1000 141 / 167, 171 / 206, 265 / 270, 471 / 417.
+    const long own_tiles = std::max(heads * (few.whole ? q.batch : a.own_x), 2l * device_cus()), per_unit = units * key_tiles <= (9 + most) * own_tiles ? 1 : 2;
     a.shares = (int)std::max(1l, std::min(per_unit * device_cus() / units, key_tiles / 4));
     a.shared_tiles = (int)(units * a.shares);
     a.shared_slice = (a.shared_tiles + 7) / 8;

@@ -109,3 +109,19 @@ def test_counters_in_front_of_a_workspace(tmp_path):
     exe = str(tmp_path / "check")
     subprocess.check_call(["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "include"), os.path.join(ROOT, "tests", "join_counters_check.cpp"), "-o", exe])
     assert subprocess.run([exe], capture_output=True, text=True).stdout == "ok\n"
+
+
+def work_bytes(variant, batch, shared, own, heads, kv_heads, dim, dtype):
+    c = cache(dtype=dtype, kv_heads=kv_heads, head_dim=dim, page_size=64, pages=1 << 20, **(dict(k_scale=AT, v_scale=AT) if dtype == gp.E4M3 else {}))
+    p = prefix(shared, cache=c, dtype=gp.F16, batch=batch, tokens=batch, max_new=1, start=None, max_len=shared + own, table_width=-(-(shared + own) // 64), heads=heads, ld_q=heads * dim, ld_out=heads * dim,
+               variant=variant)
+    n = C.c_size_t()
+    gp.check(gp.lib().gp_prefix_attention_work_bytes(C.byref(p), C.byref(n)))
+    return n.value
+
+
+@pytest.mark.parametrize("shared", [8192, 16384, 32768])
+def test_one_sequence_more_does_not_change_how_the_shared_keys_are_cut(shared):
+    """about as many sequences as fill the chip once: the workspace, of which a part of the shared keys takes 66 KB, grows by a sequence's share of it"""
+    sizes = [work_bytes(gp.PREFIX_TOGETHER, batch, shared, 100, 32, 8, 128, gp.E4M3) for batch in (62, 63, 64)]
+    assert max(sizes) - min(sizes) < 1 << 20, sizes
