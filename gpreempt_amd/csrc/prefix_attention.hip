@@ -254,16 +254,18 @@ static int plan_prefix(const gp_prefix_attention_params *p, PrefixPlan *pl) {
     pl->nt = rows <= 16 ? 1 : 2;
     few.row_blocks = (int)((rows + 16 * pl->nt - 1) / (16 * pl->nt));
     const long heads = (long)few.row_blocks * q.cache.kv_heads;
-    // Once for all, or for each sequence as if nothing were shared: the first has some 10 to 20 us of parts that meet in front of it, the second reads (batch - 1) times what is shared once more, from caches
-    // where it is small.  Us, once / each (100 own tokens, one new): e4m3, 8 heads of 128 (32 of queries), 1024 shared tokens: 64 sequences 25 / 25; 4096: 16 sequences 30 / 22, 64 35 / 58; 16384: 8 sequences
-    // 47 / 37, 16 48 / 61, 64 55 / 212; bf16, 16384: 4 sequences 48 / 36, 8 49 / 56; bf16, 12 heads of 64: 1024: 64 sequences 17 / 37; 4096: 8 sequences 23 / 23, 16 23 / 35.
+    // Once for all, or for each sequence as if nothing were shared: the first has some 10 to 30 us of parts that meet in front of it, more for more keys, the second reads (batch - 1) times what is shared once more,
+    // from caches where it is small.  Us, once / each (up to 100 own tokens, one new), around the border of 8 heads of 128 (32 of queries), e4m3, 1024 shared tokens: 64 sequences 25.5 / 25.3, 96 26 / 36; 4096: 16
+    // sequences 30 / 23, 24 31 / 32, 32 32 / 33, 48 34 / 49; 16384: 8 sequences 40 / 36, 12 40 / 53; fp16, 1024: 32 sequences 26 / 17, 48 26 / 26, 64 27 / 29; 16384: 4 sequences 42 / 35, 6 42 / 54; 2 heads of 128 (32 of
+    // queries), fp16, 4096: 48 sequences 34 / 32, 64 34 / 33, 96 38 / 45; 12 heads of 64, bf16, where the second is slower for the same bytes: 1024: 16 sequences 17.0 / 15.4, 24 17.4 / 18.7; 4096: 8 22.8 / 23.3.
+    // Of 225 measured pairs the choice costs 0.5 % on average and 15 % at most.
     GP_REQUIRE(p->shared_len <= (1 << 30), "prefix_attention: shared_len must be at most 2^30");
     GP_REQUIRE(p->variant >= GP_PREFIX_AUTO && p->variant <= GP_PREFIX_EACH, "prefix_attention: variant %d", p->variant);
     const bool can = p->shared_len > 0 && rows <= PREFIX_ROWS && heads * q.batch <= PREFIX_UNITS;
     const long reach = std::min((long)q.max_len, (long)q.table_width * q.cache.page_size);  // (what is shared behind it nobody sees)
     GP_REQUIRE(can || p->variant != GP_PREFIX_TOGETHER, "prefix_attention: together only behind shared tokens, up to %d query rows of a sequence to a head of the cache and %d blocks of 16 or 32 of them", PREFIX_ROWS, PREFIX_UNITS);
-    const double megabytes = 0x1p-19 * p->shared_len * q.cache.kv_heads * q.cache.head_dim * (q.cache.dtype == GP_E4M3 ? 1 : 2);
-    pl->shared = can && reach >= p->shared_len && (p->variant == GP_PREFIX_AUTO ? (q.batch - 1) * megabytes >= std::min(80 + 5 * megabytes, 280.) : p->variant == GP_PREFIX_TOGETHER);
+    const double megabytes = 0x1p-19 * p->shared_len * q.cache.kv_heads * q.cache.head_dim * (q.cache.dtype == GP_E4M3 ? 1 : 2) * (q.cache.head_dim == 64 ? 2.5 : 1);
+    pl->shared = can && reach >= p->shared_len && (p->variant == GP_PREFIX_AUTO ? (q.batch - 1) * megabytes >= std::min(150 + 10 * megabytes, 280.) : p->variant == GP_PREFIX_TOGETHER);
     if (!pl->shared) return GP_SUCC;
     a.table = p->shared_table;
     a.shared_len = few.skip = p->shared_len;

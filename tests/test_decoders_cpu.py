@@ -125,3 +125,15 @@ def test_one_sequence_more_does_not_change_how_the_shared_keys_are_cut(shared):
     """about as many sequences as fill the chip once: the workspace, of which a part of the shared keys takes 66 KB, grows by a sequence's share of it"""
     sizes = [work_bytes(gp.PREFIX_TOGETHER, batch, shared, 100, 32, 8, 128, gp.E4M3) for batch in (62, 63, 64)]
     assert max(sizes) - min(sizes) < 1 << 20, sizes
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, dtype, shared, each, together", [
+    (32, 8, 128, gp.E4M3, 1024, 48, 96), (32, 8, 128, gp.E4M3, 4096, 16, 48), (32, 8, 128, gp.E4M3, 16384, 8, 12), (32, 8, 128, gp.F16, 1024, 32, 64), (32, 8, 128, gp.F16, 16384, 4, 6),
+    (8, 1, 128, gp.E4M3, 8192, 48, 128), (32, 2, 128, gp.F16, 4096, 32, 96), (12, 12, 64, gp.F16, 1024, 12, 32), (12, 12, 64, gp.F16, 4096, 6, 12),
+])
+def test_the_launcher_chooses_what_is_faster(heads, kv_heads, dim, dtype, shared, each, together):
+    """numbers of sequences on either side of where measurements cross"""
+    for batch, variant in ((each, gp.PREFIX_EACH), (together, gp.PREFIX_TOGETHER)):
+        sizes = {v: work_bytes(v, batch, shared, 100, heads, kv_heads, dim, dtype) for v in (gp.PREFIX_AUTO, gp.PREFIX_EACH, gp.PREFIX_TOGETHER)}
+        assert sizes[gp.PREFIX_EACH] != sizes[gp.PREFIX_TOGETHER]
+        assert sizes[gp.PREFIX_AUTO] == sizes[variant], (batch, sizes)
