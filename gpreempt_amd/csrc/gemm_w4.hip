@@ -212,7 +212,7 @@ __device__ __forceinline__ void w4_tile(const W4Args &a, TileIdx t, char *lds) {
 }
 
 template <typename T, int G, int MT, int NT, int WAVES, int LOOP = LOOP_ANY>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : MT * NT > 2 ? 2 : 4) void gemm_w4_kernel(W4Args a, BlpArgs blp) {
+__global__ __launch_bounds__(64 * WAVES, MT * NT > 2 ? 2 : 4) void gemm_w4_kernel(W4Args a, BlpArgs blp) {
     extern __shared__ __attribute__((aligned(16))) unsigned char w4_lds[];
     tiles<LOOP>(blp, [&](TileIdx t) { w4_tile<T, G, MT, NT, WAVES>(a, t, (char *)w4_lds); });
 }

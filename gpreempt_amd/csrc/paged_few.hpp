@@ -115,63 +115,6 @@ template <typename T, int D, int ROWS> struct FewOut {
     __device__ __forceinline__ void done(const FewSequence &, int, int) const {}  // all rows of the block
 };
 
-// Joins the results of `parts` parts of some rows, in their order: 16 * NT rows at most, `rows` of them there.  get(i, r, d): four values of row r of the i-th; get_ml(i, r): its reference
-// and sum; put(r, d, v, top, sum).  (up to FEW_JOIN of them at a time: first their factors, which every thread needs, then their values, eight loads of a thread in
-// flight.  A part that no row saw anything of has factor 0, and its values are zeros.)
-template <int D, int NT, int LDS_FLOATS, class Get, class GetMl, class Put>
-__device__ __forceinline__ void join_parts(int parts, int rows, float *lds, Get &&get, GetMl &&get_ml, Put &&put) {
-#pragma clang fp contract(off)
-    constexpr int ROWS = 16 * NT;
-    constexpr int FEW_JOIN = LDS_FLOATS / (2 * ROWS) < 256 ? LDS_FLOATS / (2 * ROWS) : 256;
-    constexpr int ITEMS = (ROWS * D / 4 + FEW_NT - 1) / FEW_NT;  // of a thread: four values of one row
-    const int tid = threadIdx.x;
-    f32x4 v[ITEMS];
-    float top[ITEMS], sum[ITEMS];
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) { v[k] = f32x4{0.f, 0.f, 0.f, 0.f}; top[k] = -INFINITY; sum[k] = 0.f; }
-    for (int i0 = 0; i0 < parts; i0 += FEW_JOIN) {
-        const int n = parts - i0 < FEW_JOIN ? parts - i0 : FEW_JOIN;
-        __syncthreads();
-        for (int u = tid; u < n * rows; u += FEW_NT) {
-            const int i = u / rows, r = u - i * rows;
-            *(f32x2 *)(lds + 2 * (i * ROWS + r)) = get_ml(i0 + i, r);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < ITEMS; ++k) {
-            const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
-            if (r >= rows) continue;
-            float now = top[k];
-            for (int i = 0; i < n; ++i) now = fmaxf(now, lds[2 * (i * ROWS + r)]);
-            const float base = now == -INFINITY ? 0.f : now, f0 = __builtin_amdgcn_exp2f(top[k] - base);
-            top[k] = now;
-            sum[k] *= f0;
-            v[k] *= f0;
-            for (int i = 0; i < n; i += 8) {
-                f32x4 y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    y[e] = get(i0 + (i + e < n ? i + e : i), r, d);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (i + e >= n) break;
-                    const f32x2 ms = *(const f32x2 *)(lds + 2 * ((i + e) * ROWS + r));
-                    const float f = __builtin_amdgcn_exp2f(ms[0] - base);
-                    sum[k] = fmaf(f, ms[1], sum[k]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) v[k][c] = fmaf(f, y[e][c], v[k][c]);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-        const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
-        if (r < rows) put(r, d, v[k], top[k], sum[k]);
-    }
-}
-
 // Keys [c0, kend) of one sequence; then its rows are finished, or its part of them waits in slot `slot` for the others.
 // first_share, last_share: the parts that the sequence's keys are spread over.
 template <typename T, int D, bool E8, int NT, class Out>
@@ -441,13 +384,59 @@ __device__ __forceinline__ void attend_stretch(const FewArgs &a, const FewSequen
     __syncthreads();
     if (came != parts - 1) return;
     if (tid == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // (up to FEW_JOIN of them at a time: first their factors, which every thread needs, then their values, eight loads of a thread in flight.
+    // A part that no row saw anything of has factor 0, and its values are zeros.)
     const float *all = a.partial + ((long)hr * a.shares + first_share) * 2 * few_partial_floats<NT, D>();
     auto part_at = [&](int i) { return all + (2l * i + (i == 0)) * few_partial_floats<NT, D>(); };  // the first part is what its tile did last
-    join_parts<D, NT, few_lds_floats<NT, D>()>(parts, rows, lds, [&](int i, int r, int d) {
-        const float *from = part_at(i) + r * D + d;
-        const f32x2 x = get_shared(from), y = get_shared(from + 2);
-        return f32x4{x[0], x[1], y[0], y[1]};
-    }, [&](int i, int r) { return get_shared(part_at(i) + ROWS * D + 2 * r); }, [&](int r, int d, f32x4 v, float top, float sum) { out.put(f, b, hr, r, d, v, top, sum); });
+    constexpr int FEW_JOIN = few_lds_floats<NT, D>() / (2 * ROWS) < 256 ? few_lds_floats<NT, D>() / (2 * ROWS) : 256;
+    constexpr int ITEMS = (ROWS * D / 4 + FEW_NT - 1) / FEW_NT;  // of a thread: four values of one row
+    f32x4 v[ITEMS];
+    float top[ITEMS], sum[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) { v[k] = f32x4{0.f, 0.f, 0.f, 0.f}; top[k] = -INFINITY; sum[k] = 0.f; }
+    for (int i0 = 0; i0 < parts; i0 += FEW_JOIN) {
+        const int n = parts - i0 < FEW_JOIN ? parts - i0 : FEW_JOIN;
+        __syncthreads();
+        for (int u = tid; u < n * rows; u += FEW_NT) {
+            const int i = u / rows, r = u - i * rows;
+            *(f32x2 *)(lds + 2 * (i * ROWS + r)) = get_shared(part_at(i0 + i) + ROWS * D + 2 * r);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
+            if (r >= rows) continue;
+            float now = top[k];
+            for (int i = 0; i < n; ++i) now = fmaxf(now, lds[2 * (i * ROWS + r)]);
+            const float base = now == -INFINITY ? 0.f : now, f0 = __builtin_amdgcn_exp2f(top[k] - base);
+            top[k] = now;
+            sum[k] *= f0;
+            v[k] *= f0;
+            for (int i = 0; i < n; i += 8) {
+                f32x2 y[8][2];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float *from = part_at(i0 + (i + e < n ? i + e : i)) + r * D + d;
+                    y[e][0] = get_shared(from);
+                    y[e][1] = get_shared(from + 2);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (i + e >= n) break;
+                    const f32x2 ms = *(const f32x2 *)(lds + 2 * ((i + e) * ROWS + r));
+                    const float f1 = __builtin_amdgcn_exp2f(ms[0] - base);
+                    sum[k] = fmaf(f1, ms[1], sum[k]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[k][c] = fmaf(f1, y[e][c / 2][c % 2], v[k][c]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int u = tid + k * FEW_NT, r = u / (D / 4), d = u % (D / 4) * 4;
+        if (r < rows) out.put(f, b, hr, r, d, v[k], top[k], sum[k]);
+    }
     out.done(f, b, hr);
 }
 

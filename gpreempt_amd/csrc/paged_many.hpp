@@ -122,12 +122,6 @@ __device__ __forceinline__ void many_keys(const Keys &keys, const ManyRow &row_o
     static_assert(KROWS * KLOADS == MANY_KEYS, "the loads of a tile's keys");
     u32x4 kr[KLOADS];
     VRow vr[4];
-    auto block_at = [&](int page, int key) -> long {
-        if constexpr (PAGED) return (((long)(page < 0 ? 0 : page) * keys.cache.kv_heads + keys.kvh) * keys.cache.page_size + (key & (keys.cache.page_size - 1))) * D * ES;
-        else return (key < keys.last ? key : keys.last) * keys.ld;
-    };
-    auto cached_k = [&]() { if constexpr (PAGED) return (const char *)keys.cache.k; else return keys.k; };
-    auto cached_v = [&]() { if constexpr (PAGED) return (const char *)keys.cache.v; else return keys.v; };
     // (packed: a lane's rows of a tile as offsets of 32 bits from the tile's first, which the wavefront shares; in the tile where the sequence ends they stop at its last row.  A multiplication of 64 bits
     // for each load instead: 1540 us for 1520)
     unsigned krow[KLOADS], vrow[4];
@@ -149,23 +143,19 @@ __device__ __forceinline__ void many_keys(const Keys &keys, const ManyRow &row_o
             for (int i = 0; i < KLOADS; ++i) kr[i] = *(const u32x4 *)(k + krow[i]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) vr[e] = *(const VRow *)(v + vrow[e]);
-            return;
-        }
-        const int sub = (tile - window) * 4;
+        } else {
+            auto block_at = [&](int page, int key) -> long { return (((long)(page < 0 ? 0 : page) * keys.cache.kv_heads + keys.kvh) * keys.cache.page_size + (key & (keys.cache.page_size - 1))) * D * ES; };
+            const int sub = (tile - window) * 4;
 #pragma unroll
-        for (int i = 0; i < KLOADS; ++i) {
-            const int row = i * KROWS + tid / (D * ES / 16), chunk = tid % (D * ES / 16);
-            const int page = __builtin_amdgcn_readlane(page_l, sub + (i * KROWS + wave * (64 / (D * ES / 16))) / 16);  // (a wavefront's rows are 16 or part of them)
-            kr[i] = *(const u32x4 *)(cached_k() + block_at(page, tile * MANY_KEYS + row) + chunk * 16);
-        }
-        const int page = __builtin_amdgcn_readlane(page_l, sub + wave), key0 = tile * MANY_KEYS + wave * 16 + lane / 16 * 4;
-        if constexpr (PAGED) {
-            const char *at = cached_v() + block_at(page, key0) + lane % 16 * (VV * ES);
+            for (int i = 0; i < KLOADS; ++i) {
+                const int row = i * KROWS + tid / (D * ES / 16), chunk = tid % (D * ES / 16);
+                const int page = __builtin_amdgcn_readlane(page_l, sub + (i * KROWS + wave * (64 / (D * ES / 16))) / 16);  // (a wavefront's rows are 16 or part of them)
+                kr[i] = *(const u32x4 *)((const char *)keys.cache.k + block_at(page, tile * MANY_KEYS + row) + chunk * 16);
+            }
+            const int page = __builtin_amdgcn_readlane(page_l, sub + wave), key0 = tile * MANY_KEYS + wave * 16 + lane / 16 * 4;
+            const char *at = (const char *)keys.cache.v + block_at(page, key0) + lane % 16 * (VV * ES);
 #pragma unroll
             for (int e = 0; e < 4; ++e) vr[e] = *(const VRow *)(at + e * D * ES);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vr[e] = *(const VRow *)(cached_v() + block_at(page, key0 + e) + lane % 16 * (VV * ES));
         }
     };
     // ---- ... and on to LDS ----
