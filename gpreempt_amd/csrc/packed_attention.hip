@@ -58,7 +58,8 @@ __device__ __forceinline__ void attend_packed(const PackedArgs &a, TileIdx t, ch
 template <typename T, int D, int LOOP = LOOP_ANY>
 __global__ __launch_bounds__(MANY_NT, D == 64 ? 3 : 2) void packed_attention_kernel(PackedArgs a, BlpArgs blp) {
     extern __shared__ __attribute__((aligned(16))) unsigned char packed_lds[];
-    tiles<LOOP>(blp, [&](TileIdx t) { attend_packed<T, D>(a, t, (char *)packed_lds); });
+    // (claims through counters are dealt out, or one of an XCD's would have the longest prompt: four prompts up to 8192, preemptible, 2099 -> 1584 us)
+    tiles<LOOP>(blp, [&](TileIdx t) { attend_packed<T, D>(a, dealt_tile<LOOP>(blp, t), (char *)packed_lds); });
 }
 
 }  // namespace gp

@@ -507,6 +507,11 @@ __device__ __forceinline__ void tiles(const BlpArgs &b, Body &&body) {
     else if constexpr (LOOP == LOOP_FIXED) tile_fixed(b, body);
     else tile_loop(b, body);
 }
+// (for bodies whose tiles are not alike) the tile that stands in for `t` where claims go through several counters: see dealt() in util/slice_map.h
+template <int LOOP> __device__ __forceinline__ TileIdx dealt_tile(const BlpArgs &b, TileIdx t) {
+    if (LOOP != LOOP_ANY || !b.executed) return t;
+    return decode_tile(dealt((t.z * b.sy + t.y) * b.sx + t.x, b.total, b.groups), b.sx, b.sy);
+}
 template <int LOOP, class Body>
 __device__ __forceinline__ void spans(const BlpArgs &b, Body &&body);
 

@@ -90,4 +90,17 @@ GP_HD int xcd_contiguous(int b, int total) {
     return k * q + (k < r ? k : r) + i;
 }
 
+// Tiles that are not alike (heavy ones first): the counters of an XCD own runs of its part of the tile order, one of them all the heavy tiles.  Dealt out, the run that index `idx` of `total` is in has every
+// per-th tile of the XCD's part, in their order, so all its counters go through the part side by side (per = groups / kXcds).  A permutation of 0 .. total - 1, whatever the grid.
+GP_HD int dealt(int idx, int total, int groups) {
+    const int per = groups / kXcds;
+    if (per <= 1) return idx;
+    const int q = total / kXcds, r = total % kXcds, longer = r * (q + 1);
+    const int k = idx < longer ? idx / (q + 1) : r + (idx - longer) / q;  // (q is 0 only if every index is in front of `longer`)
+    const int begin = k * q + (k < r ? k : r), n = q + (k < r), j = idx - begin;
+    const int run = n / per, more = n % per, front = more * (run + 1);
+    const int a = j < front ? j / (run + 1) : more + (j - front) / run, c = j < front ? j % (run + 1) : (j - front) % run;
+    return begin + c * per + a;
+}
+
 }  // namespace gp

@@ -842,3 +842,35 @@ def test_what_nobody_sees_is_not_read_for_all(gp):
         got = a.launch().total_tiles
         assert (got == 2 * 3) if tiles else got >= 16
         a.check()
+
+
+# ---- claims through several counters ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_claims_through_counters_have_the_bits_of_a_plain_launch(gp, which):
+    """fewer workgroups than tiles, which claim through 16, 32 and 64 counters, whole and stopped and resumed"""
+    call = [lambda: Prefix(gp, "bf16", "e4m3", begin_alike(S.Sequences([1300 + i for i in range(70)], None, 64, gen(92)), 1280), 8, 2, 128, True, 93),
+            lambda: Prefix(gp, "f16", "f16", begin_alike(S.Sequences([2060, 2100, 1500, 2049] * 8, [2, 1, 3, 1] * 8, 64, gen(94), width=33), 2048), 16, 4, 64, True, 95),
+            lambda: Packed(gp, "bf16", [2000, 700, 5, 1300], 8, 2, 64, True, 96),
+            lambda: Packed(gp, "f16", [100 + 7 * i for i in range(30)], 4, 4, 128, False, 97),
+            lambda: Attend(gp, "bf16", "e4m3", S.Sequences([900, 1800, 400], [900, 1500, 300], 64, gen(98)), 8, 2, 128, True, 99)][which]()
+    clean = getattr(call, "clean", lambda: call.out.fill_(7.0))
+    call.launch()
+    want = call.left()
+    for groups in (16, 32, 64):
+        flag = gp.Flag()
+        st = gp.BlpState(1, flag, groups)
+        clean()
+        info = call.launch(st.ctx(max_workgroups=64))
+        assert info.total_tiles > info.grid  # claims go through the counters
+        assert same(call.left(), want), groups
+        st.reset()
+        clean()
+        call.launch(st.ctx(inject_at=groups, max_workgroups=64, poll_every=1))
+        call.left()
+        assert flag.get() == 1
+        flag.set(0)
+        st.clear_stop()
+        call.launch(st.ctx(max_workgroups=64, poll_every=1))
+        assert same(call.left(), want), groups

@@ -22,3 +22,10 @@ def test_conv_prologue_arithmetic(tmp_path):
                     os.path.join(ROOT, "tests", "conv_addr_check.cpp")], check=True)
     out = subprocess.run([exe], check=True, capture_output=True, text=True).stdout
     assert out.startswith("ok "), out
+
+
+def test_tiles_that_are_not_alike_are_dealt_out(tmp_path):
+    exe = str(tmp_path / "dealt_check")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I" + os.path.join(ROOT, "include"), "-o", exe, os.path.join(ROOT, "tests", "dealt_check.cpp")], check=True)
+    out = subprocess.run([exe], check=True, capture_output=True, text=True).stdout
+    assert out.startswith("ok "), out
