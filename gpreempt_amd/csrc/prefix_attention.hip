@@ -296,7 +296,8 @@ static int plan_prefix(const gp_prefix_attention_params *p, PrefixPlan *pl) {
     // 4, 8, 16 and 32 tiles of shared keys to a tile of own ones, or to half a compute unit: 63 sequences of up to 100 own keys, e4m3, 39 / 46, 51 / 53, 73 / 71; 256 of up to 316 78 / 89, 119 / 117, 203 / 183,
     // 385 / 322; 64 of up to 2048 63 / 72, 62 / 75, 80 / 91, 125 / 120; fp16 96 / 104, 86 / 107, 108 / 127, 149 / 157; 256 of up to 1000 141 / 167, 171 / 206, 265 / 270, 471 / 417.
     const long own_tiles = std::max(heads * (few.whole ? q.batch : a.own_x), 2l * device_cus()), per_unit = units * key_tiles <= (9 + most) * own_tiles ? 1 : 2;
-    a.shares = (int)std::max(1l, std::min(per_unit * device_cus() / units, key_tiles / 4));
+    // (two to a compute unit: a place is left for the workgroup that reads the flag, or a part would wait for it: 5 sequences with 4 new tokens behind 131072, bf16, preemptible, 176 -> 148 us, plain 144 level)
+    a.shares = (int)std::max(1l, std::min((per_unit * device_cus() - (per_unit == 2 ? kXcds : 0)) / units, key_tiles / 4));
     a.shared_tiles = (int)(units * a.shares);
     a.shared_slice = (a.shared_tiles + 7) / 8;
     a.own_slice = (int)((heads * a.own_x + 7) / 8);

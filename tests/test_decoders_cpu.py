@@ -137,3 +137,10 @@ def test_the_launcher_chooses_what_is_faster(heads, kv_heads, dim, dtype, shared
         sizes = {v: work_bytes(v, batch, shared, 100, heads, kv_heads, dim, dtype) for v in (gp.PREFIX_AUTO, gp.PREFIX_EACH, gp.PREFIX_TOGETHER)}
         assert sizes[gp.PREFIX_EACH] != sizes[gp.PREFIX_TOGETHER]
         assert sizes[gp.PREFIX_AUTO] == sizes[variant], (batch, sizes)
+
+
+def test_the_shared_tiles_leave_a_place_for_whoever_reads_the_flag():
+    """behind 131072 tokens two workgroups to each of 256 compute units, less one for each XCD: 63 parts of eight heads, of 66 KB each"""
+    part, rows = (128 // 2 + 2) * 256 * 4, 16 * (128 + 2) * 4  # bytes of what 128 rows, and 16, come to
+    others = 69632 + 8 * 5 * rows + 8 * 32 * 2 * rows  # counters, own keys, parts of a sequence that ends within what is shared
+    assert (work_bytes(gp.PREFIX_TOGETHER, 5, 131072, 100, 32, 8, 128, gp.F16) - others) // part == 8 * 63
