@@ -874,3 +874,23 @@ def test_claims_through_counters_have_the_bits_of_a_plain_launch(gp, which):
         st.clear_stop()
         call.launch(st.ctx(max_workgroups=64, poll_every=1))
         assert same(call.left(), want), groups
+
+
+def test_many_sequences_of_which_some_end_within_a_long_beginning(gp):
+    """more sequences than a workgroup's threads look at together, the ones that end early among the last, the first, or nobody"""
+    seqs = long_beginning([2560 + 3 + i % 5 for i in range(600)], None, 128, 2560, gen(100))
+    a = Prefix(gp, "f16", "f16", seqs, 1, 1, 64, True, 101)
+    whole = None
+    for early in ([], [599], [0, 255, 256, 300, 598]):
+        lens = list(seqs.lens)
+        for b in early:
+            seqs.lens[b] = 2500 - b
+        a.dev["kv_len"].copy_(torch.tensor(seqs.lens, dtype=torch.int32))
+        a.clean()
+        a.launch()
+        if early == [599]:  # nobody else's result changes
+            assert torch.equal(a.left()[:599], whole[:599]) and not torch.equal(a.left()[599], whole[599])
+        else:
+            a.check()
+        whole = a.left()
+        seqs.lens = lens
