@@ -223,8 +223,8 @@ __global__ __launch_bounds__(64 * WAVES, MT * NT > 2 ? 2 : 4) void gemm_w4_kerne
 // LDS, 128 values of a row at a time in two buffers.
 //   v_mfma_f32_32x32x16   A as A, W as B: lane l has 8 values of row l % 32.
 // The products are of A with q - z, whole numbers of eight bits and exact; a group's sum meets its scale in fp32: nothing is rounded to 16 bits but the result, as for few rows.
-// Measured (rounding scale * (q - z) to 16 bits in front of the products in brackets): 4001 x 8192 x 8192, bf16, groups of 128: 663 to 706 us, 760 to 810 TFLOP/s (571); fp16 633 (568); of 64 736 (614); of 32 885 to 901 (622);
-// 2048 x 4096 x 4096 82 to 92 (88 to 92), 128 x 22528 x 4096 58 (68).  Tiles of 256 x 256 in eight wavefronts, one to a compute unit: 645, of 64 642, of 32 797, 2048 x 4096 x 4096 174.  Widening W a step
+// Measured (rounding scale * (q - z) to 16 bits in front of the products in brackets): 4001 x 8192 x 8192, bf16, groups of 128: 640 to 706 us, 760 to 840 TFLOP/s (571 to 577); fp16 633 to 667 (568 to 604); of 64 736 to 743 (614 to 633); of 32 861 to 901 (606 to 622);
+// 2048 x 4096 x 4096 82 to 92 (88 to 93), 1024 x 4096 x 4096 62 (72), 128 x 22528 x 4096 58 (68).  Tiles of 256 x 256 in eight wavefronts, one to a compute unit: 645, of 64 642, of 32 797, 2048 x 4096 x 4096 174.  Widening W a step
 // ahead between the matrix instructions: 687.
 constexpr int W4M_ROWS = 128, W4M_NT = 256, W4M_STEP = 128;
 constexpr int W4M_BUFFER = W4M_ROWS * W4M_STEP * 2;  // bytes

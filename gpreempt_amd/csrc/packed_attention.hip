@@ -3,7 +3,7 @@
 // A tile is one head of keys and values and 128 query rows of a sequence that share it (its tokens times the query heads of the head): many_keys in paged_many.hpp,
 // its keys and values from rows of the packed tensors.  Bound as that is, by matrix and vector instructions that seldom overlap.
 //
-// Measured: four sequences of 1024 to 8192 tokens, causal, 32 heads over 8 of 128, bf16: 1438 to 1529 us on different days, 910 to 967 TFLOP/s (a large matrix product: 1150).  37 sequences of 48 to 384, 12 heads of 64, fp16, not
+// Measured: four sequences of 1024 to 8192 tokens, causal, 32 heads over 8 of 128, bf16: 1409 to 1529 us on different days, 910 to 987 TFLOP/s (a large matrix product: 1150).  37 sequences of 48 to 384, 12 heads of 64, fp16, not
 // causal: 28 us for 55 MB: 1332 workgroups of six steps at most, whose beginnings count as much as their steps.  Heads of 64: three workgroups to a compute unit (32 registers less than the compiler takes by
 // itself): 973 -> 920 us for four sequences up to 8192, with four 1270.
 #include "paged_many.hpp"

@@ -6,8 +6,10 @@
 // Both are tiles of one launch, the shared ones first, and leave a reference, a sum and a weighted sum per row.  The parts of the shared keys are joined two by two, and whoever comes second to a
 // sequence's rows, with what its own or what the shared keys come to, joins both; in one order whoever that is.
 //
-// Measured (32 heads of queries over 8 of 128; each sequence for itself in brackets): 64 sequences behind 8192 tokens, up to 2048 of their own, e4m3: 62 us (152) for 169 MB; 5 with 4 new tokens behind 131072, bf16:
-// 143 us (397), 100 of it 128-row tiles with 80 rows and 30 parts that meet over six levels; 256 behind 16384, fp16: 124 us (1879), 560 TFLOP/s.  A part's result, 66 KB, is written in 2 us and read in 3.
+// Measured, on different days (32 heads of queries over 8 of 128; each sequence for itself in brackets): 64 sequences behind 8192 tokens, up to 2048 of their own, e4m3: 61 to 64 us (152) for 169 MB; 5 with 4 new
+// tokens behind 131072, bf16: 143 to 146 us (397), some 100 us of it tiles of which 80 of 128 rows are there, and some 30 us in which 63 parts meet over six levels; 256 behind 16384, fp16: 124 to 134 us (1879), 520 to
+// 560 TFLOP/s.  A part's result, 66 KB, is written in 2 us and read in 3.  16 sequences with up to 8 new tokens, which are 32 rows to a head, behind 16384: bf16 79 us, e4m3 68, 31 and 65 registers of a lane in scratch
+// memory.  Preemptible, with nothing to stop for: 68 us (65 plain, calls one by one), 148 (147), 181 (139: more tiles than workgroups, which claim them, and 70 registers in scratch memory).
 #include <algorithm>
 #include "paged_few.hpp"
 #include "paged_many.hpp"
