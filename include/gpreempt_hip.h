@@ -643,7 +643,8 @@ typedef struct gp_prefix_attention_params {
     gp_paged_attention_params attention;
     int shared_len;
     const int *shared_table;
-    int variant;  /* 0 = chosen by the launcher: once for all sequences together, or for each as gp_launch_paged_attention does, which is quicker where little is shared by few */
+    int variant;  /* 0 = chosen by the launcher: once for all sequences together, or for each as gp_launch_paged_attention does, which is quicker where little is shared by few.  (Where max_len or
+                   * the table ends in front of shared_len no sequence sees all of it: for each, whatever is asked for.) */
 } gp_prefix_attention_params;
 int gp_prefix_attention_work_bytes(const gp_prefix_attention_params *p, size_t *bytes);
 int gp_launch_prefix_attention(const gp_prefix_attention_params *p, const gp_preempt_ctx *ctx, gp_stream s, gp_launch_info *info);
